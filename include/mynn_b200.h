@@ -538,6 +538,39 @@ int mynn_b200_dense_matmul_ex(void *stream, void *out, const void *act, const vo
 int mynn_b200_moe_matmul(void *stream, void *out, const void *act, const void *w, void *route_workspace, void *gather_workspace, int M, int N,
                          int K, int experts, int top, int gather, int glu, int dtype, int out_dtype, int32_t *status);
 
+/* ---------------------------------------------------------------------------------------------
+ * Paged caches and drafted tokens.  No counterpart in the engine, whose caches are reserved in full and whose batch has one length.
+ *
+ * A paged cache is two tensors [pages, Hkv, page, D] (keys, values) that sequences share.  Position j of sequence b lies in row j % page of page
+ * block_table[b, j / page]; block_table int32 [B, table_pages] may hold any number outside 0 .. pages - 1 where the sequence has no page: nothing is
+ * written there, and its positions are not seen.  lengths int32 [B] counts the positions of each sequence WITH its new tokens, counts int32 [B] (may be
+ * NULL: S each) the new tokens, of which there are places for S: token s < counts[b] is at position lengths[b] - counts[b] + s.  Both are read on the device, where
+ * counts are taken as 0 .. S and lengths as at least 0; positions behind the block table hold nothing.  A sequence of count 0 is idle.  pages * Hkv * page < 2^31. */
+/* proj [B, S, (Hq + 2 Hkv) * D] (q, k, v heads) of the new tokens: rotation of the first rot_dims dimensions of every q and k head at f32 table
+ * rows [positions, rot_dims / 2] (halves: dimension i with i + rot_dims / 2, else 2i with 2i + 1), with qk_norm v / sqrt(mean(v^2) + eps)
+ * afterwards; q to q_out [B, Hq, S, D] (zeros where there is no token), k and v to the pages.  A token at a position that is negative, behind the block table
+ * or, with rot_dims, behind the rotation table is no token.  Sequences do not share the pages they append to. */
+int mynn_b200_paged_rotary_append(void *stream, void *q_out, void *k_pages, void *v_pages, const void *proj, const float *cos_table,
+                                  const float *sin_table, const int32_t *lengths, const int32_t *counts, const int32_t *block_table, int B, int S,
+                                  int Hq, int Hkv, int D, int rot_dims, int halves, int qk_norm, float eps, int page, int pages, int table_pages,
+                                  int positions, int dtype);
+/* out [B, S, Hq, D] = softmax(scale * q k^T) v over the cache, q [B, Hq, S, D].  A query at position i sees position j <= i when window <= 0, or
+ * i - j < window, or j < sinks (pages that hold no such position may have been given back: their entries are not read).  softcap > 0: scores go through
+ * softcap * tanh(. / softcap).  Rows that see nothing are zeros.  D <= 256.  workspace: scratch of mynn_b200_paged_attention_workspace_bytes
+ * (of the current device), 16-byte aligned; nothing in it outlives the call. */
+size_t mynn_b200_paged_attention_workspace_bytes(int B, int S, int Hq, int Hkv, int D, int page, int table_pages);
+int mynn_b200_paged_attention(void *stream, void *out, const void *q, const void *k_pages, const void *v_pages, const int32_t *block_table,
+                              const int32_t *lengths, const int32_t *counts, float scale, float softcap, int window, int sinks, int B, int S, int Hq,
+                              int Hkv, int D, int page, int pages, int table_pages, int dtype, void *workspace, size_t workspace_bytes);
+/* Drafted tokens int32 [B, K] (counts int32 [B] of them, NULL: K each; taken as at most K) against the target's probabilities p = target [B, K + 1, V] at the
+ * K + 1 positions and the draft's q = draft [B, K, V] they were drawn from (NULL: they were not drawn but certain, q = 1 at the token), both in
+ * dtype.  Token i is accepted while accept[b, i] * q_i(x_i) < p_i(x_i) (a token outside the vocabulary is not); accepted_out int32 [B] counts
+ * them, n.  tokens_out int32 [B, K + 1]: the accepted ones, then one token drawn from max(p_n - q_n, 0), behind all of them from p_n, then -1.  The draw
+ * is the first token whose running sum exceeds sample[b] times the whole sum, in 64 bits; where p_n - q_n leaves nothing it is from p_n, and where
+ * p_n has nothing either the token is -1.  accept f32 [B, K], sample f32 [B] in [0, 1). */
+int mynn_b200_verify_draft(void *stream, int32_t *tokens_out, int32_t *accepted_out, const void *target, const void *draft, const int32_t *tokens,
+                           const int32_t *counts, const float *accept, const float *sample, int B, int K, int V, int dtype);
+
 /* How many CTAs the 16-bit decode attention kernel lets share the kv rows of one (batch, kv head) pair, given an upper bound
  * of the rows and the number of CTAs of that kernel an SM holds (2 for the ring form at head_dim 128, else 4).  This is the
  * operator's plan; a model's step of few pairs takes CTAs of more warps and fewer of them.  Pure host

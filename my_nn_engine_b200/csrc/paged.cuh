@@ -1,0 +1,125 @@
+// Paged caches: which cached rows the queries of a sequence see, how those rows are dealt out to the CTAs of a launch, and the launch
+// parameters that the kernels of paged_attention.cu share.
+//
+// A cache is pages [pages, Hkv, page, D]; position j of sequence b lies in row j % page of page table[b, j / page].  lengths[b] counts the positions
+// of the sequence with its new tokens, counts[b] the new tokens: query s of the sequence sits at position lengths[b] - counts[b] + s.
+//
+// Sequences of a batch have lengths of their own, so a fixed number of CTAs per sequence would leave most of the GPU waiting for the longest one.
+// The visible rows are cut into tiles of kPagedTile positions, and all tiles of all (sequence, kv head) pairs, one pair behind the other, are
+// dealt out evenly: each CTA takes one run of `share` tiles, which may end one pair, hold a few whole ones and begin another.  A pair that
+// lies in one CTA is finished there; the parts of the others go to a workspace and are joined by a second kernel.  A CTA has at most two parts:
+// the pair its run begins inside of (slot 0) and the pair it ends inside of (slot 1).  The lengths are on the device, so every CTA works out the division itself.
+#pragma once
+#include <limits.h>
+
+#include "common.cuh"
+
+namespace mynn {
+
+constexpr int kPagedTile = 16;
+constexpr int kPagedWindow = INT_MAX - (1 << 17);
+
+struct PagedAttention {
+    void *out;
+    const void *q, *k, *v;
+    const int32_t *table, *lengths, *counts;  // counts null: S each
+    float scale, softcap;
+    int window, sinks;  // window: at most kPagedWindow (positions are below 2^31, and new tokens may lie before the first one)
+    int B, S, Hq, G, group, D;
+    int page, pages, width;  // rows of a page, pages of the cache, pages in a row of the table
+    int row_blocks, block_rows;  // the group * S query rows of a pair, row r = head * S + s, in blocks
+    int round;                   // shares are multiples of it: the tiles that the warps of a CTA take at a time
+    float *ws;                   // [row block][CTA][2] parts of block_rows * (D + 2) floats: rows, then maxima, then sums
+};
+
+// What the new queries of a sequence see: the tiles of the first tokens, then those from the oldest query's window on.
+struct PagedSpan {
+    int len, count, rows;         // rows: positions that the block table has entries for
+    int sink_tiles, skip, tiles;  // skip: tiles between the two parts
+    __device__ __forceinline__ int base(int t) const { return (t + (t < sink_tiles ? 0 : skip)) * kPagedTile; }
+};
+
+__device__ __forceinline__ PagedSpan paged_span(const PagedAttention &p, int b) {
+    PagedSpan s;
+    s.len = max(p.lengths[b], 0);
+    s.rows = min(s.len, p.width * p.page);
+    s.count = p.counts ? min(max(p.counts[b], 0), p.S) : p.S;
+    const int oldest = s.len - s.count;
+    const int all = (s.rows + kPagedTile - 1) / kPagedTile;
+    const int lo = p.window > 0 ? min(max(0, oldest - p.window + 1) / kPagedTile, all) : 0;  // the tile that the windows begin in
+    s.sink_tiles = min((min(p.sinks, s.rows) + kPagedTile - 1) / kPagedTile, lo);
+    s.skip = lo - s.sink_tiles;
+    s.tiles = s.count > 0 ? all - s.skip : 0;
+    return s;
+}
+
+// Does query s (position oldest + s) see position j?
+__device__ __forceinline__ bool paged_sees(const PagedAttention &p, const PagedSpan &sp, int s, int j) {
+    const int at = sp.len - sp.count + s;
+    return s < sp.count && j <= at && (p.window <= 0 || at - j < p.window || j < p.sinks);
+}
+
+// The row of the cache that holds position j of sequence b for kv head h; -1 where no query sees it or the table names no page.
+__device__ __forceinline__ int paged_row(const PagedAttention &p, const PagedSpan &sp, int b, int h, int j) {
+    if (j >= sp.rows || (p.window > 0 && sp.len - sp.count - j >= p.window && j >= p.sinks)) return -1;
+    const int i = j / p.page, pg = p.table[(size_t)b * p.width + i];
+    return (unsigned)pg < (unsigned)p.pages ? (pg * p.G + h) * p.page + (j - i * p.page) : -1;
+}
+// All queries of the sequence see all of the tile (what a tile holds that only some see has to be kept from the others, not only weighted by zero: it may
+// be infinite).
+__device__ __forceinline__ bool paged_tile_full(const PagedAttention &p, const PagedSpan &sp, int base) {
+    return base + kPagedTile - 1 <= sp.len - sp.count && (p.window <= 0 || sp.len - 1 - base < p.window || base + kPagedTile <= p.sinks);
+}
+
+struct PagedShare {
+    long long total, share;
+    int b, h, t;  // where this CTA's run begins (b == B: it has none)
+};
+
+__device__ __forceinline__ long long paged_share(long long total, int ctas, int round) {
+    const long long s = (total + ctas - 1) / ctas;
+    return max((s + round - 1) / round, 1ll) * round;
+}
+
+// Called by all threads of a CTA: the total number of tiles and the place of tile cta * share.  Each thread sums a run of sequences.
+template <int THREADS>
+__device__ __forceinline__ PagedShare paged_find(const PagedAttention &p, int cta, int ctas) {
+    __shared__ long long warp_sums[THREADS / 32];
+    __shared__ PagedShare found;
+    const int per = (p.B + THREADS - 1) / THREADS, b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    long long mine = 0;
+    for (int b = b0; b < b1; b++) mine += (long long)paged_span(p, b).tiles * p.G;
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+    }
+    if (lane == 31) warp_sums[warp] = incl;
+    __syncthreads();
+    long long before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; w++) {
+        if (w < warp) before += warp_sums[w];
+        total += warp_sums[w];
+    }
+    const long long share = paged_share(total, ctas, p.round), begin = cta * share, end = before + incl;
+    long long at = end - mine;
+    if (threadIdx.x == 0 && begin >= total) found = {total, share, p.B, 0, 0};
+    if (begin >= at && begin < end) {
+        for (int b = b0; b < b1; b++) {
+            const int n = paged_span(p, b).tiles;
+            if (begin < at + (long long)n * p.G) {
+                const long long rest = begin - at;
+                found = {total, share, b, (int)(rest / n), (int)(rest % n)};
+                break;
+            }
+            at += (long long)n * p.G;
+        }
+    }
+    __syncthreads();
+    return found;
+}
+
+}  // namespace mynn

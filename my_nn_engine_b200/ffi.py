@@ -124,6 +124,10 @@ SIGNATURES = {
     "mynn_b200_moe_route": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int]),
     "mynn_b200_dense_matmul": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "mynn_b200_moe_matmul": (c_int, [c_void_p] * 6 + [c_int] * 9 + [c_void_p]),
+    "mynn_b200_paged_rotary_append": (c_int, [c_void_p] * 10 + [c_int] * 8 + [c_float] + [c_int] * 5),
+    "mynn_b200_paged_attention_workspace_bytes": (c_size_t, [c_int] * 7),
+    "mynn_b200_paged_attention": (c_int, [c_void_p] * 8 + [c_float, c_float] + [c_int] * 11 + [c_void_p, c_size_t]),
+    "mynn_b200_verify_draft": (c_int, [c_void_p] * 9 + [c_int] * 4),
     "mynn_b200_model_tp_export": (c_int, [c_void_p, c_void_p]),
     "mynn_b200_model_tp_attach": (c_int, [c_void_p, c_void_p]),
     "mynn_b200_attention_decode_splits": (c_int, [c_int, c_int, c_int, c_int]),

@@ -7,6 +7,7 @@ tensors and the call raises otherwise.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 
@@ -604,3 +605,107 @@ def dense_matmul_ex(act, w, act_fn=ffi.ACT_NONE, f32_columns=0, block=0, status=
     ffi.check(ffi.lib().mynn_b200_dense_matmul_ex(_stream(), _ptr(out), _ptr(act), _ptr(w), M, N, K, _dt(act), _dt(out), act_fn, _ptr(extra),
                                                   main if f32_columns else 0, block, M * block, 0, block, 1, 0, 0, _ptr(status)))
     return (out, extra) if f32_columns else out
+
+
+# ---- paged caches and drafted tokens ----------------------------------------------------------------------------------
+def _int32(name, t, shape):
+    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != shape):
+        raise ValueError(f"{name} must be an int32 tensor of shape {shape}, not {t.dtype} {tuple(t.shape)}")
+    return t
+
+
+def _on_device_of(first, *others):
+    """The tensors' device as a context, after a check that it is one device: the operators of this section run on their tensors' device and its
+    current stream, whichever device is current."""
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device}")
+    if not first.is_cuda:
+        raise ValueError("mynn_b200 operators need CUDA tensors (there is no CPU path)")
+    return _HERE if _device is not None and first.device.index == _device() else torch.cuda.device(first.device)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _pages(k_pages, v_pages, dtype, block_table, lengths, counts, batch):
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError(f"k_pages and v_pages must have one shape [pages, kv heads, page, D], not {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    if k_pages.dtype != dtype or v_pages.dtype != dtype:
+        raise TypeError("the pages must have the dtype of the queries")
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be [B, pages of a sequence]")
+    _int32("block_table", block_table, (batch, block_table.shape[1]))
+    _int32("lengths", lengths, (batch,))
+    _int32("counts", counts, (batch,))
+
+
+def paged_rotary_append(proj, lengths, block_table, k_pages, v_pages, heads, cos=None, sin=None, counts=None, halves=True, qk_norm=False, eps=1e-6):
+    """``rotary_append`` over a paged cache: proj [B, S, (heads + 2 G) D] of the new tokens -> q [B, heads, S, D], rotated and (``qk_norm``) normed per head; the
+    new keys (likewise) and values go to the pages [pages, G, page, D] in place.  Sequence b has ``lengths[b]`` positions with its new tokens, of
+    which it has ``counts[b]`` (None: S); token s is at position lengths[b] - counts[b] + s, in row position % page of page block_table[b, position
+    // page].  A place without a token gets a zero query, a position without a page (an entry outside the cache, such as -1) is not stored.  lengths, counts,
+    block_table: int32 CUDA tensors.  cos / sin: f32 [positions, rotated / 2], None: no rotation."""
+    B, S, C = proj.shape
+    _pages(k_pages, v_pages, proj.dtype, block_table, lengths, counts, B)
+    n, G, page, D = k_pages.shape
+    if C != (heads + 2 * G) * D:
+        raise ValueError(f"proj has {C} columns, {heads} query and 2 x {G} cached heads of {D} need {(heads + 2 * G) * D}")
+    if (cos is None) != (sin is None) or (cos is not None and (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape)):
+        raise ValueError("cos and sin must be f32 tensors of one shape [positions, rotated / 2], or both None")
+    with _on_device_of(proj, lengths, block_table, k_pages, v_pages, cos, sin, counts):
+        q = torch.empty(B, heads, S, D, dtype=proj.dtype, device=proj.device)
+        ffi.check(ffi.lib().mynn_b200_paged_rotary_append(
+            _stream(), _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(proj), _ptr(cos), _ptr(sin), _ptr(lengths), _ptr(counts), _ptr(block_table), B, S, heads, G, D,
+            0 if cos is None else 2 * cos.shape[1], int(halves), int(qk_norm), eps, page, n, block_table.shape[1], 0 if cos is None else cos.shape[0], _dt(proj)))
+    return q
+
+
+@functools.lru_cache(maxsize=4096)
+def _paged_ws_bytes(device, *sizes):
+    return ffi.lib().mynn_b200_paged_attention_workspace_bytes(*sizes)
+
+
+def paged_attention(q, k_pages, v_pages, block_table, lengths, scale, counts=None, window=0, sinks=0, softcap=0.0, out=None):
+    """Attention of the new tokens of each sequence over a paged cache that holds them already (see ``paged_rotary_append`` for lengths, counts,
+    block_table): q [B, Hq, S, D], one query per sequence or a few drafted ones -> [B, S, Hq, D].  With ``window`` a query sees the last ``window`` positions
+    up to its own, and the first ``sinks`` ones of the sequence; pages that hold none of these may have been given back.  softcap: cap on the
+    scores (0: none).  A query that sees nothing (an idle sequence, a place without a token) gives zeros."""
+    B, Hq, S, D = q.shape
+    _pages(k_pages, v_pages, q.dtype, block_table, lengths, counts, B)
+    n, G, page, width = *k_pages.shape[:3], block_table.shape[1]
+    if k_pages.shape[3] != D:
+        raise ValueError(f"heads of {D} over a cache of heads of {k_pages.shape[3]}")
+    with _on_device_of(q, k_pages, v_pages, block_table, lengths, counts, out):
+        if out is None:
+            out = torch.empty(B, S, Hq, D, dtype=q.dtype, device=q.device)
+        elif out.shape != (B, S, Hq, D) or out.dtype != q.dtype:
+            raise ValueError(f"out must be {(B, S, Hq, D)} in the dtype of the queries")
+        # not kept between calls: two captured graphs, or two streams, never share it
+        size = _paged_ws_bytes(q.device.index, B, S, Hq, G, D, page, width)
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+        ffi.check(ffi.lib().mynn_b200_paged_attention(_stream(), _ptr(out), _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(block_table), _ptr(lengths), _ptr(counts),
+                                                      scale, softcap, window, sinks, B, S, Hq, G, D, page, n, width, _dt(q), _ptr(ws), size))
+    return out
+
+
+def verify_draft(target, tokens, accept, sample, draft=None, counts=None):
+    """Drafted tokens int32 [B, K] against the target's probabilities [B, K + 1, V] at their positions and the one behind, with the probabilities [B, K, V] that
+    they were drawn from (None: they were not drawn, a lookup or a greedy draft).  Token i stands while accept[b, i] * q_i < p_i; behind the standing
+    ones comes one drawn from max(p - q, 0) with sample[b], or from p behind all of them.  accept f32 [B, K] and sample f32 [B]: random numbers in
+    [0, 1).  counts int32 [B]: drafted tokens of each sequence, None: K.  Returns (tokens int32 [B, K + 1], -1 behind the drawn one; number of standing
+    tokens int32 [B])."""
+    B, K1, V = target.shape
+    K = K1 - 1
+    _int32("tokens", tokens, (B, K))
+    _int32("counts", counts, (B,))
+    if draft is not None and (draft.dtype != target.dtype or tuple(draft.shape) != (B, K, V)):
+        raise ValueError(f"draft must be {(B, K, V)} in the dtype of target")
+    if accept.dtype != torch.float32 or tuple(accept.shape) != (B, K) or sample.dtype != torch.float32 or tuple(sample.shape) != (B,):
+        raise ValueError(f"accept and sample must be f32 tensors of shapes {(B, K)} and {(B,)}")
+    with _on_device_of(target, tokens, accept, sample, draft, counts):
+        out = torch.empty(B, K1, dtype=torch.int32, device=target.device)
+        taken = torch.empty(B, dtype=torch.int32, device=target.device)
+        ffi.check(ffi.lib().mynn_b200_verify_draft(_stream(), _ptr(out), _ptr(taken), _ptr(target), _ptr(draft), _ptr(tokens), _ptr(counts), _ptr(accept),
+                                                   _ptr(sample), B, K, V, _dt(target)))
+    return out, taken
