@@ -192,6 +192,343 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32) paged_attention_plain_ke
     }
 }
 
+// ---- 16-bit caches on the tensor cores --------------------------------------------------------------------------------
+// Bound by the one pass over the cache.  A team of RW warps takes tiles of 16 positions: cp.async brings a tile's rows, wherever their pages lie, to a ring of
+// STAGES tiles in shared memory, each warp a share of the rows, and each warp then multiplies the whole tile with 8 NT query rows of its own, so that a row of the
+// cache is read once for up to 64 query rows (all heads of a group, all drafts).  Both products are mma.m16n8k16 on fragments that are 16-byte pieces of
+// the rows, as in the attention over contiguous caches: S = Q K^T with the dimensions of a step permuted, O^T = V^T P^T with pairs of positions put together
+// by byte permutes; weights enter as a 16-bit part and its remainder (16 bits in all), scores, maxima and sums are f32.  D is padded to DP with zeros, on the chip
+// only.
+template <int DP, int NT, int RW>
+struct MmaShape {
+    static constexpr int W = 4, TEAMS = W / RW, ROWS = 8 * NT * RW;
+    static constexpr int TILE_BYTES = 2 * kPagedTile * DP * 2;
+    static constexpr int CTAS = DP > 128 ? 1 : 2;  // per SM
+    static constexpr int STAGES = (CTAS == 2 ? 96 : 192) * 1024 / TEAMS / TILE_BYTES;
+    static constexpr int ACC = DP / 16 * NT * 4;   // accumulators of a lane
+    static constexpr int PEERS = TEAMS == 1 ? 0 : W / 2;
+    static constexpr size_t SMEM = (size_t)TEAMS * STAGES * TILE_BYTES + (size_t)PEERS * ACC * 32 * 4;
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Where a 16-byte piece c of a row lies among the eight of its 128 bytes: two neighbouring rows' pieces t .. t + 3 (keys) and four even or odd rows' pieces 2 i,
+// 2 i + 1 (values) are in different banks.
+__device__ __forceinline__ int paged_swizzle(int row, int c) { return c ^ (row & 6) ^ ((row & 1) << 2); }
+
+template <typename T>
+__device__ __forceinline__ bool has_special(uint32_t x) {  // infinity or NaN in one of two 16-bit numbers
+    constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    return (x & e) == e || (x >> 16 & e) == e;
+}
+
+template <typename T, int DP, int NT, int RW>
+__global__ void __launch_bounds__(128, MmaShape<DP, NT, RW>::CTAS) paged_attention_mma_kernel(const PagedAttention p) {
+    using Shape = MmaShape<DP, NT, RW>;
+    constexpr int W = Shape::W, TEAMS = Shape::TEAMS, STAGES = Shape::STAGES, TILE = kPagedTile, KCH = DP / 32, VH = DP / 64, CPR = DP / 8;
+    constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+    extern __shared__ __align__(128) uint8_t raw[];
+    __shared__ uint32_t there[W][STAGES];       // which rows of a tile exist
+    __shared__ float peer_m[W][16], peer_l[W][16];
+    pdl_trigger();
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, team = warp / RW, member = warp % RW;
+    const int cta = blockIdx.x, ctas = gridDim.x, D = p.D, R = p.group * p.S, r0 = blockIdx.y * Shape::ROWS;
+    uint8_t *ring = raw + (size_t)team * STAGES * Shape::TILE_BYTES;
+    float4 *peers = reinterpret_cast<float4 *>(raw + (size_t)TEAMS * STAGES * Shape::TILE_BYTES);
+    const uint32_t ring_at = smem_u32(ring);
+    const PagedShare run = paged_find<W * 32>(p, cta, ctas);
+    for (int b = cta; b < p.B; b += ctas)  // sequences that see nothing at all belong to no run
+        if (blockIdx.y == 0 && paged_span(p, b).tiles == 0)
+            for (size_t n = (size_t)p.S * p.Hq * D / 8, i = threadIdx.x; i < n; i += W * 32) reinterpret_cast<uint4 *>(p.out)[b * n + i] = make_uint4(0, 0, 0, 0);
+    auto team_sync = [&]() {
+        if constexpr (RW == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(RW * 32) : "memory");
+    };
+    // the rows of this lane: 0 (and 1) are accumulator row g (and g + 8), mine[2 n + e] are the columns 8 n + 2 t + e of the second product
+    auto row_index = [&](int i) { return r0 + member * 8 * NT + i; };
+    const float unit = p.scale * kLog2e;
+    int b = run.b, h = run.h, t0 = run.t;
+    long long left = run.share;
+    for (bool first = true; b < p.B && left > 0; first = false) {
+        const PagedSpan sp = paged_span(p, b);
+        if (sp.tiles == 0) {
+            b++;
+            h = t0 = 0;
+            continue;
+        }
+        const int t1 = (int)min((long long)sp.tiles, t0 + left);
+        const int mine = t0 + team < t1 ? (t1 - t0 - team + TEAMS - 1) / TEAMS : 0;
+        const int oldest = sp.len - sp.count;
+        // last position that a row sees, -1: the row is no query
+        auto last_seen = [&](int i) {
+            const int r = row_index(i);
+            return r < R && r % p.S < sp.count ? oldest + r % p.S : -1;
+        };
+        int at[NT];
+#pragma unroll
+        for (int n = 0; n < NT; n++) at[n] = last_seen(8 * n + g);
+        auto sees = [&](int last, int j) { return j <= last && (p.window <= 0 || last - j < p.window || j < p.sinks); };
+        auto row_of = [&](int j) { return j < mine ? paged_row(p, sp, b, h, sp.base(t0 + team + TEAMS * j) + (lane & 15)) : -1; };
+        auto issue = [&](int j, int row) {
+            const int stage = j % STAGES;
+            const uint32_t to = ring_at + stage * Shape::TILE_BYTES;
+            const uint32_t exist = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+            if (lane == 0) there[warp][stage] = exist;
+            if (j < mine) {
+#pragma unroll
+                for (int i = 0; i < TILE * CPR / 32 / RW; i++) {
+                    const int idx = (i * RW + member) * 32 + lane, r = idx / CPR, c = idx % CPR;
+                    const int from = __shfl_sync(0xffffffffu, row, r);
+                    const size_t src = (size_t)max(from, 0) * D + (8 * c < D ? 8 * c : 0);
+                    const bool in = from >= 0 && 8 * c < D;
+                    const uint32_t dst = to + r * (DP * 2) + (c >> 3) * 128 + paged_swizzle(r, c & 7) * 16;
+                    copy16_at(dst, reinterpret_cast<const T *>(p.k) + src, in);
+                    copy16_at(dst + TILE * DP * 2, reinterpret_cast<const T *>(p.v) + src, in);
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        team_sync();  // the ring is free
+#pragma unroll
+        for (int j = 0; j < STAGES - 1; j++) issue(j, row_of(j));
+        int next = row_of(STAGES - 1);
+
+        uint2 qa[NT][2 * KCH];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const int r = min(row_index(8 * n + g), R - 1);
+            const T *qr = reinterpret_cast<const T *>(p.q) + (((size_t)b * p.Hq + h * p.group + r / p.S) * p.S + r % p.S) * D;
+#pragma unroll
+            for (int i = 0; i < 2 * KCH; i++) {
+                const int d = 8 * (t + 4 * (i >> 1)) + 4 * (i & 1);
+                qa[n][i] = at[n] >= 0 && d < D ? *reinterpret_cast<const uint2 *>(qr + d) : make_uint2(0u, 0u);
+            }
+        }
+        float o[VH * 4][NT][4], m[NT], l[NT];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            m[n] = -INFINITY, l[n] = 0.f;
+#pragma unroll
+            for (int i = 0; i < VH * 4; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[i][n][e] = 0.f;
+        }
+#pragma unroll 1
+        for (int j = 0; j < mine; j++) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+            team_sync();  // tile j is here, and tile j - 1 is done with
+            issue(j + STAGES - 1, next);
+            next = row_of(j + STAGES);
+            const uint8_t *K = ring + (j % STAGES) * Shape::TILE_BYTES, *V = K + TILE * DP * 2;
+            const int base = sp.base(t0 + team + TEAMS * j);
+            const uint32_t exist = there[warp][j % STAGES];
+            // ---- S = Q K^T: x[n][2 c + e] is row 8 n + g, position base + 8 c + 2 t + e ----
+            float x[NT][4];
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < KCH; i++) {
+                    const uint4 kr = *reinterpret_cast<const uint4 *>(K + (8 * c + g) * (DP * 2) + (i >> 1) * 128 + paged_swizzle(g, t + 4 * (i & 1)) * 16);
+                    if constexpr (NT == 1) {
+                        mma_kv<T>(acc, qa[0][2 * i].x, 0u, qa[0][2 * i].y, 0u, kr.x, kr.y);
+                        mma_kv<T>(acc, qa[0][2 * i + 1].x, 0u, qa[0][2 * i + 1].y, 0u, kr.z, kr.w);
+                    } else {
+                        mma_kv<T>(acc, qa[0][2 * i].x, qa[1][2 * i].x, qa[0][2 * i].y, qa[1][2 * i].y, kr.x, kr.y);
+                        mma_kv<T>(acc, qa[0][2 * i + 1].x, qa[1][2 * i + 1].x, qa[0][2 * i + 1].y, qa[1][2 * i + 1].y, kr.z, kr.w);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n++) x[n][2 * c] = acc[2 * n], x[n][2 * c + 1] = acc[2 * n + 1];
+            }
+            const bool full = exist == 0xffffu && (p.S == 1 || paged_tile_full(p, sp, base));
+            uint32_t hi[NT][2], lo[NT][2];
+            float keep[NT];
+            bool moved = false;
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (p.softcap > 0.f) x[n][i] = kLog2e * fast_soft_cap(x[n][i] * p.scale, p.softcap);
+                    else x[n][i] *= unit;
+                    const int bit = 8 * (i >> 1) + 2 * t + (i & 1);
+                    if (!full && !((exist >> bit & 1) && sees(at[n], base + bit))) x[n][i] = -INFINITY;
+                    top = fmaxf(top, x[n][i]);
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float now = fmaxf(m[n], top), ref = merge_reference(now);
+                keep[n] = exp2_approx(m[n] - ref);
+                moved |= now > m[n];
+                m[n] = now;
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[n][i] = exp2_approx(x[n][i] - ref);
+                l[n] = l[n] * keep[n] + ((x[n][0] + x[n][1]) + (x[n][2] + x[n][3]));  // of this lane's positions
+                split_pack<T>(x[n][0], x[n][1], hi[n][0], lo[n][0]);
+                split_pack<T>(x[n][2], x[n][3], hi[n][1], lo[n][1]);
+            }
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const float k0 = __shfl_sync(0xffffffffu, keep[n], 8 * t), k1 = __shfl_sync(0xffffffffu, keep[n], 8 * t + 4);
+#pragma unroll
+                    for (int i = 0; i < VH * 4; i++) o[i][n][0] *= k0, o[i][n][1] *= k1, o[i][n][2] *= k0, o[i][n][3] *= k1;
+                }
+            }
+            // ---- O^T += V^T P^T: o[4 v + i][n] is dimensions 64 v + 8 g + 2 i (registers 0, 1) and + 1 (2, 3) of rows 8 n + 2 t and + 1 ----
+            bool special = false;
+#pragma unroll
+            for (int v = 0; v < VH; v++) {
+                uint32_t vr[4][4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int row = 2 * t + (r & 1) + 8 * (r >> 1);
+                    const uint4 u = *reinterpret_cast<const uint4 *>(V + row * (DP * 2) + v * 128 + paged_swizzle(row, g) * 16);
+                    vr[r][0] = u.x, vr[r][1] = u.y, vr[r][2] = u.z, vr[r][3] = u.w;
+                }
+                if (!full && p.S > 1) {
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) special |= has_special<T>(vr[r][i]);
+                    special = __any_sync(0xffffffffu, special);
+                }
+                if (special) {
+                    // A value that is no number, which not every row sees: position by position, added only where it is seen.  (What stands in
+                    // `special` from the slab in front does no harm.)
+#pragma unroll 1
+                    for (int k = 0; k < TILE; k++) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            uint32_t one[4];
+#pragma unroll
+                            for (int r = 0; r < 4; r++) one[r] = 2 * t + (r & 1) + 8 * (r >> 1) == k ? vr[r][i] : 0u;
+                            const uint32_t a0 = __byte_perm(one[0], one[1], 0x5410u), a1 = __byte_perm(one[0], one[1], 0x7632u);
+                            const uint32_t a2 = __byte_perm(one[2], one[3], 0x5410u), a3 = __byte_perm(one[2], one[3], 0x7632u);
+#pragma unroll
+                            for (int n = 0; n < NT; n++) {
+                                float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                                mma_kv<T>(acc, a0, a1, a2, a3, hi[n][0], hi[n][1]);
+                                mma_kv<T>(acc, a0, a1, a2, a3, lo[n][0], lo[n][1]);
+                                const bool s0 = (exist >> k & 1) && sees(last_seen(8 * n + 2 * t), base + k), s1 = (exist >> k & 1) && sees(last_seen(8 * n + 2 * t + 1), base + k);
+                                float(&to)[4] = o[4 * v + i][n];
+                                if (s0) to[0] += acc[0], to[2] += acc[2];
+                                if (s1) to[1] += acc[1], to[3] += acc[3];
+                            }
+                        }
+                    }
+                    continue;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t a0 = __byte_perm(vr[0][i], vr[1][i], 0x5410u), a1 = __byte_perm(vr[0][i], vr[1][i], 0x7632u);
+                    const uint32_t a2 = __byte_perm(vr[2][i], vr[3][i], 0x5410u), a3 = __byte_perm(vr[2][i], vr[3][i], 0x7632u);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        mma_kv<T>(o[4 * v + i][n], a0, a1, a2, a3, hi[n][0], hi[n][1]);
+                        mma_kv<T>(o[4 * v + i][n], a0, a1, a2, a3, lo[n][0], lo[n][1]);
+                    }
+                }
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
+            l[n] += __shfl_xor_sync(0xffffffffu, l[n], 2);
+            if (at[n] < 0) m[n] = -INFINITY, l[n] = 0.f;  // a row that is no query, which tiles that all see are not masked for
+        }
+        // ---- the teams meet: half of them hand their sums to the other half, register by register ----
+#pragma unroll
+        for (int half = TEAMS / 2; half > 0; half >>= 1) {
+            const int slot = (team - half) * RW + member;
+            if (team >= half && team < 2 * half) {
+#pragma unroll
+                for (int i = 0; i < VH * 4; i++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++) peers[(slot * (Shape::ACC / 4) + i * NT + n) * 32 + lane] = *reinterpret_cast<const float4 *>(o[i][n]);
+                if (t == 0) {
+#pragma unroll
+                    for (int n = 0; n < NT; n++) peer_m[slot][8 * n + g] = m[n], peer_l[slot][8 * n + g] = l[n];
+                }
+            }
+            __syncthreads();
+            if (team < half) {
+                const int from = team * RW + member;
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const float m2 = peer_m[from][8 * n + g], top = fmaxf(m[n], m2), ref = merge_reference(top), f = exp2_approx(m[n] - ref), f2 = exp2_approx(m2 - ref);
+                    m[n] = top;
+                    l[n] = l[n] * f + peer_l[from][8 * n + g] * f2;
+                    const float a = __shfl_sync(0xffffffffu, f, 8 * t), c = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+                    const float a2 = __shfl_sync(0xffffffffu, f2, 8 * t), c2 = __shfl_sync(0xffffffffu, f2, 8 * t + 4);
+#pragma unroll
+                    for (int i = 0; i < VH * 4; i++) {
+                        const float4 u = peers[(from * (Shape::ACC / 4) + i * NT + n) * 32 + lane];
+                        o[i][n][0] = o[i][n][0] * a + u.x * a2;
+                        o[i][n][1] = o[i][n][1] * c + u.y * c2;
+                        o[i][n][2] = o[i][n][2] * a + u.z * a2;
+                        o[i][n][3] = o[i][n][3] * c + u.w * c2;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (team == 0) {
+            const bool whole = t0 == 0 && t1 == sp.tiles;
+            float *part = p.ws + (((size_t)blockIdx.y * ctas + cta) * 2 + (first ? 0 : 1)) * Shape::ROWS * (D + 2);
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const float L = __shfl_sync(0xffffffffu, l[n], 8 * t + 4 * e);
+                    const int i0 = member * 8 * NT + 8 * n + 2 * t + e, r = r0 + i0;
+                    if (r >= R) continue;
+                    if (whole) {
+                        T *to = reinterpret_cast<T *>(p.out) + (((size_t)b * p.S + r % p.S) * p.Hq + h * p.group + r / p.S) * D;
+#pragma unroll
+                        for (int v = 0; v < VH; v++) {
+                            __align__(16) T y[8];
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                y[2 * i] = from_f32<T>(paged_quotient(o[4 * v + i][n][e], L));
+                                y[2 * i + 1] = from_f32<T>(paged_quotient(o[4 * v + i][n][2 + e], L));
+                            }
+                            if (64 * v + 8 * g < D) *reinterpret_cast<uint4 *>(to + 64 * v + 8 * g) = *reinterpret_cast<const uint4 *>(y);
+                        }
+                    } else {
+#pragma unroll
+                        for (int v = 0; v < VH; v++) {
+                            float4 *to = reinterpret_cast<float4 *>(part + (size_t)i0 * D + 64 * v + 8 * g);
+                            if (64 * v + 8 * g < D) {
+                                to[0] = make_float4(o[4 * v][n][e], o[4 * v][n][2 + e], o[4 * v + 1][n][e], o[4 * v + 1][n][2 + e]);
+                                to[1] = make_float4(o[4 * v + 2][n][e], o[4 * v + 2][n][2 + e], o[4 * v + 3][n][e], o[4 * v + 3][n][2 + e]);
+                            }
+                        }
+                    }
+                }
+                if (!whole && t == 0) {
+                    const int i0 = member * 8 * NT + 8 * n + g;
+                    part[Shape::ROWS * D + i0] = m[n] * kLn2;
+                    part[Shape::ROWS * D + Shape::ROWS + i0] = l[n];
+                }
+            }
+        }
+        left -= t1 - t0;
+        t0 = 0;
+        if (++h == p.G) {
+            h = 0;
+            b++;
+        }
+    }
+}
+
 // ---- parts of pairs that lie in several CTAs ------------------------------------------------------------------------------
 constexpr int kJoinThreads = 256;
 template <typename T>
@@ -255,8 +592,12 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
     }
 }
 
+// How the launch is cut: kernel, query rows of a block, CTAs.
 struct PagedPlan {
+    bool mma;
+    int dim, tiles_of_rows, team;  // padded head dimension, 8-row blocks of a warp, warps of a team
     int ctas, block_rows, row_blocks, round;
+    size_t bytes(int D) const { return (size_t)ctas * row_blocks * 2 * block_rows * (D + 2) * sizeof(float); }
 };
 
 static int paged_sms(int *sms) {
@@ -266,21 +607,52 @@ static int paged_sms(int *sms) {
     return MYNN_OK;
 }
 
-static PagedPlan paged_plan(int B, int S, int Hq, int Hkv, int D, int page, int width, int sms) {
+static PagedPlan paged_plan(int B, int S, int Hq, int Hkv, int D, int page, int width, int sms, bool mma) {
     PagedPlan n;
-    n.block_rows = kPlainRows;
-    n.row_blocks = (int)(((long long)Hq / Hkv * S + n.block_rows - 1) / n.block_rows);
-    n.round = D > 128 ? kPlainWarps<8> : kPlainWarps<4>;
+    const int R = Hq / Hkv * S;
+    n.mma = mma;
+    n.dim = D <= 64 ? 64 : D <= 128 ? 128 : D <= 192 ? 192 : 256;
+    n.tiles_of_rows = R <= 8 ? 1 : 2;
+    n.team = R <= 16 ? 1 : R <= 32 ? 2 : 4;
+    n.block_rows = mma ? 8 * n.tiles_of_rows * n.team : kPlainRows;
+    n.row_blocks = (R + n.block_rows - 1) / n.block_rows;
+    n.round = mma || D <= 128 ? 4 : kPlainWarps<8>;
     const long long tiles = ((long long)width * page + kPagedTile - 1) / kPagedTile * Hkv * B;
-    n.ctas = (int)std::min<long long>(sms, std::max<long long>(1, (tiles + n.round - 1) / n.round));
+    const int most = mma && n.dim <= 128 ? 2 * sms : sms;
+    n.ctas = (int)std::min<long long>(most, std::max<long long>(1, (tiles + n.round - 1) / n.round));
     return n;
+}
+
+template <typename T, int DP, int NT, int RW>
+static int launch_mma(cudaStream_t st, const PagedAttention &p, int ctas) {
+    static SmemLimit limit;
+    MYNN_CUDA_OK(limit.raise((const void *)paged_attention_mma_kernel<T, DP, NT, RW>, MmaShape<DP, NT, RW>::SMEM));
+    MYNN_CUDA_OK(launch_dependent(paged_attention_mma_kernel<T, DP, NT, RW>, dim3(ctas, p.row_blocks), dim3(128), MmaShape<DP, NT, RW>::SMEM, st, p));
+    MYNN_LAUNCH_OK("paged_attention_mma_kernel");
+    return MYNN_OK;
+}
+template <typename T, int DP>
+static int launch_mma_rows(cudaStream_t st, const PagedAttention &p, const PagedPlan &n) {
+    if (n.team == 4) return launch_mma<T, DP, 2, 4>(st, p, n.ctas);
+    if (n.team == 2) return launch_mma<T, DP, 2, 2>(st, p, n.ctas);
+    return n.tiles_of_rows == 2 ? launch_mma<T, DP, 2, 1>(st, p, n.ctas) : launch_mma<T, DP, 1, 1>(st, p, n.ctas);
+}
+template <typename T>
+static int launch_mma_any(cudaStream_t st, const PagedAttention &p, const PagedPlan &n) {
+    switch (n.dim) {
+        case 64: return launch_mma_rows<T, 64>(st, p, n);
+        case 128: return launch_mma_rows<T, 128>(st, p, n);
+        case 192: return launch_mma_rows<T, 192>(st, p, n);
+        default: return launch_mma_rows<T, 256>(st, p, n);
+    }
 }
 
 template <typename T, int DL>
 static int launch_plain(cudaStream_t st, const PagedAttention &p, int ctas, int vec) {
     const dim3 grid(ctas, p.row_blocks), block(kPlainWarps<DL> * 32);
+    static SmemLimit limits[2];
     auto go = [&](auto kern) -> int {
-        MYNN_CUDA_OK(cudaFuncSetAttribute((const void *)kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plain_smem<DL>()));
+        MYNN_CUDA_OK(limits[vec == 4].raise((const void *)kern, plain_smem<DL>()));
         MYNN_CUDA_OK(launch_dependent(kern, grid, block, plain_smem<DL>(), st, p));
         MYNN_LAUNCH_OK("paged_attention_plain_kernel");
         return MYNN_OK;
@@ -306,8 +678,7 @@ static int paged_check(int B, int S, int Hq, int Hkv, int D, int page, int width
 extern "C" size_t mynn_b200_paged_attention_workspace_bytes(int B, int S, int Hq, int Hkv, int D, int page, int table_pages) {
     int sms = 0;
     if (paged_check(B, S, Hq, Hkv, D, page, table_pages) != MYNN_OK || B == 0 || paged_sms(&sms) != MYNN_OK) return 0;
-    const PagedPlan n = paged_plan(B, S, Hq, Hkv, D, page, table_pages, sms);
-    return (size_t)n.ctas * n.row_blocks * 2 * n.block_rows * (D + 2) * sizeof(float);
+    return std::max(paged_plan(B, S, Hq, Hkv, D, page, table_pages, sms, true).bytes(D), paged_plan(B, S, Hq, Hkv, D, page, table_pages, sms, false).bytes(D));
 }
 
 extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q, const void *k_pages, const void *v_pages, const int32_t *block_table,
@@ -321,12 +692,14 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
     if (!out || !q || !block_table || !lengths || (pages && (!k_pages || !v_pages))) return fail(MYNN_E_ARG, "paged_attention: null pointer");
     int sms = 0;
     if (const int e = paged_sms(&sms)) return e;
-    const PagedPlan n = paged_plan(B, S, Hq, Hkv, D, page, table_pages, sms);
-    const size_t need = (size_t)n.ctas * n.row_blocks * 2 * n.block_rows * (D + 2) * sizeof(float);
+    const bool mma = dtype != MYNN_F32 && D % 8 == 0 && ((uintptr_t)out | (uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0;
+    const PagedPlan n = paged_plan(B, S, Hq, Hkv, D, page, table_pages, sms, mma);
+    const size_t need = n.bytes(D);
     if (!workspace || workspace_bytes < need) return fail(MYNN_E_ARG, "paged_attention: workspace of %zu bytes, %zu are needed", workspace_bytes, need);
     if ((uintptr_t)workspace % 16) return fail(MYNN_E_ARG, "paged_attention: the workspace is not aligned to 16 bytes");
     PagedAttention p;
-    p.out = out, p.q = q, p.k = k_pages, p.v = v_pages;
+    p.out = out, p.q = q;
+    p.k = pages ? k_pages : q, p.v = pages ? v_pages : q;  // (a copy of nothing has an address too)
     p.table = block_table, p.lengths = lengths, p.counts = counts;
     p.scale = scale, p.softcap = softcap, p.window = std::min(window, kPagedWindow), p.sinks = sinks;
     p.B = B, p.S = S, p.Hq = Hq, p.G = Hkv, p.group = Hq / Hkv, p.D = D;
@@ -336,8 +709,10 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
     const cudaStream_t st = (cudaStream_t)stream;
     const int vec = D % 4 == 0 && ((uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0 ? 4 : 1;
     MYNN_DISPATCH_DTYPE(dtype, T, {
-        int e;
-        if (D <= 32) e = launch_plain<T, 1>(st, p, n.ctas, vec);
+        int e = MYNN_OK;
+        if (n.mma) {
+            if constexpr (!std::is_same<T, float>::value) e = launch_mma_any<T>(st, p, n);
+        } else if (D <= 32) e = launch_plain<T, 1>(st, p, n.ctas, vec);
         else if (D <= 64) e = launch_plain<T, 2>(st, p, n.ctas, vec);
         else if (D <= 96) e = launch_plain<T, 3>(st, p, n.ctas, vec);
         else if (D <= 128) e = launch_plain<T, 4>(st, p, n.ctas, vec);
