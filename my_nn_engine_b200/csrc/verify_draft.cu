@@ -3,9 +3,10 @@
 // Draft token x_i stands while u_i q_i(x_i) < p_i(x_i); the first one that does not, n, is replaced by a draw from max(p_n - q_n, 0), and behind K standing tokens
 // comes a draw from p_K: the first token whose running sum exceeds r times the whole sum.  So the tokens are distributed as the target's own.
 //
-// Of (2 K + 1) V probabilities only the one or two rows of the draw are read whole.  A cluster of CTAs takes a sequence, each CTA a range of the vocabulary and each warp a
-// part of it: sums per warp, then which part the running sum ends in, then that part again, 128 tokens at a time.  A difference of two f32
-// numbers and sums of 1e5 of them decide on whole numbers, so they are held in 64 bits: a sum in f32 is off by more than many a token's probability.
+// Of (2 K + 1) V probabilities only the one or two rows of the draw are read whole.  A cluster of up to eight CTAs takes a sequence, each CTA a range of the vocabulary and each
+// warp a part of it: sums per warp, then which CTA's and which warp's part the running sum ends in, then that part again, from L2.  A difference of two
+// f32 numbers and sums of 1e5 of them decide on whole numbers, so they are held in 64 bits: a sum in f32 is off by more than many a token's
+// probability.  The order of the sums is fixed.
 #include "common.cuh"
 #include "tcgen05.cuh"
 
@@ -19,101 +20,192 @@ struct VerifyDraft {
     int B, K, V;
 };
 
-constexpr int kVerifyWarps = 16;
+constexpr int kVerifyWarps = 8;
 
-template <typename T>
-__device__ __forceinline__ double weight_of(const T *p, const T *q, int i, int without) {
-    const double a = (double)to_f32<T>(p[i]), w = q ? a - (double)to_f32<T>(q[i]) : a;
-    return i != without && w > 0.0 ? w : 0.0;
+__device__ __forceinline__ double ld_cluster_f64(uint32_t addr) {
+    double v;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ double warp_sum_f64(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
 }
 
-// One CTA per sequence.
+// The row that the token is drawn from: p - q, or p without one token; what is not positive has no weight.
 template <typename T>
-__global__ void __launch_bounds__(kVerifyWarps * 32) verify_draft_kernel(const VerifyDraft p) {
-    __shared__ double sums[kVerifyWarps];
-    __shared__ int sm_n, sm_pick;
+struct DrawRow {
+    const T *p, *q;  // q may be null
+    int without;
+    __device__ __forceinline__ double weight(float a, float c, int i) const {
+        const double w = (double)a - (double)c;
+        return i != without && w > 0.0 ? w : 0.0;
+    }
+    // Weights of tokens at + VEC * lane + 32 VEC u (u < U), those behind `end` zero: loads first.
+    template <int VEC, int U>
+    __device__ __forceinline__ void load(int at, int end, int lane, double (&w)[U][VEC]) const {
+        __align__(16) T a[U][VEC], c[U][VEC];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = at + VEC * (lane + 32 * u);
+            if constexpr (VEC > 1) {
+                *reinterpret_cast<uint4 *>(a[u]) = i < end ? __ldg(reinterpret_cast<const uint4 *>(p + i)) : make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4 *>(c[u]) = q && i < end ? __ldg(reinterpret_cast<const uint4 *>(q + i)) : make_uint4(0, 0, 0, 0);
+            } else {
+                a[u][0] = i < end ? p[i] : from_f32<T>(0.f);
+                c[u][0] = q && i < end ? q[i] : from_f32<T>(0.f);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < VEC; e++) w[u][e] = weight(to_f32<T>(a[u][e]), to_f32<T>(c[u][e]), at + VEC * (lane + 32 * u) + e);
+    }
+};
+
+// grid (cluster, B).  VEC: elements of a 16-byte piece where all rows begin on 16 bytes, else 1.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kVerifyWarps * 32, 3) verify_draft_kernel(const VerifyDraft p) {
+    constexpr int U = VEC == 1 ? 8 : 16 / VEC;  // pieces of a lane in flight per row: 8 x 1, 4 x 4 or 2 x 8 numbers
+    constexpr int STEP = 32 * VEC * U;
+    __shared__ double sums[kVerifyWarps], whole[2];
+    __shared__ int pick;
     pdl_trigger();
     pdl_wait();
-    const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, K = p.K, V = p.V;
+    const int b = blockIdx.y, rank = blockIdx.x, ranks = gridDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, K = p.K, V = p.V;
     const int drafts = p.counts ? min(max(p.counts[b], 0), K) : K;
     const T *target = reinterpret_cast<const T *>(p.target) + (size_t)b * (K + 1) * V;
     const T *draft = p.draft ? reinterpret_cast<const T *>(p.draft) + (size_t)b * K * V : nullptr;
-    if (warp == 0) {
-        int n = drafts;
-        for (int i = lane; i < drafts; i += 32) {
+    const float sample = p.sample[b];
+    int n = drafts;  // drafts that stand: every warp looks for itself
+    for (int i0 = 0; i0 < drafts; i0 += 32) {
+        const int i = i0 + lane;
+        bool falls = false;
+        if (i < drafts) {
             const int x = p.tokens[(size_t)b * K + i];
-            bool stands = false;
+            const float u = p.accept[(size_t)b * K + i];
+            falls = true;
             if ((unsigned)x < (unsigned)V) {
                 const double q = draft ? (double)to_f32<T>(draft[(size_t)i * V + x]) : 1.0;
-                stands = (double)p.accept[(size_t)b * K + i] * q < (double)to_f32<T>(target[(size_t)i * V + x]);
-            }
-            if (!stands) {
-                n = i;
-                break;
+                falls = !((double)u * q < (double)to_f32<T>(target[(size_t)i * V + x]));  // (24 by 24 bits: exact)
             }
         }
-        n = __reduce_min_sync(0xffffffffu, n);
-        if (lane == 0) sm_n = n;
+        const unsigned any = __ballot_sync(0xffffffffu, falls);
+        if (any) {
+            n = i0 + __ffs(any) - 1;
+            break;
+        }
     }
-    __syncthreads();
-    const int n = sm_n;
-    const T *pr = target + (size_t)n * V, *qr = n < drafts && draft ? draft + (size_t)n * V : nullptr;
-    int without = n < drafts && !draft ? p.tokens[(size_t)b * K + n] : -1;
-    const int per = (V + kVerifyWarps - 1) / kVerifyWarps, lo = min(warp * per, V), hi = min(lo + per, V);
-    double total = 0.0;
-    for (int pass = 0; pass < 2; pass++) {
-        double mine = 0.0;
-        for (int i = lo + lane; i < hi; i += 32) mine += weight_of(pr, qr, i, without);
+    DrawRow<T> row = {target + (size_t)n * V, n < drafts && draft ? draft + (size_t)n * V : nullptr, n < drafts && !draft ? p.tokens[(size_t)b * K + n] : -1};
+    // parts of whole steps: the cluster's ranks in order, in each its warps
+    const int parts = ranks * kVerifyWarps, per = ((V + parts - 1) / parts + 32 * VEC - 1) / (32 * VEC) * (32 * VEC);
+    const int lo = (int)min((long long)(rank * kVerifyWarps + warp) * per, (long long)V), hi = min(lo + per, V);
+    double total = 0.0, before = 0.0, mine = 0.0;
+    bool chosen = false;
+    for (int pass = 0;; pass++) {
+        double w[U][VEC], sum = 0.0;
+        for (int at = lo; at < hi; at += STEP) {
+            row.template load<VEC, U>(at, hi, lane, w);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-        if (lane == 0) sums[warp] = mine;
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int e = 0; e < VEC; e++) sum += w[u][e];
+        }
+        sum = warp_sum_f64(sum);
+        if (lane == 0) sums[warp] = sum;
         __syncthreads();
+        mine = 0.0;
+#pragma unroll
+        for (int i = 0; i < kVerifyWarps; i++) mine += sums[i];
+        if (threadIdx.x == 0) whole[pass] = mine;
+        cluster_sync_all();
+        // where the running sum exceeds sample * total; if it never does (the product was rounded up to the total) the last part with any weight
+        double part[8];
+#pragma unroll
+        for (int r = 0; r < 8; r++) part[r] = r < ranks ? ld_cluster_f64(map_rank(smem_u32(&whole[pass]), r)) : 0.0;
         total = 0.0;
-        for (int w = 0; w < kVerifyWarps; w++) total += sums[w];
-        __syncthreads();
-        if (total > 0.0 || (!qr && without < 0)) break;
-        qr = nullptr;  // nothing is left of the target where the draft is taken off: the draw is from the target itself
-        without = -1;
-        if (lane == 0) sums[warp] = 0.0;
-    }
-    if (threadIdx.x == 0) sm_pick = -1;
-    __syncthreads();
-    const double goal = (double)p.sample[b] * total;
-    // the warp whose part the running sum exceeds the goal in; without one (the goal rounded up to the whole sum) the last that has any weight
-    double before = 0.0;
-    int chosen = -1;
-    {
-        double run = 0.0;
-        for (int w = 0; w < kVerifyWarps; w++) {
-            if (!(sums[w] > 0.0)) continue;
-            chosen = w;
-            before = run;
-            run += sums[w];
-            if (run > goal) break;
-        }
-    }
-    if (warp == chosen) {
-        int pick = -1, last = -1;
-        double run = before;
-        for (int base = lo; base < hi && pick < 0; base += 32) {
-            const int i = base + lane;
-            const double w = i < hi ? weight_of(pr, qr, i, without) : 0.0;
-            double incl = w;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double up = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += up;
+        for (int r = 0; r < 8; r++) total += part[r];
+        const double goal = (double)sample * total;
+        double run = 0.0;
+        int at = -1;
+#pragma unroll
+        for (int r = 0; r < 8; r++) {
+            if (part[r] > 0.0 && (at < 0 || run <= goal)) {
+                at = r;
+                before = run;
+                run += part[r];
             }
-            const unsigned over = __ballot_sync(0xffffffffu, w > 0.0 && run + incl > goal), some = __ballot_sync(0xffffffffu, w > 0.0);
-            if (over) pick = base + __ffs(over) - 1;
-            if (some) last = base + 31 - __clz(some);
-            run += __shfl_sync(0xffffffffu, incl, 31);
         }
-        if (lane == 0) sm_pick = pick >= 0 ? pick : last;
+        chosen = at == rank;
+        if (total > 0.0 || pass == 1 || (!row.q && row.without < 0)) break;
+        row.q = nullptr;  // nothing is left of the target where the draft is taken off: the draw is from the target itself
+        row.without = -1;
+        __syncthreads();  // the sums have been read
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i <= K; i += kVerifyWarps * 32) p.tokens_out[(size_t)b * (K + 1) + i] = i < n ? p.tokens[(size_t)b * K + i] : i == n ? sm_pick : -1;
-    if (threadIdx.x == 0) p.accepted_out[b] = n;
+    if (chosen || (rank == 0 && !(total > 0.0))) {
+        const double goal = (double)sample * total;
+        if (threadIdx.x == 0) pick = -1;
+        __syncthreads();
+        double run = before;
+        int at = -1;
+#pragma unroll
+        for (int i = 0; i < kVerifyWarps; i++) {
+            if (sums[i] > 0.0 && (at < 0 || run <= goal)) {
+                at = i;
+                before = run;
+                run += sums[i];
+            }
+        }
+        if (chosen && warp == at) {
+            int found = -1, last = -1;
+            for (int base = lo; base < hi && found < 0; base += STEP) {
+                double w[U][VEC], own[U], all[U];
+                row.template load<VEC, U>(base, hi, lane, w);
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    own[u] = 0.0;
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) own[u] += w[u][e];
+                    all[u] = warp_sum_f64(own[u]);
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (found >= 0 || !(all[u] > 0.0)) continue;
+                    double incl = own[u];
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const double up = __shfl_up_sync(0xffffffffu, incl, o);
+                        if (lane >= o) incl += up;
+                    }
+                    double sum = before + (incl - own[u]);
+                    int over = -1, some = -1;
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) {
+                        sum += w[u][e];
+                        if (w[u][e] > 0.0) {
+                            some = e;
+                            if (over < 0 && sum > goal) over = e;
+                        }
+                    }
+                    const unsigned overs = __ballot_sync(0xffffffffu, over >= 0), somes = __ballot_sync(0xffffffffu, some >= 0);
+                    if (overs) {
+                        const int l = __ffs(overs) - 1;
+                        found = base + VEC * (l + 32 * u) + __shfl_sync(0xffffffffu, over, l);
+                    }
+                    const int l = 31 - __clz(somes);
+                    last = base + VEC * (l + 32 * u) + __shfl_sync(0xffffffffu, some, l);
+                    before += all[u];
+                }
+            }
+            if (lane == 0) pick = found >= 0 ? found : last;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i <= K; i += kVerifyWarps * 32) p.tokens_out[(size_t)b * (K + 1) + i] = i < n ? p.tokens[(size_t)b * K + i] : i == n ? pick : -1;
+        if (threadIdx.x == 0) p.accepted_out[b] = n;
+    }
+    cluster_sync_all();  // nobody leaves while its sums may still be read
 }
 
 }  // namespace mynn
@@ -124,7 +216,7 @@ extern "C" int mynn_b200_verify_draft(void *stream, int32_t *tokens_out, int32_t
                                       const int32_t *counts, const float *accept, const float *sample, int B, int K, int V, int dtype) {
     if (B < 0 || K < 0 || V < 1) return fail(MYNN_E_ARG, "verify_draft: bad shape");
     if (!dtype_ok(dtype)) return fail(MYNN_E_ARG, "verify_draft: bad dtype %d", dtype);
-    if (K > 1024 || V > 1 << 30) return fail(MYNN_E_UNSUPPORTED, "verify_draft: %d drafted tokens of a vocabulary of %d", K, V);
+    if (K > 1024 || V > 1 << 30 || B > 65535) return fail(MYNN_E_UNSUPPORTED, "verify_draft: %d sequences of %d drafted tokens of a vocabulary of %d", B, K, V);
     if (B == 0) return MYNN_OK;
     if (!tokens_out || !accepted_out || !target || !sample || (K && (!tokens || !accept))) return fail(MYNN_E_ARG, "verify_draft: null pointer");
     VerifyDraft p;
@@ -133,7 +225,17 @@ extern "C" int mynn_b200_verify_draft(void *stream, int32_t *tokens_out, int32_t
     p.tokens = tokens, p.counts = counts;
     p.accept = accept, p.sample = sample;
     p.B = B, p.K = K, p.V = V;
-    MYNN_DISPATCH_DTYPE(dtype, T, { MYNN_CUDA_OK(launch_dependent(verify_draft_kernel<T>, dim3(B), dim3(kVerifyWarps * 32), 0, (cudaStream_t)stream, p)); });
+    // As many CTAs per sequence as keep a warp's part at a step or more.
+    int ranks = 1;
+    while (ranks < 8 && (long long)V >= 2ll * ranks * kVerifyWarps * 256) ranks *= 2;
+    const dim3 grid(ranks, B), block(kVerifyWarps * 32);
+    const cudaStream_t st = (cudaStream_t)stream;
+    MYNN_DISPATCH_DTYPE(dtype, T, {
+        constexpr int VEC = 16 / sizeof(T);
+        const bool vec = V % VEC == 0 && ((uintptr_t)target | (uintptr_t)draft) % 16 == 0;
+        if (vec) MYNN_CUDA_OK(launch_ex(true, ranks, verify_draft_kernel<T, VEC>, grid, block, 0, st, p));
+        else MYNN_CUDA_OK(launch_ex(true, ranks, verify_draft_kernel<T, 1>, grid, block, 0, st, p));
+    });
     MYNN_LAUNCH_OK("verify_draft_kernel");
     return MYNN_OK;
 }

@@ -43,7 +43,7 @@ def test_append_refuses_sizes_beyond_its_limits(bad):
 
 
 @pytest.mark.parametrize("bad,code", [(dict(B=-1), ffi.E_ARG), (dict(K=-1), ffi.E_ARG), (dict(V=0), ffi.E_ARG), (dict(dtype=9), ffi.E_ARG), (dict(tokens=None), ffi.E_ARG),
-                                      (dict(K=1025), ffi.E_UNSUPPORTED), (dict(V=(1 << 30) + 1), ffi.E_UNSUPPORTED)])
+                                      (dict(K=1025), ffi.E_UNSUPPORTED), (dict(B=65536), ffi.E_UNSUPPORTED), (dict(V=(1 << 30) + 1), ffi.E_UNSUPPORTED)])
 def test_verification_refuses(bad, code):
     assert verify(**bad) == code and "verify_draft" in ffi.last_error()
 
