@@ -1,8 +1,11 @@
 // The step between the q/k/v projection and attention over a paged cache: rotation of the new tokens' q and k, their division by the root mean square
 // per head, and the append to the pages, in one launch.  Every sequence has a length and a number of new tokens of its own.
 //
-// One warp takes one head of one token: rotated dimension i and its partner are half a rotated range apart or next door, so a head is staged as f32 in shared memory;
-// rotation and norm are f32, the result is rounded once.
+// Rotation and norm are f32, the result is rounded once.  A CTA takes one token.  Where heads come in pieces of eight numbers, a thread holds two pieces: piece i of
+// the rotated half and its partner half a rotated range away, or two neighbours; it does so for one head after the other, so a token's angles are read once per
+// thread, and a head's norm is a sum over the few threads that share it.  Other sizes (paged_append_any_kernel): a warp per head, staged in shared memory.
+#include <algorithm>
+
 #include "common.cuh"
 #include "paged.cuh"
 
@@ -21,8 +24,128 @@ struct PagedAppend {
 
 constexpr int kAppendWarps = 8;
 
+struct AppendToken {
+    int b, s, pos;
+    bool real;
+    size_t row;   // of the cache for kv head 0 (heads are `page` rows apart)
+    bool stored;  // the table names a page
+};
+
+__device__ __forceinline__ AppendToken append_token(const PagedAppend &p, int b, int s) {
+    AppendToken k = {b, s, 0, false, 0, false};
+    const int len = max(p.lengths[b], 0), count = p.counts ? min(max(p.counts[b], 0), p.S) : p.S;
+    k.pos = len - count + s;
+    k.real = s < count && k.pos >= 0 && k.pos < p.width * p.page && (p.rot_dims == 0 || k.pos < p.positions);
+    if (k.real) {
+        const int i = k.pos / p.page, pg = p.table[(size_t)b * p.width + i];
+        k.stored = (unsigned)pg < (unsigned)p.pages;
+        k.row = k.stored ? (size_t)pg * p.G * p.page + (k.pos - i * p.page) : 0;
+    }
+    return k;
+}
+
+// Eight numbers as they come from or go to memory.
 template <typename T>
-__global__ void __launch_bounds__(kAppendWarps * 32) paged_append_kernel(const PagedAppend p) {
+struct Piece {
+    static constexpr int N = 8 * sizeof(T) / 16;
+    uint4 raw[N];
+    __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+        for (int i = 0; i < N; i++) raw[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+    }
+    __device__ __forceinline__ void store(T *p) const {
+#pragma unroll
+        for (int i = 0; i < N; i++) reinterpret_cast<uint4 *>(p)[i] = raw[i];
+    }
+    __device__ __forceinline__ float at(int i) const { return to_f32<T>(reinterpret_cast<const T *>(raw)[i]); }
+    __device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T *>(raw)[i] = from_f32<T>(v); }
+};
+
+// grid (S, B); a group of `lanes` threads (a power of two) per head, thread i of it with pieces c0 and c1.  D a multiple of 16, rot_dims of 16 (halves) or 8.
+template <typename T>
+__global__ void __launch_bounds__(512) paged_append_kernel(const PagedAppend p, int lanes) {
+    pdl_trigger();
+    pdl_wait();
+    const int s = blockIdx.x, b = blockIdx.y, sub = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = blockDim.x / lanes;
+    const int heads = p.Hq + 2 * p.G, half = p.rot_dims >> 1, pairs = p.D / 16;
+    const bool in = sub < pairs;
+    const unsigned sharers = (0xffffffffu >> (32 - lanes)) << (threadIdx.x & 31 & ~(lanes - 1));  // the threads of this head
+    // with halves the first half / 8 threads have partners, the others two pieces behind the rotated range
+    const bool split = p.halves && sub < half / 8;
+    const int d0 = split ? 8 * sub : 16 * sub, d1 = split ? d0 + half : d0 + 8;
+    const T *src = reinterpret_cast<const T *>(p.proj) + ((size_t)b * p.S + s) * heads * p.D;
+    Piece<T> x0, x1;
+    if (in && group < heads) x0.load(src + (size_t)group * p.D + d0), x1.load(src + (size_t)group * p.D + d1);
+    const AppendToken k = append_token(p, b, s);
+    // angles of the pairs in the two pieces: halves (d0 + i, d1 + i), else (d0 + 2 i, d0 + 2 i + 1) and the same in the second piece
+    float c[8], a[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) c[i] = 1.f, a[i] = 0.f;
+    if (in && k.real && p.rot_dims > 0) {
+        const float *cs = p.cos_t + (size_t)k.pos * half, *sn = p.sin_t + (size_t)k.pos * half;
+        const int first = split ? d0 : d0 / 2;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (split || (!p.halves && first + i < half)) c[i] = cs[first + i], a[i] = sn[first + i];
+    }
+    for (int head = group; head < heads; head += groups) {
+        Piece<T> y0, y1;
+        const bool key = head < p.Hq + p.G;
+        if (key && k.real) {
+            float u[8], w[8], ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) u[i] = in ? x0.at(i) : 0.f, w[i] = in ? x1.at(i) : 0.f;
+            if (split) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float lo = rope_low(u[i], w[i], c[i], a[i]), hi = rope_high(u[i], w[i], c[i], a[i]);
+                    u[i] = lo, w[i] = hi;
+                }
+            } else if (!p.halves && p.rot_dims > 0) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (d0 + 2 * i < p.rot_dims) {
+                        const float lo = rope_low(u[2 * i], u[2 * i + 1], c[i], a[i]), hi = rope_high(u[2 * i], u[2 * i + 1], c[i], a[i]);
+                        u[2 * i] = lo, u[2 * i + 1] = hi;
+                    }
+                    if (d1 + 2 * i < p.rot_dims) {
+                        const float lo = rope_low(w[2 * i], w[2 * i + 1], c[4 + i], a[4 + i]), hi = rope_high(w[2 * i], w[2 * i + 1], c[4 + i], a[4 + i]);
+                        w[2 * i] = lo, w[2 * i + 1] = hi;
+                    }
+                }
+            }
+            float inv = 1.f;
+            if (p.qk_norm) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) ss += u[i] * u[i] + w[i] * w[i];
+                for (int o = lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(sharers, ss, o);
+                inv = 1.0f / sqrtf(ss / (float)p.D + p.eps);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) y0.set(i, u[i] * inv), y1.set(i, w[i] * inv);
+        } else {
+            y0 = x0, y1 = x1;
+        }
+        if (in) {
+            T *dst = nullptr;
+            if (head < p.Hq) {
+                dst = reinterpret_cast<T *>(p.q_out) + (((size_t)b * p.Hq + head) * p.S + s) * p.D;
+                if (!k.real)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) y0.set(i, 0.f), y1.set(i, 0.f);
+            } else if (k.stored) {
+                const int kv = head - p.Hq - (key ? 0 : p.G);
+                dst = reinterpret_cast<T *>(key ? p.k : p.v) + (k.row + (size_t)kv * p.page) * p.D;
+            }
+            if (dst) y0.store(dst + d0), y1.store(dst + d1);
+            const int next = head + groups;
+            if (next < heads) x0.load(src + (size_t)next * p.D + d0), x1.load(src + (size_t)next * p.D + d1);
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kAppendWarps * 32) paged_append_any_kernel(const PagedAppend p) {
     extern __shared__ float sm[];
     pdl_trigger();
     pdl_wait();
@@ -30,22 +153,19 @@ __global__ void __launch_bounds__(kAppendWarps * 32) paged_append_kernel(const P
     const long long job = (long long)blockIdx.x * kAppendWarps + warp, token = job / heads;
     if (token >= (long long)p.B * p.S) return;
     const int head = (int)(job - token * heads), b = (int)(token / p.S), s = (int)(token - (long long)b * p.S);
-    const int len = max(p.lengths[b], 0), count = p.counts ? min(max(p.counts[b], 0), p.S) : p.S;
-    const int pos = len - count + s;
-    const bool real = s < count && pos >= 0 && pos < p.width * p.page && (p.rot_dims == 0 || pos < p.positions);
+    const AppendToken k = append_token(p, b, s);
     const T *src = reinterpret_cast<const T *>(p.proj) + (size_t)job * p.D;
     T *dst;
     if (head < p.Hq) {
         dst = reinterpret_cast<T *>(p.q_out) + (((size_t)b * p.Hq + head) * p.S + s) * p.D;
-        if (!real) {
+        if (!k.real) {
             for (int d = lane; d < p.D; d += 32) dst[d] = from_f32<T>(0.f);
             return;
         }
     } else {
-        if (!real) return;
-        const int i = pos / p.page, pg = p.table[(size_t)b * p.width + i], kv = (head - p.Hq) % p.G;
-        if ((unsigned)pg >= (unsigned)p.pages) return;
-        dst = reinterpret_cast<T *>(head < p.Hq + p.G ? p.k : p.v) + (((size_t)pg * p.G + kv) * p.page + pos - i * p.page) * p.D;
+        if (!k.stored) return;
+        const int kv = (head - p.Hq) % p.G;
+        dst = reinterpret_cast<T *>(head < p.Hq + p.G ? p.k : p.v) + (k.row + (size_t)kv * p.page) * p.D;
         if (head >= p.Hq + p.G) {
             for (int d = lane; d < p.D; d += 32) dst[d] = src[d];
             return;
@@ -55,7 +175,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) paged_append_kernel(const P
     for (int d = lane; d < p.D; d += 32) x[d] = to_f32<T>(src[d]);
     __syncwarp();
     const int half = p.rot_dims >> 1;
-    const float *cs = p.cos_t + (size_t)pos * half, *sn = p.sin_t + (size_t)pos * half;
+    const float *cs = p.cos_t + (size_t)k.pos * half, *sn = p.sin_t + (size_t)k.pos * half;
     for (int i = lane; i < half; i += 32) {
         const int lo = p.halves ? i : 2 * i, hi = p.halves ? i + half : 2 * i + 1;
         const float a = x[lo], c = x[hi];
@@ -98,10 +218,21 @@ extern "C" int mynn_b200_paged_rotary_append(void *stream, void *q_out, void *k_
     p.B = B, p.S = S, p.Hq = Hq, p.G = Hkv, p.D = D;
     p.rot_dims = rot_dims, p.halves = halves, p.qk_norm = qk_norm, p.eps = eps;
     p.page = page, p.pages = pages, p.width = table_pages, p.positions = positions;
+    const cudaStream_t st = (cudaStream_t)stream;
+    const bool pieces = D % 16 == 0 && D <= 512 && rot_dims % (halves ? 16 : 8) == 0 && B <= 65535 &&
+                        ((uintptr_t)proj | (uintptr_t)q_out | (uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0;
+    if (pieces) {
+        // 32 sequences of one token, 48 heads of 128: 6.7 us with a warp per head
+        int lanes = 1;
+        while (lanes < D / 16) lanes *= 2;
+        const int threads = (int)std::min<long long>(512, ((long long)(Hq + 2 * Hkv) * lanes + 31) / 32 * 32);
+        MYNN_DISPATCH_DTYPE(dtype, T, { MYNN_CUDA_OK(launch_dependent(paged_append_kernel<T>, dim3(S, B), dim3(threads), 0, st, p, lanes)); });
+        MYNN_LAUNCH_OK("paged_append_kernel");
+        return MYNN_OK;
+    }
     MYNN_DISPATCH_DTYPE(dtype, T, {
-        MYNN_CUDA_OK(launch_dependent(paged_append_kernel<T>, dim3((unsigned)blocks), dim3(kAppendWarps * 32), (size_t)kAppendWarps * D * sizeof(float),
-                                      (cudaStream_t)stream, p));
+        MYNN_CUDA_OK(launch_dependent(paged_append_any_kernel<T>, dim3((unsigned)blocks), dim3(kAppendWarps * 32), (size_t)kAppendWarps * D * sizeof(float), st, p));
     });
-    MYNN_LAUNCH_OK("paged_append_kernel");
+    MYNN_LAUNCH_OK("paged_append_any_kernel");
     return MYNN_OK;
 }
