@@ -8,7 +8,8 @@
 // The visible rows are cut into tiles of kPagedTile positions, and all tiles of all (sequence, kv head) pairs, one pair behind the other, are
 // dealt out evenly: each CTA takes one run of `share` tiles, which may end one pair, hold a few whole ones and begin another.  A pair that
 // lies in one CTA is finished there; the parts of the others go to a workspace and are joined by a second kernel.  A CTA has at most two parts:
-// the pair its run begins inside of (slot 0) and the pair it ends inside of (slot 1).  The lengths are on the device, so every CTA works out the division itself.
+// the pair its run begins inside of (slot 0) and the pair it ends inside of (slot 1); it records the one that begins in it and ends elsewhere.  The lengths are on
+// the device, so every CTA works out the division itself.  Where the block table has room for a few tiles only, a pair is not worth cutting: each has a CTA.
 #pragma once
 #include <limits.h>
 
@@ -29,7 +30,9 @@ struct PagedAttention {
     int page, pages, width;  // rows of a page, pages of the cache, pages in a row of the table
     int row_blocks, block_rows;  // the group * S query rows of a pair, row r = head * S + s, in blocks
     int round;                   // shares are multiples of it: the tiles that the warps of a CTA take at a time
+    int4 *records;               // per CTA the pair that begins in it and ends in another: {b, h, last CTA, slot}, or b == -1
     float *ws;                   // [row block][CTA][2] parts of block_rows * (D + 2) floats: rows, then maxima, then sums
+    int whole;                   // each pair is left to a CTA of its own
 };
 
 // What the new queries of a sequence see: the tiles of the first tokens, then those from the oldest query's window on.
@@ -81,11 +84,46 @@ __device__ __forceinline__ long long paged_share(long long total, int ctas, int 
     return max((s + round - 1) / round, 1ll) * round;
 }
 
+// What a CTA takes one after the other: tiles t0 .. t1 - 1 of pair (b, h).
+struct PagedRun {
+    int b, h, t0, t1;
+    long long share, left;
+    int4 record;
+    bool first;
+    __device__ __forceinline__ void begin(const PagedAttention &p, const PagedShare &s) {
+        b = s.b, h = s.h, t0 = s.t;
+        share = left = s.share;
+        record = make_int4(-1, 0, 0, 0);
+        first = true;
+    }
+    // On to the next pair that has tiles; false: there is none.
+    __device__ __forceinline__ bool more(const PagedAttention &p, PagedSpan &sp) {
+        for (; b < p.B && left > 0; b++, h = t0 = 0) {
+            sp = paged_span(p, b);
+            if (sp.tiles == 0) continue;
+            t1 = (int)min((long long)sp.tiles, t0 + left);
+            if (t0 == 0 && t1 < sp.tiles) record = make_int4(b, h, blockIdx.x + (int)((sp.tiles - t1 + share - 1) / share), first ? 0 : 1);
+            return true;
+        }
+        return false;
+    }
+    __device__ __forceinline__ void advance(const PagedAttention &p) {
+        left -= t1 - t0;
+        t0 = 0;
+        first = false;
+        if (++h == p.G) h = 0, b++;
+    }
+};
+
 // Called by all threads of a CTA: the total number of tiles and the place of tile cta * share.  Each thread sums a run of sequences.
 template <int THREADS>
 __device__ __forceinline__ PagedShare paged_find(const PagedAttention &p, int cta, int ctas) {
     __shared__ long long warp_sums[THREADS / 32];
     __shared__ PagedShare found;
+    if (p.whole) {
+        const int b = cta / p.G, n = paged_span(p, b).tiles;
+        return {0, n, b, cta - b * p.G, 0};
+    }
     const int per = (p.B + THREADS - 1) / THREADS, b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     long long mine = 0;

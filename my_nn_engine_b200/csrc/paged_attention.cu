@@ -40,22 +40,16 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32) paged_attention_plain_ke
     float *sq = sm, *ring = sm + RB * PITCH + warp * (2 * 2 * TILE * PITCH), *weights = sm + RB * PITCH + W * (2 * 2 * TILE * PITCH) + warp * TILE * RB;
     for (int i = threadIdx.x; i < RB * PITCH; i += W * 32) sq[i] = 0.f;
     for (int i = lane; i < 2 * 2 * TILE * PITCH; i += 32) ring[i] = 0.f;  // what lies behind D is never written again
-    const PagedShare run = paged_find<W * 32>(p, cta, ctas);
     auto place = [&](int b, int h, int r, int d) { return (((size_t)b * p.S + r % p.S) * p.Hq + h * p.group + r / p.S) * D + d; };
-    for (int b = cta; b < p.B; b += ctas)  // sequences that see nothing at all belong to no run
+    for (int b = cta; b < p.B; b += ctas)  // sequences that see nothing at all are in no CTA's run
         if (paged_span(p, b).tiles == 0)
             for (int i = threadIdx.x; i < p.G * rows * D; i += W * 32)
                 reinterpret_cast<T *>(p.out)[place(b, i / (rows * D), r0 + i / D % rows, i % D)] = from_f32<T>(0.f);
-    int b = run.b, h = run.h, t0 = run.t;
-    long long left = run.share;
-    for (bool first = true; b < p.B && left > 0; first = false) {
-        const PagedSpan sp = paged_span(p, b);
-        if (sp.tiles == 0) {
-            b++;
-            h = t0 = 0;
-            continue;
-        }
-        const int t1 = (int)min((long long)sp.tiles, t0 + left);
+    PagedRun run;
+    run.begin(p, paged_find<W * 32>(p, cta, ctas));
+    PagedSpan sp;
+    for (; run.more(p, sp); run.advance(p)) {
+        const int b = run.b, h = run.h, t0 = run.t0, t1 = run.t1;
         __syncthreads();
         for (int i = threadIdx.x; i < rows * D; i += W * 32) {
             const int r = r0 + i / D;
@@ -160,7 +154,7 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32) paged_attention_plain_ke
         }
         __syncthreads();
         const bool whole = t0 == 0 && t1 == sp.tiles;
-        float *part = p.ws + (((size_t)blockIdx.y * ctas + cta) * 2 + (first ? 0 : 1)) * RB * (D + 2);
+        float *part = p.ws + (((size_t)blockIdx.y * ctas + cta) * 2 + (run.first ? 0 : 1)) * RB * (D + 2);
         for (int i = threadIdx.x; i < rows * D; i += W * 32) {
             const int r = i / D;
             float top = -INFINITY, L = 0.f, O = 0.f;
@@ -183,13 +177,8 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32) paged_attention_plain_ke
         __syncthreads();
         // the stages' columns behind D are zeros again
         for (int i = lane; i < 2 * 2 * TILE * PITCH; i += 32) ring[i] = 0.f;
-        left -= t1 - t0;
-        t0 = 0;
-        if (++h == p.G) {
-            h = 0;
-            b++;
-        }
     }
+    if (blockIdx.y == 0 && threadIdx.x == 0 && !p.whole) p.records[cta] = run.record;
 }
 
 // ---- 16-bit caches on the tensor cores --------------------------------------------------------------------------------
@@ -241,8 +230,7 @@ __global__ void __launch_bounds__(128, MmaShape<DP, NT, RW>::CTAS) paged_attenti
     uint8_t *ring = raw + (size_t)team * STAGES * Shape::TILE_BYTES;
     float4 *peers = reinterpret_cast<float4 *>(raw + (size_t)TEAMS * STAGES * Shape::TILE_BYTES);
     const uint32_t ring_at = smem_u32(ring);
-    const PagedShare run = paged_find<W * 32>(p, cta, ctas);
-    for (int b = cta; b < p.B; b += ctas)  // sequences that see nothing at all belong to no run
+    for (int b = cta; b < p.B; b += ctas)  // sequences that see nothing at all are in no CTA's run
         if (blockIdx.y == 0 && paged_span(p, b).tiles == 0)
             for (size_t n = (size_t)p.S * p.Hq * D / 8, i = threadIdx.x; i < n; i += W * 32) reinterpret_cast<uint4 *>(p.out)[b * n + i] = make_uint4(0, 0, 0, 0);
     auto team_sync = [&]() {
@@ -252,16 +240,11 @@ __global__ void __launch_bounds__(128, MmaShape<DP, NT, RW>::CTAS) paged_attenti
     // the rows of this lane: 0 (and 1) are accumulator row g (and g + 8), mine[2 n + e] are the columns 8 n + 2 t + e of the second product
     auto row_index = [&](int i) { return r0 + member * 8 * NT + i; };
     const float unit = p.scale * kLog2e;
-    int b = run.b, h = run.h, t0 = run.t;
-    long long left = run.share;
-    for (bool first = true; b < p.B && left > 0; first = false) {
-        const PagedSpan sp = paged_span(p, b);
-        if (sp.tiles == 0) {
-            b++;
-            h = t0 = 0;
-            continue;
-        }
-        const int t1 = (int)min((long long)sp.tiles, t0 + left);
+    PagedRun run;
+    run.begin(p, paged_find<W * 32>(p, cta, ctas));
+    PagedSpan sp;
+    for (; run.more(p, sp); run.advance(p)) {
+        const int b = run.b, h = run.h, t0 = run.t0, t1 = run.t1;
         const int mine = t0 + team < t1 ? (t1 - t0 - team + TEAMS - 1) / TEAMS : 0;
         const int oldest = sp.len - sp.count;
         // last position that a row sees, -1: the row is no query
@@ -482,7 +465,7 @@ __global__ void __launch_bounds__(128, MmaShape<DP, NT, RW>::CTAS) paged_attenti
         }
         if (team == 0) {
             const bool whole = t0 == 0 && t1 == sp.tiles;
-            float *part = p.ws + (((size_t)blockIdx.y * ctas + cta) * 2 + (first ? 0 : 1)) * Shape::ROWS * (D + 2);
+            float *part = p.ws + (((size_t)blockIdx.y * ctas + cta) * 2 + (run.first ? 0 : 1)) * Shape::ROWS * (D + 2);
 #pragma unroll
             for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -520,76 +503,93 @@ __global__ void __launch_bounds__(128, MmaShape<DP, NT, RW>::CTAS) paged_attenti
                 }
             }
         }
-        left -= t1 - t0;
-        t0 = 0;
-        if (++h == p.G) {
-            h = 0;
-            b++;
-        }
     }
+    if (blockIdx.y == 0 && threadIdx.x == 0 && !p.whole) p.records[cta] = run.record;
 }
 
 // ---- parts of pairs that lie in several CTAs ------------------------------------------------------------------------------
-constexpr int kJoinThreads = 256;
-template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(const PagedAttention p, int ctas) {
-    __shared__ long long sums[2][kJoinThreads / 32];
+// grid (CTAs of the kernel in front, row groups): a CTA takes `rows` rows (1, 2, 4 or 8) of the pair that the CTA of its number recorded, 8 / rows warps
+// each; the parts of a row are dealt out to its warps, eight at a time and loads first.  V: floats of a load.
+constexpr int kJoinWarps = 8;
+template <typename T, int V>
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_attention_join_kernel(const PagedAttention p, int ctas, int rows) {
+    constexpr int ITEMS = 8 / V, U = 8;
+    __shared__ float sums[kJoinWarps][256], weights[kJoinWarps];
     pdl_trigger();
     pdl_wait();
-    const int b = blockIdx.x / p.G, h = blockIdx.x - b * p.G, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    long long total = 0, before = 0;
-    for (int i = threadIdx.x; i < p.B; i += kJoinThreads) {
-        const long long n = (long long)paged_span(p, i).tiles * p.G;
-        total += n;
-        if (i < b) before += n;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        total += __shfl_xor_sync(0xffffffffu, total, o);
-        before += __shfl_xor_sync(0xffffffffu, before, o);
-    }
-    if (lane == 0) sums[0][warp] = total, sums[1][warp] = before;
-    __syncthreads();
-    total = before = 0;
-#pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; w++) total += sums[0][w], before += sums[1][w];
-    const int tiles = paged_span(p, b).tiles;
-    const long long share = paged_share(total, ctas, p.round), begin = before + (long long)h * tiles;
-    if (tiles == 0) return;
-    const int c0 = (int)(begin / share), c1 = (int)((begin + tiles - 1) / share);
-    if (c0 == c1) return;
-    const int R = p.block_rows, r0 = blockIdx.y * R, rows = min(p.group * p.S - r0, R), D = p.D;
-    const int slot = begin > c0 * share ? 1 : 0;
-    const float *parts = p.ws + (size_t)blockIdx.y * ctas * 2 * R * (D + 2);
-    auto part = [&](int c) { return parts + ((size_t)c * 2 + (c == c0 ? slot : 0)) * R * (D + 2); };
-    for (int i = threadIdx.x; i < rows * D; i += kJoinThreads) {
-        const int r = i / D;
-        float top = -INFINITY, L = 0.f, O = 0.f;
-        for (int c = c0; c <= c1; c += 8) {
-            float ms[8], ls[8], os[8], now = top;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const bool in = c + j <= c1;
-                const float *from = part(in ? c + j : c1);
-                ms[j] = in ? from[R * D + r] : -INFINITY;
-                ls[j] = in ? from[R * D + R + r] : 0.f;
-                os[j] = in ? from[i] : 0.f;
-                now = fmaxf(now, ms[j]);
+    const int4 rec = p.records[blockIdx.x];
+    if (rec.x < 0) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = kJoinWarps / rows, sub = warp & (per - 1);
+    const int c0 = blockIdx.x, n = rec.z - c0 + 1, R = p.block_rows, D = p.D;
+    const int r = blockIdx.y * rows + warp / per, block = r / R, i0 = r - block * R;
+    const bool in = r < p.group * p.S;
+    const float *parts = p.ws + (size_t)block * ctas * 2 * R * (D + 2);
+    auto part = [&](int c) { return parts + ((size_t)(c0 + c) * 2 + (c == 0 ? rec.w : 0)) * R * (D + 2); };
+    float top = -INFINITY, L = 0.f, O[ITEMS][V] = {};
+    if (in) {
+        for (int c = lane; c < n; c += 32) top = fmaxf(top, part(c)[R * D + i0]);
+        top = warp_max(top);
+        const float ref = merge_reference(top);
+        for (int c = sub; c < n; c += per * U) {
+            const int mine = c + per * (lane & (U - 1));
+            float f = 0.f;
+            if (mine < n) {
+                const float *from = part(mine) + R * D + i0;
+                f = expf(from[0] - ref);
+                L += lane < U ? f * from[R] : 0.f;
             }
-            const float ref = merge_reference(now), keep = expf(top - ref);
-            L *= keep;
-            O *= keep;
+            float v[U][ITEMS][V];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float f = expf(ms[j] - ref);
-                L += ls[j] * f;
-                O += os[j] * f;
+            for (int u = 0; u < U; u++) {
+                const float *from = part(min(c + per * u, n - 1)) + (size_t)i0 * D;
+#pragma unroll
+                for (int k = 0; k < ITEMS; k++) {
+                    const int d = V * (lane + 32 * k);
+                    if constexpr (V == 4) {
+                        const float4 x = d < D ? *reinterpret_cast<const float4 *>(from + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        v[u][k][0] = x.x, v[u][k][1] = x.y, v[u][k][2] = x.z, v[u][k][3] = x.w;
+                    } else {
+                        v[u][k][0] = d < D ? from[d] : 0.f;
+                    }
+                }
             }
-            top = now;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const float fu = __shfl_sync(0xffffffffu, f, u);
+                if (c + per * u < n)
+#pragma unroll
+                    for (int k = 0; k < ITEMS; k++)
+#pragma unroll
+                        for (int e = 0; e < V; e++) O[k][e] += fu * v[u][k][e];
+            }
         }
-        const int row = r0 + r;
-        reinterpret_cast<T *>(p.out)[(((size_t)b * p.S + row % p.S) * p.Hq + h * p.group + row / p.S) * D + i - r * D] = from_f32<T>(paged_quotient(O, L));
+        L = warp_sum(L);
     }
+    if (per > 1) {
+        if (lane == 0) weights[warp] = L;
+#pragma unroll
+        for (int k = 0; k < ITEMS; k++)
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                if (V * (lane + 32 * k) < D) sums[warp][V * (lane + 32 * k) + e] = O[k][e];
+        __syncthreads();
+        if (sub > 0) return;
+        for (int w = 1; w < per; w++) {
+            L += weights[warp + w];
+#pragma unroll
+            for (int k = 0; k < ITEMS; k++)
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                    if (V * (lane + 32 * k) < D) O[k][e] += sums[warp + w][V * (lane + 32 * k) + e];
+        }
+    }
+    if (!in) return;
+    T *out = reinterpret_cast<T *>(p.out) + (((size_t)rec.x * p.S + r % p.S) * p.Hq + rec.y * p.group + r / p.S) * D;
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++)
+#pragma unroll
+        for (int e = 0; e < V; e++)
+            if (V * (lane + 32 * k) < D) out[V * (lane + 32 * k) + e] = from_f32<T>(paged_quotient(O[k][e], L));
 }
 
 // How the launch is cut: kernel, query rows of a block, CTAs.
@@ -597,8 +597,12 @@ struct PagedPlan {
     bool mma;
     int dim, tiles_of_rows, team;  // padded head dimension, 8-row blocks of a warp, warps of a team
     int ctas, block_rows, row_blocks, round;
-    size_t bytes(int D) const { return (size_t)ctas * row_blocks * 2 * block_rows * (D + 2) * sizeof(float); }
+    bool whole;
+    size_t bytes(int D) const { return whole ? 16 : (size_t)ctas * sizeof(int4) + (size_t)ctas * row_blocks * 2 * block_rows * (D + 2) * sizeof(float); }
 };
+
+// Tiles of a pair up to which it is not cut.
+constexpr int kPagedWhole = 32;
 
 static int paged_sms(int *sms) {
     int dev = 0;
@@ -617,9 +621,9 @@ static PagedPlan paged_plan(int B, int S, int Hq, int Hkv, int D, int page, int 
     n.block_rows = mma ? 8 * n.tiles_of_rows * n.team : kPlainRows;
     n.row_blocks = (R + n.block_rows - 1) / n.block_rows;
     n.round = mma || D <= 128 ? 4 : kPlainWarps<8>;
-    const long long tiles = ((long long)width * page + kPagedTile - 1) / kPagedTile * Hkv * B;
-    const int most = mma && n.dim <= 128 ? 2 * sms : sms;
-    n.ctas = (int)std::min<long long>(most, std::max<long long>(1, (tiles + n.round - 1) / n.round));
+    const long long tiles = ((long long)width * page + kPagedTile - 1) / kPagedTile, most = mma && n.dim <= 128 ? 2 * sms : sms;
+    n.whole = tiles <= kPagedWhole;
+    n.ctas = n.whole ? B * Hkv : (int)std::min<long long>(most, std::max<long long>(1, (tiles * Hkv * B + n.round - 1) / n.round));
     return n;
 }
 
@@ -705,7 +709,9 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
     p.B = B, p.S = S, p.Hq = Hq, p.G = Hkv, p.group = Hq / Hkv, p.D = D;
     p.page = page, p.pages = pages, p.width = table_pages;
     p.row_blocks = n.row_blocks, p.block_rows = n.block_rows, p.round = n.round;
-    p.ws = reinterpret_cast<float *>(workspace);
+    p.whole = n.whole;
+    p.records = reinterpret_cast<int4 *>(workspace);
+    p.ws = reinterpret_cast<float *>(p.records + (n.whole ? 0 : n.ctas));
     const cudaStream_t st = (cudaStream_t)stream;
     const int vec = D % 4 == 0 && ((uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0 ? 4 : 1;
     MYNN_DISPATCH_DTYPE(dtype, T, {
@@ -718,7 +724,11 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
         else if (D <= 128) e = launch_plain<T, 4>(st, p, n.ctas, vec);
         else e = launch_plain<T, 8>(st, p, n.ctas, vec);
         if (e != MYNN_OK) return e;
-        MYNN_CUDA_OK(launch_dependent(paged_attention_join_kernel<T>, dim3(B * Hkv, n.row_blocks), dim3(kJoinThreads), 0, st, p, n.ctas));
+        if (n.whole) return MYNN_OK;
+        const int R = p.group * S, rows = R == 1 ? 1 : R == 2 ? 2 : R <= 4 ? 4 : 8;
+        const dim3 grid(n.ctas, (R + rows - 1) / rows), block(kJoinWarps * 32);
+        if (D % 4 == 0) MYNN_CUDA_OK(launch_dependent(paged_attention_join_kernel<T, 4>, grid, block, 0, st, p, n.ctas, rows));
+        else MYNN_CUDA_OK(launch_dependent(paged_attention_join_kernel<T, 1>, grid, block, 0, st, p, n.ctas, rows));
         MYNN_LAUNCH_OK("paged_attention_join_kernel");
     });
     return MYNN_OK;
