@@ -42,33 +42,35 @@ struct DrawRow {
         const double w = (double)a - (double)c;
         return i != without && w > 0.0 ? w : 0.0;
     }
-    // Weights of tokens at + VEC * lane + 32 VEC u (u < U), those behind `end` zero: loads first.
-    template <int VEC, int U>
-    __device__ __forceinline__ void load(int at, int end, int lane, double (&w)[U][VEC]) const {
-        __align__(16) T a[U][VEC], c[U][VEC];
+};
+
+// Numbers at + VEC * lane + 32 VEC u (u < U) of the row's two parts, zeros from `end` on.
+template <typename T, int VEC, int U>
+struct DrawPieces {
+    __align__(16) T a[U][VEC], c[U][VEC];
+    __device__ __forceinline__ void load(const DrawRow<T> &row, int at, int end, int lane) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int i = at + VEC * (lane + 32 * u);
             if constexpr (VEC > 1) {
-                *reinterpret_cast<uint4 *>(a[u]) = i < end ? __ldg(reinterpret_cast<const uint4 *>(p + i)) : make_uint4(0, 0, 0, 0);
-                *reinterpret_cast<uint4 *>(c[u]) = q && i < end ? __ldg(reinterpret_cast<const uint4 *>(q + i)) : make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4 *>(a[u]) = i < end ? __ldg(reinterpret_cast<const uint4 *>(row.p + i)) : make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4 *>(c[u]) = row.q && i < end ? __ldg(reinterpret_cast<const uint4 *>(row.q + i)) : make_uint4(0, 0, 0, 0);
             } else {
-                a[u][0] = i < end ? p[i] : from_f32<T>(0.f);
-                c[u][0] = q && i < end ? q[i] : from_f32<T>(0.f);
+                a[u][0] = i < end ? row.p[i] : from_f32<T>(0.f);
+                c[u][0] = row.q && i < end ? row.q[i] : from_f32<T>(0.f);
             }
         }
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int e = 0; e < VEC; e++) w[u][e] = weight(to_f32<T>(a[u][e]), to_f32<T>(c[u][e]), at + VEC * (lane + 32 * u) + e);
+    }
+    __device__ __forceinline__ double weight(const DrawRow<T> &row, int at, int lane, int u, int e) const {
+        return row.weight(to_f32<T>(a[u][e]), to_f32<T>(c[u][e]), at + VEC * (lane + 32 * u) + e);
     }
 };
 
 // grid (cluster, B).  VEC: elements of a 16-byte piece where all rows begin on 16 bytes, else 1.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kVerifyWarps * 32, 3) verify_draft_kernel(const VerifyDraft p) {
-    constexpr int U = VEC == 1 ? 8 : 16 / VEC;  // pieces of a lane in flight per row: 8 x 1, 4 x 4 or 2 x 8 numbers
-    constexpr int STEP = 32 * VEC * U;
+__global__ void __launch_bounds__(kVerifyWarps * 32, 4) verify_draft_kernel(const VerifyDraft p) {
+    constexpr int U = VEC == 1 ? 8 : 2;  // pieces of a lane in flight per row: 8 x 1, 2 x 4 or 2 x 8 numbers
+    constexpr int STEP = 32 * VEC * U, GROUPS = 4;
     __shared__ double sums[kVerifyWarps], whole[2];
     __shared__ int pick;
     pdl_trigger();
@@ -101,19 +103,28 @@ __global__ void __launch_bounds__(kVerifyWarps * 32, 3) verify_draft_kernel(cons
     // parts of whole steps: the cluster's ranks in order, in each its warps
     const int parts = ranks * kVerifyWarps, per = ((V + parts - 1) / parts + 32 * VEC - 1) / (32 * VEC) * (32 * VEC);
     const int lo = (int)min((long long)(rank * kVerifyWarps + warp) * per, (long long)V), hi = min(lo + per, V);
+    const int stride = (per + GROUPS * STEP - 1) / (GROUPS * STEP) * STEP;  // a part is summed in up to four groups, so that little of it is read again
+    double group[GROUPS];
     double total = 0.0, before = 0.0, mine = 0.0;
     bool chosen = false;
     for (int pass = 0;; pass++) {
-        double w[U][VEC], sum = 0.0;
-        for (int at = lo; at < hi; at += STEP) {
-            row.template load<VEC, U>(at, hi, lane, w);
 #pragma unroll
-            for (int u = 0; u < U; u++)
+        for (int k = 0; k < GROUPS; k++) {
+            group[k] = 0.0;
+            const int end = min(lo + (k + 1) * stride, hi);
+#pragma unroll 1
+            for (int at = lo + k * stride; at < end; at += STEP) {
+                DrawPieces<T, VEC, U> x;
+                x.load(row, at, end, lane);
 #pragma unroll
-                for (int e = 0; e < VEC; e++) sum += w[u][e];
+                for (int u = 0; u < U; u++)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) group[k] += x.weight(row, at, lane, u, e);
+            }
         }
-        sum = warp_sum_f64(sum);
-        if (lane == 0) sums[warp] = sum;
+#pragma unroll
+        for (int k = 0; k < GROUPS; k++) group[k] = warp_sum_f64(group[k]);
+        if (lane == 0) sums[warp] = (group[0] + group[1]) + (group[2] + group[3]);
         __syncthreads();
         mine = 0.0;
 #pragma unroll
@@ -159,20 +170,36 @@ __global__ void __launch_bounds__(kVerifyWarps * 32, 3) verify_draft_kernel(cons
             }
         }
         if (chosen && warp == at) {
-            int found = -1, last = -1;
-            for (int base = lo; base < hi && found < 0; base += STEP) {
-                double w[U][VEC], own[U], all[U];
-                row.template load<VEC, U>(base, hi, lane, w);
+            int found = -1, k0 = -1;
+            run = before;
+#pragma unroll
+            for (int k = 0; k < GROUPS; k++) {
+                if (group[k] > 0.0 && (k0 < 0 || run <= goal)) {
+                    k0 = k;
+                    before = run;
+                    run += group[k];
+                }
+            }
+            const int from = lo + k0 * stride, end = min(from + stride, hi);
+#pragma unroll 1
+            for (int base = from; base < end && found < 0; base += 32 * VEC * U) {
+                DrawPieces<T, VEC, U> x;
+                double own[U];
+                x.load(row, base, end, lane);
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     own[u] = 0.0;
 #pragma unroll
-                    for (int e = 0; e < VEC; e++) own[u] += w[u][e];
-                    all[u] = warp_sum_f64(own[u]);
+                    for (int e = 0; e < VEC; e++) own[u] += x.weight(row, base, lane, u, e);
                 }
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    if (found >= 0 || !(all[u] > 0.0)) continue;
+                    const double all = warp_sum_f64(own[u]);
+                    if (found >= 0) continue;
+                    if (!(before + all > goal)) {
+                        before += all;
+                        continue;
+                    }
                     double incl = own[u];
 #pragma unroll
                     for (int o = 1; o < 32; o <<= 1) {
@@ -180,26 +207,28 @@ __global__ void __launch_bounds__(kVerifyWarps * 32, 3) verify_draft_kernel(cons
                         if (lane >= o) incl += up;
                     }
                     double sum = before + (incl - own[u]);
-                    int over = -1, some = -1;
+                    int over = -1;
 #pragma unroll
                     for (int e = 0; e < VEC; e++) {
-                        sum += w[u][e];
-                        if (w[u][e] > 0.0) {
-                            some = e;
-                            if (over < 0 && sum > goal) over = e;
-                        }
+                        const double w = x.weight(row, base, lane, u, e);
+                        sum += w;
+                        if (over < 0 && w > 0.0 && sum > goal) over = e;
                     }
-                    const unsigned overs = __ballot_sync(0xffffffffu, over >= 0), somes = __ballot_sync(0xffffffffu, some >= 0);
+                    const unsigned overs = __ballot_sync(0xffffffffu, over >= 0);
                     if (overs) {
                         const int l = __ffs(overs) - 1;
                         found = base + VEC * (l + 32 * u) + __shfl_sync(0xffffffffu, over, l);
                     }
-                    const int l = 31 - __clz(somes);
-                    last = base + VEC * (l + 32 * u) + __shfl_sync(0xffffffffu, some, l);
-                    before += all[u];
+                    before += all;
                 }
             }
-            if (lane == 0) pick = found >= 0 ? found : last;
+            if (found < 0) {  // sums in another order, or a goal that was rounded up to the total: the last token with any weight
+                int last = -1;
+                for (int i = from + lane; i < end; i += 32)
+                    if (row.weight(to_f32<T>(row.p[i]), row.q ? to_f32<T>(row.q[i]) : 0.f, i) > 0.0) last = i;
+                found = __reduce_max_sync(0xffffffffu, last);
+            }
+            if (lane == 0) pick = found;
         }
         __syncthreads();
         for (int i = threadIdx.x; i <= K; i += kVerifyWarps * 32) p.tokens_out[(size_t)b * (K + 1) + i] = i < n ? p.tokens[(size_t)b * K + i] : i == n ? pick : -1;
