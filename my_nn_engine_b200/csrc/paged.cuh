@@ -33,6 +33,7 @@ struct PagedAttention {
     int4 *records;               // per CTA the pair that begins in it and ends in another: {b, h, last CTA, slot}, or b == -1
     float *ws;                   // [row block][CTA][2] parts of block_rows * (D + 2) floats: rows, then maxima, then sums
     int whole;                   // each pair is left to a CTA of its own
+    int strips;                  // tiles lie in one page each, and rows are as long on the chip as in the cache
 };
 
 // What the new queries of a sequence see: the tiles of the first tokens, then those from the oldest query's window on.

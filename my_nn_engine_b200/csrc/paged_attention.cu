@@ -182,21 +182,24 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32) paged_attention_plain_ke
 }
 
 // ---- 16-bit caches on the tensor cores --------------------------------------------------------------------------------
-// Bound by the one pass over the cache.  A team of RW warps takes tiles of 16 positions: cp.async brings a tile's rows, wherever their pages lie, to a ring of
-// STAGES tiles in shared memory, each warp a share of the rows, and each warp then multiplies the whole tile with 8 NT query rows of its own, so that a row of the
-// cache is read once for up to 64 query rows (all heads of a group, all drafts).  Both products are mma.m16n8k16 on fragments that are 16-byte pieces of
-// the rows, as in the attention over contiguous caches: S = Q K^T with the dimensions of a step permuted, O^T = V^T P^T with pairs of positions put together
-// by byte permutes; weights enter as a 16-bit part and its remainder (16 bits in all), scores, maxima and sums are f32.  D is padded to DP with zeros, on the chip
-// only.
-template <int DP, int NT, int RW>
+// Bound by the one pass over the cache.  A team of RW warps takes tiles of 16 positions: cp.async brings a tile's rows, wherever their pages lie, to a ring in shared
+// memory whose entries are the keys or the values of a tile, each warp a share of the rows, and each warp then multiplies the whole tile with eight query rows of its
+// own, so that a row of the cache is read once for up to 64 query rows (all heads of a group, all drafts).  Both products are mma.m16n8k16 on fragments that
+// are 16-byte pieces of the rows, as in the attention over contiguous caches: S = Q K^T with the dimensions of a step permuted, O^T = V^T P^T with pairs of
+// positions put together by byte permutes; weights enter as a 16-bit part and its remainder (16 bits in all), scores, maxima and sums are f32.  D is padded to DP with
+// zeros, on the chip only.
+// The chain of one tile is long (two products, a softmax) and each warp walks it alone, so warps are what hides it: sixteen per SM, eight query rows each, rather than
+// eight with sixteen rows (96 mixed sequences of heads of 64: eight warps per SM 97 us).
+template <int DP, int RW>
 struct MmaShape {
-    static constexpr int W = 4, TEAMS = W / RW, ROWS = 8 * NT * RW;
-    static constexpr int TILE_BYTES = 2 * kPagedTile * DP * 2;
+    static constexpr int W = 8, TEAMS = W / RW, ROWS = 8 * RW;
+    static constexpr int ENTRY = kPagedTile * DP * 2;
     static constexpr int CTAS = DP > 128 ? 1 : 2;  // per SM
-    static constexpr int STAGES = (CTAS == 2 ? 96 : 192) * 1024 / TEAMS / TILE_BYTES;
-    static constexpr int ACC = DP / 16 * NT * 4;   // accumulators of a lane
-    static constexpr int PEERS = TEAMS == 1 ? 0 : W / 2;
-    static constexpr size_t SMEM = (size_t)TEAMS * STAGES * TILE_BYTES + (size_t)PEERS * ACC * 32 * 4;
+    static constexpr int FIT = (CTAS == 2 ? 96 : 192) * 1024 / TEAMS / ENTRY;
+    static constexpr int AHEAD = FIT >= 9 ? 4 : (FIT - 1) / 2, STAGES = 2 * AHEAD + 1;  // tiles on their way while one is worked on
+    static constexpr int ACC = DP / 4;  // accumulators of a lane
+    static constexpr size_t RING = (size_t)TEAMS * STAGES * ENTRY, PEERS = TEAMS == 1 ? 0 : (size_t)W / 2 * ACC * 32 * 4;
+    static constexpr size_t SMEM = RING > PEERS ? RING : PEERS;
 };
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -209,26 +212,27 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // 2 i + 1 (values) are in different banks.
 __device__ __forceinline__ int paged_swizzle(int row, int c) { return c ^ (row & 6) ^ ((row & 1) << 2); }
 
+__device__ __forceinline__ void copy16_now(uint32_t smem, const void *gmem) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory"); }
+
 template <typename T>
 __device__ __forceinline__ bool has_special(uint32_t x) {  // infinity or NaN in one of two 16-bit numbers
     constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
     return (x & e) == e || (x >> 16 & e) == e;
 }
 
-template <typename T, int DP, int NT, int RW>
-__global__ void __launch_bounds__(128, MmaShape<DP, NT, RW>::CTAS) paged_attention_mma_kernel(const PagedAttention p) {
-    using Shape = MmaShape<DP, NT, RW>;
-    constexpr int W = Shape::W, TEAMS = Shape::TEAMS, STAGES = Shape::STAGES, TILE = kPagedTile, KCH = DP / 32, VH = DP / 64, CPR = DP / 8;
+template <typename T, int DP, int RW>
+__global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_mma_kernel(const PagedAttention p) {
+    using Shape = MmaShape<DP, RW>;
+    constexpr int W = Shape::W, TEAMS = Shape::TEAMS, STAGES = Shape::STAGES, AHEAD = Shape::AHEAD, TILE = kPagedTile, KCH = DP / 32, VH = DP / 64, CPR = DP / 8;
     constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
     extern __shared__ __align__(128) uint8_t raw[];
-    __shared__ uint32_t there[W][STAGES];       // which rows of a tile exist
-    __shared__ float peer_m[W][16], peer_l[W][16];
+    __shared__ float peer_m[W / 2][8], peer_l[W / 2][8];
     pdl_trigger();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, team = warp / RW, member = warp % RW;
-    const int cta = blockIdx.x, ctas = gridDim.x, D = p.D, R = p.group * p.S, r0 = blockIdx.y * Shape::ROWS;
-    uint8_t *ring = raw + (size_t)team * STAGES * Shape::TILE_BYTES;
-    float4 *peers = reinterpret_cast<float4 *>(raw + (size_t)TEAMS * STAGES * Shape::TILE_BYTES);
+    const int cta = blockIdx.x, ctas = gridDim.x, D = p.D, R = p.group * p.S, r0 = blockIdx.y * Shape::ROWS + member * 8;
+    uint8_t *ring = raw + (size_t)team * STAGES * Shape::ENTRY;
+    float4 *peers = reinterpret_cast<float4 *>(raw);  // over the rings, when they are idle
     const uint32_t ring_at = smem_u32(ring);
     for (int b = cta; b < p.B; b += ctas)  // sequences that see nothing at all are in no CTA's run
         if (blockIdx.y == 0 && paged_span(p, b).tiles == 0)
@@ -237,8 +241,6 @@ __global__ void __launch_bounds__(128, MmaShape<DP, NT, RW>::CTAS) paged_attenti
         if constexpr (RW == 1) __syncwarp();
         else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(RW * 32) : "memory");
     };
-    // the rows of this lane: 0 (and 1) are accumulator row g (and g + 8), mine[2 n + e] are the columns 8 n + 2 t + e of the second product
-    auto row_index = [&](int i) { return r0 + member * 8 * NT + i; };
     const float unit = p.scale * kLog2e;
     PagedRun run;
     run.begin(p, paged_find<W * 32>(p, cta, ctas));
@@ -247,132 +249,151 @@ __global__ void __launch_bounds__(128, MmaShape<DP, NT, RW>::CTAS) paged_attenti
         const int b = run.b, h = run.h, t0 = run.t0, t1 = run.t1;
         const int mine = t0 + team < t1 ? (t1 - t0 - team + TEAMS - 1) / TEAMS : 0;
         const int oldest = sp.len - sp.count;
-        // last position that a row sees, -1: the row is no query
+        // last position that row r0 + i sees, -1: it is no query
         auto last_seen = [&](int i) {
-            const int r = row_index(i);
+            const int r = r0 + i;
             return r < R && r % p.S < sp.count ? oldest + r % p.S : -1;
         };
-        int at[NT];
-#pragma unroll
-        for (int n = 0; n < NT; n++) at[n] = last_seen(8 * n + g);
+        const int at = last_seen(g);
         auto sees = [&](int last, int j) { return j <= last && (p.window <= 0 || last - j < p.window || j < p.sinks); };
-        auto row_of = [&](int j) { return j < mine ? paged_row(p, sp, b, h, sp.base(t0 + team + TEAMS * j) + (lane & 15)) : -1; };
-        auto issue = [&](int j, int row) {
-            const int stage = j % STAGES;
-            const uint32_t to = ring_at + stage * Shape::TILE_BYTES;
-            const uint32_t exist = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
-            if (lane == 0) there[warp][stage] = exist;
-            if (j < mine) {
+        auto base_of = [&](int j) { return sp.base(t0 + team + TEAMS * j); };
+        // The first row of a tile whose sixteen rows lie one behind the other and are all seen, for 32 tiles at once, one per lane; -1 for others.
+        auto strips_of = [&](int j) {
+            const int pos = base_of(j);
+            if (j >= mine || !p.strips || pos + TILE > sp.rows || (p.window > 0 && oldest - pos >= p.window && pos + TILE > p.sinks)) return -1;
+            return paged_row(p, sp, b, h, pos);
+        };
+        auto row_of = [&](int j) { return j < mine ? paged_row(p, sp, b, h, base_of(j) + (lane & 15)) : -1; };
+        // The keys or the values of a tile to an entry of the ring.  strip: uniform; row: of position lane % 16, where strip < 0.
+        auto issue = [&](const void *rows, uint32_t entry, bool in_run, int strip, int row) {
+            constexpr int COPIES = (TILE * CPR + 32 * RW - 1) / (32 * RW);
+            if (in_run) {
+                if (strip >= 0) {
+                    const char *src = reinterpret_cast<const char *>(rows) + (size_t)(uint32_t)strip * (DP * 2) + (member * 32 + lane) * 16;
 #pragma unroll
-                for (int i = 0; i < TILE * CPR / 32 / RW; i++) {
-                    const int idx = (i * RW + member) * 32 + lane, r = idx / CPR, c = idx % CPR;
-                    const int from = __shfl_sync(0xffffffffu, row, r);
-                    const size_t src = (size_t)max(from, 0) * D + (8 * c < D ? 8 * c : 0);
-                    const bool in = from >= 0 && 8 * c < D;
-                    const uint32_t dst = to + r * (DP * 2) + (c >> 3) * 128 + paged_swizzle(r, c & 7) * 16;
-                    copy16_at(dst, reinterpret_cast<const T *>(p.k) + src, in);
-                    copy16_at(dst + TILE * DP * 2, reinterpret_cast<const T *>(p.v) + src, in);
+                    for (int i = 0; i < COPIES; i++) {
+                        const int idx = (i * RW + member) * 32 + lane, r = idx / CPR, c = idx % CPR;
+                        if (TILE * CPR % (32 * RW) != 0 && idx >= TILE * CPR) break;
+                        copy16_now(entry + r * (DP * 2) + (c >> 3) * 128 + paged_swizzle(r, c & 7) * 16, src + i * RW * 512);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < COPIES; i++) {
+                        const int idx = (i * RW + member) * 32 + lane, r = idx / CPR, c = idx % CPR;
+                        if (TILE * CPR % (32 * RW) != 0 && idx >= TILE * CPR) break;
+                        const int from = __shfl_sync(0xffffffffu, row, r & 15);
+                        const bool in = from >= 0 && 8 * c < D;
+                        const char *src = reinterpret_cast<const char *>(rows) + (size_t)(uint32_t)(in ? from : 0) * (uint32_t)(2 * D) + (in ? 16 * c : 0);
+                        copy16_at(entry + r * (DP * 2) + (c >> 3) * 128 + paged_swizzle(r, c & 7) * 16, src, in);
+                    }
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
-        team_sync();  // the ring is free
+        uint32_t exist[AHEAD + 1];  // which rows of the next tiles there are
+        team_sync();                // the ring is free
+        int strips = strips_of(lane), strips_next = strips_of(lane + 32), strip, row = -1;
 #pragma unroll
-        for (int j = 0; j < STAGES - 1; j++) issue(j, row_of(j));
-        int next = row_of(STAGES - 1);
+        for (int j = 0; j < AHEAD; j++) {
+            strip = __shfl_sync(0xffffffffu, strips, j);
+            if (strip < 0) row = row_of(j);
+            exist[j] = strip >= 0 ? 0xffffu : __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+            issue(p.k, ring_at + 2 * j * Shape::ENTRY, j < mine, strip, row);
+            issue(p.v, ring_at + (2 * j + 1) * Shape::ENTRY, j < mine, strip, row);
+        }
+        strip = __shfl_sync(0xffffffffu, strips, AHEAD);
+        if (strip < 0) row = row_of(AHEAD);
+        uint32_t cur = 0, free_entry = (STAGES - 1) * Shape::ENTRY;  // offsets: the entry that is read next, the one that is empty
 
-        uint2 qa[NT][2 * KCH];
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int r = min(row_index(8 * n + g), R - 1);
+        uint2 qa[2 * KCH];
+        {
+            const int r = min(r0 + g, R - 1);
             const T *qr = reinterpret_cast<const T *>(p.q) + (((size_t)b * p.Hq + h * p.group + r / p.S) * p.S + r % p.S) * D;
 #pragma unroll
             for (int i = 0; i < 2 * KCH; i++) {
                 const int d = 8 * (t + 4 * (i >> 1)) + 4 * (i & 1);
-                qa[n][i] = at[n] >= 0 && d < D ? *reinterpret_cast<const uint2 *>(qr + d) : make_uint2(0u, 0u);
+                qa[i] = at >= 0 && d < D ? *reinterpret_cast<const uint2 *>(qr + d) : make_uint2(0u, 0u);
             }
         }
-        float o[VH * 4][NT][4], m[NT], l[NT];
+        float o[VH * 4][4], m = -INFINITY, l = 0.f;
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            m[n] = -INFINITY, l[n] = 0.f;
+        for (int i = 0; i < VH * 4; i++)
 #pragma unroll
-            for (int i = 0; i < VH * 4; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) o[i][n][e] = 0.f;
-        }
+            for (int e = 0; e < 4; e++) o[i][e] = 0.f;
 #pragma unroll 1
         for (int j = 0; j < mine; j++) {
             asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-            team_sync();  // tile j is here, and tile j - 1 is done with
-            issue(j + STAGES - 1, next);
-            next = row_of(j + STAGES);
-            const uint8_t *K = ring + (j % STAGES) * Shape::TILE_BYTES, *V = K + TILE * DP * 2;
-            const int base = sp.base(t0 + team + TEAMS * j);
-            const uint32_t exist = there[warp][j % STAGES];
-            // ---- S = Q K^T: x[n][2 c + e] is row 8 n + g, position base + 8 c + 2 t + e ----
-            float x[NT][4];
+            team_sync();  // the keys of tile j are here, and the values of tile j - 1 are done with
+            const int ahead = j + AHEAD;
+            exist[AHEAD] = strip >= 0 ? 0xffffu : __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+            issue(p.k, ring_at + free_entry, ahead < mine, strip, row);
+            const int base = base_of(j);
+            const uint8_t *K = ring + cur;
+            free_entry = cur;
+            cur = cur + Shape::ENTRY == STAGES * Shape::ENTRY ? 0 : cur + Shape::ENTRY;
+            // ---- S = Q K^T: x[2 c + e] is row g, position base + 8 c + 2 t + e ----
+            float x[4];
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < KCH; i++) {
                     const uint4 kr = *reinterpret_cast<const uint4 *>(K + (8 * c + g) * (DP * 2) + (i >> 1) * 128 + paged_swizzle(g, t + 4 * (i & 1)) * 16);
-                    if constexpr (NT == 1) {
-                        mma_kv<T>(acc, qa[0][2 * i].x, 0u, qa[0][2 * i].y, 0u, kr.x, kr.y);
-                        mma_kv<T>(acc, qa[0][2 * i + 1].x, 0u, qa[0][2 * i + 1].y, 0u, kr.z, kr.w);
-                    } else {
-                        mma_kv<T>(acc, qa[0][2 * i].x, qa[1][2 * i].x, qa[0][2 * i].y, qa[1][2 * i].y, kr.x, kr.y);
-                        mma_kv<T>(acc, qa[0][2 * i + 1].x, qa[1][2 * i + 1].x, qa[0][2 * i + 1].y, qa[1][2 * i + 1].y, kr.z, kr.w);
-                    }
+                    mma_kv<T>(acc, qa[2 * i].x, 0u, qa[2 * i].y, 0u, kr.x, kr.y);
+                    mma_kv<T>(acc, qa[2 * i + 1].x, 0u, qa[2 * i + 1].y, 0u, kr.z, kr.w);
                 }
-#pragma unroll
-                for (int n = 0; n < NT; n++) x[n][2 * c] = acc[2 * n], x[n][2 * c + 1] = acc[2 * n + 1];
+                x[2 * c] = acc[0], x[2 * c + 1] = acc[1];
             }
-            const bool full = exist == 0xffffu && (p.S == 1 || paged_tile_full(p, sp, base));
-            uint32_t hi[NT][2], lo[NT][2];
-            float keep[NT];
-            bool moved = false;
+            const bool full = exist[0] == 0xffffu && (p.S == 1 || paged_tile_full(p, sp, base));
+            float top = -INFINITY;
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                float top = -INFINITY;
+            for (int i = 0; i < 4; i++) {
+                if (p.softcap > 0.f) x[i] = kLog2e * fast_soft_cap(x[i] * p.scale, p.softcap);
+                else x[i] *= unit;
+            }
+            if (!full) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    if (p.softcap > 0.f) x[n][i] = kLog2e * fast_soft_cap(x[n][i] * p.scale, p.softcap);
-                    else x[n][i] *= unit;
                     const int bit = 8 * (i >> 1) + 2 * t + (i & 1);
-                    if (!full && !((exist >> bit & 1) && sees(at[n], base + bit))) x[n][i] = -INFINITY;
-                    top = fmaxf(top, x[n][i]);
+                    if (!((exist[0] >> bit & 1) && sees(at, base + bit))) x[i] = -INFINITY;
                 }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float now = fmaxf(m[n], top), ref = merge_reference(now);
-                keep[n] = exp2_approx(m[n] - ref);
-                moved |= now > m[n];
-                m[n] = now;
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[n][i] = exp2_approx(x[n][i] - ref);
-                l[n] = l[n] * keep[n] + ((x[n][0] + x[n][1]) + (x[n][2] + x[n][3]));  // of this lane's positions
-                split_pack<T>(x[n][0], x[n][1], hi[n][0], lo[n][0]);
-                split_pack<T>(x[n][2], x[n][3], hi[n][1], lo[n][1]);
             }
+#pragma unroll
+            for (int i = 0; i < 4; i++) top = fmaxf(top, x[i]);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float now = fmaxf(m, top), ref = merge_reference(now), keep = exp2_approx(m - ref);
+            const bool moved = now > m;
+            m = now;
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = exp2_approx(x[i] - ref);
+            l = l * keep + ((x[0] + x[1]) + (x[2] + x[3]));  // of this lane's positions
+            uint32_t hi[2], lo[2];
+            split_pack<T>(x[0], x[1], hi[0], lo[0]);
+            split_pack<T>(x[2], x[3], hi[1], lo[1]);
             if (__any_sync(0xffffffffu, moved)) {
+                const float k0 = __shfl_sync(0xffffffffu, keep, 8 * t), k1 = __shfl_sync(0xffffffffu, keep, 8 * t + 4);
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    const float k0 = __shfl_sync(0xffffffffu, keep[n], 8 * t), k1 = __shfl_sync(0xffffffffu, keep[n], 8 * t + 4);
-#pragma unroll
-                    for (int i = 0; i < VH * 4; i++) o[i][n][0] *= k0, o[i][n][1] *= k1, o[i][n][2] *= k0, o[i][n][3] *= k1;
-                }
+                for (int i = 0; i < VH * 4; i++) o[i][0] *= k0, o[i][1] *= k1, o[i][2] *= k0, o[i][3] *= k1;
             }
-            // ---- O^T += V^T P^T: o[4 v + i][n] is dimensions 64 v + 8 g + 2 i (registers 0, 1) and + 1 (2, 3) of rows 8 n + 2 t and + 1 ----
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+            team_sync();  // the values of tile j are here, and its keys are done with
+            issue(p.v, ring_at + free_entry, ahead < mine, strip, row);
+            if (((ahead + 1) & 31) == 0) strips = strips_next, strips_next = strips_of(ahead + 33 + lane);
+            strip = __shfl_sync(0xffffffffu, strips, (ahead + 1) & 31);
+            if (strip < 0) row = row_of(ahead + 1);
+            const uint8_t *V = ring + cur;
+            free_entry = cur;
+            cur = cur + Shape::ENTRY == STAGES * Shape::ENTRY ? 0 : cur + Shape::ENTRY;
+            // ---- O^T += V^T P^T: o[4 v + i] is dimensions 64 v + 8 g + 2 i (registers 0, 1) and + 1 (2, 3) of rows 2 t and 2 t + 1 ----
             bool special = false;
 #pragma unroll
             for (int v = 0; v < VH; v++) {
                 uint32_t vr[4][4];
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int row = 2 * t + (r & 1) + 8 * (r >> 1);
-                    const uint4 u = *reinterpret_cast<const uint4 *>(V + row * (DP * 2) + v * 128 + paged_swizzle(row, g) * 16);
+                    const int vrow = 2 * t + (r & 1) + 8 * (r >> 1);
+                    const uint4 u = *reinterpret_cast<const uint4 *>(V + vrow * (DP * 2) + v * 128 + paged_swizzle(vrow, g) * 16);
                     vr[r][0] = u.x, vr[r][1] = u.y, vr[r][2] = u.z, vr[r][3] = u.w;
                 }
                 if (!full && p.S > 1) {
@@ -385,8 +406,10 @@ __global__ void __launch_bounds__(128, MmaShape<DP, NT, RW>::CTAS) paged_attenti
                 if (special) {
                     // A value that is no number, which not every row sees: position by position, added only where it is seen.  (What stands in
                     // `special` from the slab in front does no harm.)
+                    const int at0 = last_seen(2 * t), at1 = last_seen(2 * t + 1);
 #pragma unroll 1
                     for (int k = 0; k < TILE; k++) {
+                        const bool s0 = (exist[0] >> k & 1) && sees(at0, base + k), s1 = (exist[0] >> k & 1) && sees(at1, base + k);
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             uint32_t one[4];
@@ -394,16 +417,12 @@ __global__ void __launch_bounds__(128, MmaShape<DP, NT, RW>::CTAS) paged_attenti
                             for (int r = 0; r < 4; r++) one[r] = 2 * t + (r & 1) + 8 * (r >> 1) == k ? vr[r][i] : 0u;
                             const uint32_t a0 = __byte_perm(one[0], one[1], 0x5410u), a1 = __byte_perm(one[0], one[1], 0x7632u);
                             const uint32_t a2 = __byte_perm(one[2], one[3], 0x5410u), a3 = __byte_perm(one[2], one[3], 0x7632u);
-#pragma unroll
-                            for (int n = 0; n < NT; n++) {
-                                float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                                mma_kv<T>(acc, a0, a1, a2, a3, hi[n][0], hi[n][1]);
-                                mma_kv<T>(acc, a0, a1, a2, a3, lo[n][0], lo[n][1]);
-                                const bool s0 = (exist >> k & 1) && sees(last_seen(8 * n + 2 * t), base + k), s1 = (exist >> k & 1) && sees(last_seen(8 * n + 2 * t + 1), base + k);
-                                float(&to)[4] = o[4 * v + i][n];
-                                if (s0) to[0] += acc[0], to[2] += acc[2];
-                                if (s1) to[1] += acc[1], to[3] += acc[3];
-                            }
+                            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma_kv<T>(acc, a0, a1, a2, a3, hi[0], hi[1]);
+                            mma_kv<T>(acc, a0, a1, a2, a3, lo[0], lo[1]);
+                            float(&to)[4] = o[4 * v + i];
+                            if (s0) to[0] += acc[0], to[2] += acc[2];
+                            if (s1) to[1] += acc[1], to[3] += acc[3];
                         }
                     }
                     continue;
@@ -412,53 +431,42 @@ __global__ void __launch_bounds__(128, MmaShape<DP, NT, RW>::CTAS) paged_attenti
                 for (int i = 0; i < 4; i++) {
                     const uint32_t a0 = __byte_perm(vr[0][i], vr[1][i], 0x5410u), a1 = __byte_perm(vr[0][i], vr[1][i], 0x7632u);
                     const uint32_t a2 = __byte_perm(vr[2][i], vr[3][i], 0x5410u), a3 = __byte_perm(vr[2][i], vr[3][i], 0x7632u);
-#pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        mma_kv<T>(o[4 * v + i][n], a0, a1, a2, a3, hi[n][0], hi[n][1]);
-                        mma_kv<T>(o[4 * v + i][n], a0, a1, a2, a3, lo[n][0], lo[n][1]);
-                    }
+                    mma_kv<T>(o[4 * v + i], a0, a1, a2, a3, hi[0], hi[1]);
+                    mma_kv<T>(o[4 * v + i], a0, a1, a2, a3, lo[0], lo[1]);
                 }
             }
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) exist[i] = exist[i + 1];
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-            l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
-            l[n] += __shfl_xor_sync(0xffffffffu, l[n], 2);
-            if (at[n] < 0) m[n] = -INFINITY, l[n] = 0.f;  // a row that is no query, which tiles that all see are not masked for
-        }
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (at < 0) m = -INFINITY, l = 0.f;  // a row that is no query, which tiles that all see are not masked for
         // ---- the teams meet: half of them hand their sums to the other half, register by register ----
+        if constexpr (TEAMS > 1) __syncthreads();  // the rings are idle
 #pragma unroll
         for (int half = TEAMS / 2; half > 0; half >>= 1) {
             const int slot = (team - half) * RW + member;
             if (team >= half && team < 2 * half) {
 #pragma unroll
-                for (int i = 0; i < VH * 4; i++)
-#pragma unroll
-                    for (int n = 0; n < NT; n++) peers[(slot * (Shape::ACC / 4) + i * NT + n) * 32 + lane] = *reinterpret_cast<const float4 *>(o[i][n]);
-                if (t == 0) {
-#pragma unroll
-                    for (int n = 0; n < NT; n++) peer_m[slot][8 * n + g] = m[n], peer_l[slot][8 * n + g] = l[n];
-                }
+                for (int i = 0; i < VH * 4; i++) peers[(slot * (Shape::ACC / 4) + i) * 32 + lane] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+                if (t == 0) peer_m[slot][g] = m, peer_l[slot][g] = l;
             }
             __syncthreads();
             if (team < half) {
                 const int from = team * RW + member;
+                const float m2 = peer_m[from][g], now = fmaxf(m, m2), ref = merge_reference(now), f = exp2_approx(m - ref), f2 = exp2_approx(m2 - ref);
+                m = now;
+                l = l * f + peer_l[from][g] * f2;
+                const float a = __shfl_sync(0xffffffffu, f, 8 * t), c = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+                const float a2 = __shfl_sync(0xffffffffu, f2, 8 * t), c2 = __shfl_sync(0xffffffffu, f2, 8 * t + 4);
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    const float m2 = peer_m[from][8 * n + g], top = fmaxf(m[n], m2), ref = merge_reference(top), f = exp2_approx(m[n] - ref), f2 = exp2_approx(m2 - ref);
-                    m[n] = top;
-                    l[n] = l[n] * f + peer_l[from][8 * n + g] * f2;
-                    const float a = __shfl_sync(0xffffffffu, f, 8 * t), c = __shfl_sync(0xffffffffu, f, 8 * t + 4);
-                    const float a2 = __shfl_sync(0xffffffffu, f2, 8 * t), c2 = __shfl_sync(0xffffffffu, f2, 8 * t + 4);
-#pragma unroll
-                    for (int i = 0; i < VH * 4; i++) {
-                        const float4 u = peers[(from * (Shape::ACC / 4) + i * NT + n) * 32 + lane];
-                        o[i][n][0] = o[i][n][0] * a + u.x * a2;
-                        o[i][n][1] = o[i][n][1] * c + u.y * c2;
-                        o[i][n][2] = o[i][n][2] * a + u.z * a2;
-                        o[i][n][3] = o[i][n][3] * c + u.w * c2;
-                    }
+                for (int i = 0; i < VH * 4; i++) {
+                    const float4 u = peers[(from * (Shape::ACC / 4) + i) * 32 + lane];
+                    o[i][0] = o[i][0] * a + u.x * a2;
+                    o[i][1] = o[i][1] * c + u.y * c2;
+                    o[i][2] = o[i][2] * a + u.z * a2;
+                    o[i][3] = o[i][3] * c + u.w * c2;
                 }
             }
             __syncthreads();
@@ -467,40 +475,36 @@ __global__ void __launch_bounds__(128, MmaShape<DP, NT, RW>::CTAS) paged_attenti
             const bool whole = t0 == 0 && t1 == sp.tiles;
             float *part = p.ws + (((size_t)blockIdx.y * ctas + cta) * 2 + (run.first ? 0 : 1)) * Shape::ROWS * (D + 2);
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
+            for (int e = 0; e < 2; e++) {
+                const float L = __shfl_sync(0xffffffffu, l, 8 * t + 4 * e);
+                const int i0 = member * 8 + 2 * t + e, r = r0 + 2 * t + e;
+                if (r >= R) continue;
+                if (whole) {
+                    T *to = reinterpret_cast<T *>(p.out) + (((size_t)b * p.S + r % p.S) * p.Hq + h * p.group + r / p.S) * D;
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const float L = __shfl_sync(0xffffffffu, l[n], 8 * t + 4 * e);
-                    const int i0 = member * 8 * NT + 8 * n + 2 * t + e, r = r0 + i0;
-                    if (r >= R) continue;
-                    if (whole) {
-                        T *to = reinterpret_cast<T *>(p.out) + (((size_t)b * p.S + r % p.S) * p.Hq + h * p.group + r / p.S) * D;
+                    for (int v = 0; v < VH; v++) {
+                        __align__(16) T y[8];
 #pragma unroll
-                        for (int v = 0; v < VH; v++) {
-                            __align__(16) T y[8];
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                y[2 * i] = from_f32<T>(paged_quotient(o[4 * v + i][n][e], L));
-                                y[2 * i + 1] = from_f32<T>(paged_quotient(o[4 * v + i][n][2 + e], L));
-                            }
-                            if (64 * v + 8 * g < D) *reinterpret_cast<uint4 *>(to + 64 * v + 8 * g) = *reinterpret_cast<const uint4 *>(y);
+                        for (int i = 0; i < 4; i++) {
+                            y[2 * i] = from_f32<T>(paged_quotient(o[4 * v + i][e], L));
+                            y[2 * i + 1] = from_f32<T>(paged_quotient(o[4 * v + i][2 + e], L));
                         }
-                    } else {
+                        if (64 * v + 8 * g < D) *reinterpret_cast<uint4 *>(to + 64 * v + 8 * g) = *reinterpret_cast<const uint4 *>(y);
+                    }
+                } else {
 #pragma unroll
-                        for (int v = 0; v < VH; v++) {
-                            float4 *to = reinterpret_cast<float4 *>(part + (size_t)i0 * D + 64 * v + 8 * g);
-                            if (64 * v + 8 * g < D) {
-                                to[0] = make_float4(o[4 * v][n][e], o[4 * v][n][2 + e], o[4 * v + 1][n][e], o[4 * v + 1][n][2 + e]);
-                                to[1] = make_float4(o[4 * v + 2][n][e], o[4 * v + 2][n][2 + e], o[4 * v + 3][n][e], o[4 * v + 3][n][2 + e]);
-                            }
+                    for (int v = 0; v < VH; v++) {
+                        float4 *to = reinterpret_cast<float4 *>(part + (size_t)i0 * D + 64 * v + 8 * g);
+                        if (64 * v + 8 * g < D) {
+                            to[0] = make_float4(o[4 * v][e], o[4 * v][2 + e], o[4 * v + 1][e], o[4 * v + 1][2 + e]);
+                            to[1] = make_float4(o[4 * v + 2][e], o[4 * v + 2][2 + e], o[4 * v + 3][e], o[4 * v + 3][2 + e]);
                         }
                     }
                 }
-                if (!whole && t == 0) {
-                    const int i0 = member * 8 * NT + 8 * n + g;
-                    part[Shape::ROWS * D + i0] = m[n] * kLn2;
-                    part[Shape::ROWS * D + Shape::ROWS + i0] = l[n];
-                }
+            }
+            if (!whole && t == 0) {
+                part[Shape::ROWS * D + member * 8 + g] = m * kLn2;
+                part[Shape::ROWS * D + Shape::ROWS + member * 8 + g] = l;
             }
         }
     }
@@ -595,7 +599,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attention_join_kernel(c
 // How the launch is cut: kernel, query rows of a block, CTAs.
 struct PagedPlan {
     bool mma;
-    int dim, tiles_of_rows, team;  // padded head dimension, 8-row blocks of a warp, warps of a team
+    int dim, team;  // padded head dimension, warps of a team
     int ctas, block_rows, row_blocks, round;
     bool whole;
     size_t bytes(int D) const { return whole ? 16 : (size_t)ctas * sizeof(int4) + (size_t)ctas * row_blocks * 2 * block_rows * (D + 2) * sizeof(float); }
@@ -616,30 +620,32 @@ static PagedPlan paged_plan(int B, int S, int Hq, int Hkv, int D, int page, int 
     const int R = Hq / Hkv * S;
     n.mma = mma;
     n.dim = D <= 64 ? 64 : D <= 128 ? 128 : D <= 192 ? 192 : 256;
-    n.tiles_of_rows = R <= 8 ? 1 : 2;
-    n.team = R <= 16 ? 1 : R <= 32 ? 2 : 4;
-    n.block_rows = mma ? 8 * n.tiles_of_rows * n.team : kPlainRows;
+    n.team = R <= 8 ? 1 : R <= 16 ? 2 : R <= 32 ? 4 : 8;
+    n.block_rows = mma ? 8 * n.team : kPlainRows;
     n.row_blocks = (R + n.block_rows - 1) / n.block_rows;
-    n.round = mma || D <= 128 ? 4 : kPlainWarps<8>;
+    n.round = mma ? 8 / n.team : D <= 128 ? 4 : kPlainWarps<8>;
     const long long tiles = ((long long)width * page + kPagedTile - 1) / kPagedTile, most = mma && n.dim <= 128 ? 2 * sms : sms;
     n.whole = tiles <= kPagedWhole;
     n.ctas = n.whole ? B * Hkv : (int)std::min<long long>(most, std::max<long long>(1, (tiles * Hkv * B + n.round - 1) / n.round));
     return n;
 }
 
-template <typename T, int DP, int NT, int RW>
+template <typename T, int DP, int RW>
 static int launch_mma(cudaStream_t st, const PagedAttention &p, int ctas) {
     static SmemLimit limit;
-    MYNN_CUDA_OK(limit.raise((const void *)paged_attention_mma_kernel<T, DP, NT, RW>, MmaShape<DP, NT, RW>::SMEM));
-    MYNN_CUDA_OK(launch_dependent(paged_attention_mma_kernel<T, DP, NT, RW>, dim3(ctas, p.row_blocks), dim3(128), MmaShape<DP, NT, RW>::SMEM, st, p));
+    MYNN_CUDA_OK(limit.raise((const void *)paged_attention_mma_kernel<T, DP, RW>, MmaShape<DP, RW>::SMEM));
+    MYNN_CUDA_OK(launch_dependent(paged_attention_mma_kernel<T, DP, RW>, dim3(ctas, p.row_blocks), dim3(256), MmaShape<DP, RW>::SMEM, st, p));
     MYNN_LAUNCH_OK("paged_attention_mma_kernel");
     return MYNN_OK;
 }
 template <typename T, int DP>
 static int launch_mma_rows(cudaStream_t st, const PagedAttention &p, const PagedPlan &n) {
-    if (n.team == 4) return launch_mma<T, DP, 2, 4>(st, p, n.ctas);
-    if (n.team == 2) return launch_mma<T, DP, 2, 2>(st, p, n.ctas);
-    return n.tiles_of_rows == 2 ? launch_mma<T, DP, 2, 1>(st, p, n.ctas) : launch_mma<T, DP, 1, 1>(st, p, n.ctas);
+    switch (n.team) {
+        case 1: return launch_mma<T, DP, 1>(st, p, n.ctas);
+        case 2: return launch_mma<T, DP, 2>(st, p, n.ctas);
+        case 4: return launch_mma<T, DP, 4>(st, p, n.ctas);
+        default: return launch_mma<T, DP, 8>(st, p, n.ctas);
+    }
 }
 template <typename T>
 static int launch_mma_any(cudaStream_t st, const PagedAttention &p, const PagedPlan &n) {
@@ -710,6 +716,7 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
     p.page = page, p.pages = pages, p.width = table_pages;
     p.row_blocks = n.row_blocks, p.block_rows = n.block_rows, p.round = n.round;
     p.whole = n.whole;
+    p.strips = n.mma && page % kPagedTile == 0 && D == n.dim;
     p.records = reinterpret_cast<int4 *>(workspace);
     p.ws = reinterpret_cast<float *>(p.records + (n.whole ? 0 : n.ctas));
     const cudaStream_t st = (cudaStream_t)stream;
