@@ -185,8 +185,9 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32) paged_attention_plain_ke
 // Bound by the one pass over the cache.  A team of RW warps takes tiles of 16 positions: cp.async brings a tile's rows, wherever their pages lie, to a ring in shared
 // memory whose entries are the keys or the values of a tile, each warp a share of the rows, and each warp then multiplies the whole tile with eight query rows of its
 // own, so that a row of the cache is read once for up to 64 query rows (all heads of a group, all drafts).  Both products are mma.m16n8k16 on fragments that
-// are 16-byte pieces of the rows, as in the attention over contiguous caches: S = Q K^T with the dimensions of a step permuted, O^T = V^T P^T with pairs of
-// positions put together by byte permutes; weights enter as a 16-bit part and its remainder (16 bits in all), scores, maxima and sums are f32.  D is padded to DP with
+// are whole 8 x 8 blocks from ldmatrix, without a byte moved: S^T = K Q^T, eight query rows as columns, and O^T = V^T P^T, whose second operand is the first
+// product's result behind a transposition of its 8 x 8 blocks.  Weights enter as a 16-bit part and its remainder (16 bits in all); scores, maxima and sums are f32.  The
+// reference of the weights is moved only when a score exceeds it by 2^8, so most tiles need no maximum across lanes and no rescaling.  D is padded to DP with
 // zeros, on the chip only.
 // The chain of one tile is long (two products, a softmax) and each warp walks it alone, so warps are what hides it: sixteen per SM, eight query rows each, rather than
 // eight with sixteen rows (96 mixed sequences of heads of 64: eight warps per SM 97 us).
@@ -208,22 +209,26 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-// Where a 16-byte piece c of a row lies among the eight of its 128 bytes: two neighbouring rows' pieces t .. t + 3 (keys) and four even or odd rows' pieces 2 i,
-// 2 i + 1 (values) are in different banks.
-__device__ __forceinline__ int paged_swizzle(int row, int c) { return c ^ (row & 6) ^ ((row & 1) << 2); }
+// Where a 16-byte piece c of a row lies among the eight of its 128 bytes: the same piece of eight rows is in different banks.
+__device__ __forceinline__ int paged_swizzle(int row, int c) { return c ^ (row & 7); }
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 
 __device__ __forceinline__ void copy16_now(uint32_t smem, const void *gmem) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory"); }
 
 template <typename T>
-__device__ __forceinline__ bool has_special(uint32_t x) {  // infinity or NaN in one of two 16-bit numbers
+__device__ __forceinline__ uint32_t special_mask(uint32_t x) {  // all ones over each of two 16-bit numbers that is infinite or NaN
     constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-    return (x & e) == e || (x >> 16 & e) == e;
+    return ((x & e) == e ? 0xffffu : 0u) | ((x >> 16 & e) == e ? 0xffff0000u : 0u);
 }
 
 template <typename T, int DP, int RW>
 __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_mma_kernel(const PagedAttention p) {
     using Shape = MmaShape<DP, RW>;
-    constexpr int W = Shape::W, TEAMS = Shape::TEAMS, STAGES = Shape::STAGES, AHEAD = Shape::AHEAD, TILE = kPagedTile, KCH = DP / 32, VH = DP / 64, CPR = DP / 8;
+    constexpr int W = Shape::W, TEAMS = Shape::TEAMS, STAGES = Shape::STAGES, AHEAD = Shape::AHEAD, TILE = kPagedTile, KCH = DP / 32, CPR = DP / 8;
     constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
     extern __shared__ __align__(128) uint8_t raw[];
     __shared__ float peer_m[W / 2][8], peer_l[W / 2][8];
@@ -234,6 +239,7 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
     uint8_t *ring = raw + (size_t)team * STAGES * Shape::ENTRY;
     float4 *peers = reinterpret_cast<float4 *>(raw);  // over the rings, when they are idle
     const uint32_t ring_at = smem_u32(ring);
+    const bool busy = r0 < R;  // a warp without rows of its own only helps to copy
     for (int b = cta; b < p.B; b += ctas)  // sequences that see nothing at all are in no CTA's run
         if (blockIdx.y == 0 && paged_span(p, b).tiles == 0)
             for (size_t n = (size_t)p.S * p.Hq * D / 8, i = threadIdx.x; i < n; i += W * 32) reinterpret_cast<uint4 *>(p.out)[b * n + i] = make_uint4(0, 0, 0, 0);
@@ -254,7 +260,7 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             const int r = r0 + i;
             return r < R && r % p.S < sp.count ? oldest + r % p.S : -1;
         };
-        const int at = last_seen(g);
+        const int at[2] = {last_seen(2 * t), last_seen(2 * t + 1)};  // this lane's two rows
         auto sees = [&](int last, int j) { return j <= last && (p.window <= 0 || last - j < p.window || j < p.sinks); };
         auto base_of = [&](int j) { return sp.base(t0 + team + TEAMS * j); };
         // The first row of a tile whose sixteen rows lie one behind the other and are all seen, for 32 tiles at once, one per lane; -1 for others.
@@ -305,19 +311,22 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
         if (strip < 0) row = row_of(AHEAD);
         uint32_t cur = 0, free_entry = (STAGES - 1) * Shape::ENTRY;  // offsets: the entry that is read next, the one that is empty
 
-        uint2 qa[2 * KCH];
+        uint32_t qb[2 * KCH][2];  // row g, dimensions 16 i + 2 t and + 8
         {
             const int r = min(r0 + g, R - 1);
+            const bool in = r0 + g < R && r % p.S < sp.count;
             const T *qr = reinterpret_cast<const T *>(p.q) + (((size_t)b * p.Hq + h * p.group + r / p.S) * p.S + r % p.S) * D;
 #pragma unroll
-            for (int i = 0; i < 2 * KCH; i++) {
-                const int d = 8 * (t + 4 * (i >> 1)) + 4 * (i & 1);
-                qa[i] = at >= 0 && d < D ? *reinterpret_cast<const uint2 *>(qr + d) : make_uint2(0u, 0u);
-            }
-        }
-        float o[VH * 4][4], m = -INFINITY, l = 0.f;
+            for (int i = 0; i < 2 * KCH; i++)
 #pragma unroll
-        for (int i = 0; i < VH * 4; i++)
+                for (int e = 0; e < 2; e++) {
+                    const int d = 16 * i + 8 * e + 2 * t;
+                    qb[i][e] = in && d < D ? *reinterpret_cast<const uint32_t *>(qr + d) : 0u;
+                }
+        }
+        float o[DP / 16][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < DP / 16; i++)
 #pragma unroll
             for (int e = 0; e < 4; e++) o[i][e] = 0.f;
 #pragma unroll 1
@@ -328,53 +337,56 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             exist[AHEAD] = strip >= 0 ? 0xffffu : __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
             issue(p.k, ring_at + free_entry, ahead < mine, strip, row);
             const int base = base_of(j);
-            const uint8_t *K = ring + cur;
+            const uint32_t K = ring_at + cur;
             free_entry = cur;
             cur = cur + Shape::ENTRY == STAGES * Shape::ENTRY ? 0 : cur + Shape::ENTRY;
-            // ---- S = Q K^T: x[2 c + e] is row g, position base + 8 c + 2 t + e ----
-            float x[4];
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int i = 0; i < KCH; i++) {
-                    const uint4 kr = *reinterpret_cast<const uint4 *>(K + (8 * c + g) * (DP * 2) + (i >> 1) * 128 + paged_swizzle(g, t + 4 * (i & 1)) * 16);
-                    mma_kv<T>(acc, qa[2 * i].x, 0u, qa[2 * i].y, 0u, kr.x, kr.y);
-                    mma_kv<T>(acc, qa[2 * i + 1].x, 0u, qa[2 * i + 1].y, 0u, kr.z, kr.w);
-                }
-                x[2 * c] = acc[0], x[2 * c + 1] = acc[1];
-            }
+            // ---- S^T = K Q^T: x[2 k + e] is position base + g + 8 k, row 2 t + e ----
+            float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+            uint32_t hi[2], lo[2];
             const bool full = exist[0] == 0xffffu && (p.S == 1 || paged_tile_full(p, sp, base));
-            float top = -INFINITY;
+            if (busy) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (p.softcap > 0.f) x[i] = kLog2e * fast_soft_cap(x[i] * p.scale, p.softcap);
-                else x[i] *= unit;
-            }
-            if (!full) {
+                for (int i = 0; i < 2 * KCH; i++) {
+                    uint32_t a[4];
+                    const int krow = lane & 15;
+                    ldsm4_at(a, K + krow * (DP * 2) + (i >> 2) * 128 + paged_swizzle(krow, 2 * (i & 3) + (lane >> 4)) * 16);
+                    mma_kv<T>(i & 1 ? y : x, a[0], a[1], a[2], a[3], qb[i][0], qb[i][1]);
+                }
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int bit = 8 * (i >> 1) + 2 * t + (i & 1);
-                    if (!((exist[0] >> bit & 1) && sees(at, base + bit))) x[i] = -INFINITY;
+                    x[i] += y[i];
+                    if (p.softcap > 0.f) x[i] = kLog2e * fast_soft_cap(x[i] * p.scale, p.softcap);
+                    else x[i] *= unit;
                 }
-            }
+                if (!full) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) top = fmaxf(top, x[i]);
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float now = fmaxf(m, top), ref = merge_reference(now), keep = exp2_approx(m - ref);
-            const bool moved = now > m;
-            m = now;
+                    for (int i = 0; i < 4; i++) {
+                        const int bit = g + 8 * (i >> 1);
+                        if (!((exist[0] >> bit & 1) && sees(at[i & 1], base + bit))) x[i] = -INFINITY;
+                    }
+                }
+                if (__any_sync(0xffffffffu, fmaxf(x[0], x[2]) > m[0] + 8.f || fmaxf(x[1], x[3]) > m[1] + 8.f)) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = exp2_approx(x[i] - ref);
-            l = l * keep + ((x[0] + x[1]) + (x[2] + x[3]));  // of this lane's positions
-            uint32_t hi[2], lo[2];
-            split_pack<T>(x[0], x[1], hi[0], lo[0]);
-            split_pack<T>(x[2], x[3], hi[1], lo[1]);
-            if (__any_sync(0xffffffffu, moved)) {
-                const float k0 = __shfl_sync(0xffffffffu, keep, 8 * t), k1 = __shfl_sync(0xffffffffu, keep, 8 * t + 4);
+                    for (int e = 0; e < 2; e++) {
+                        float top = fmaxf(x[e], x[2 + e]);
 #pragma unroll
-                for (int i = 0; i < VH * 4; i++) o[i][0] *= k0, o[i][1] *= k1, o[i][2] *= k0, o[i][3] *= k1;
+                        for (int s = 4; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+                        const float now = fmaxf(m[e], top), keep = exp2_approx(m[e] - merge_reference(now));
+                        m[e] = now;
+                        l[e] *= keep;
+#pragma unroll
+                        for (int i = 0; i < DP / 16; i++) o[i][e] *= keep, o[i][2 + e] *= keep;
+                    }
+                }
+                const float r0_ = merge_reference(m[0]), r1_ = merge_reference(m[1]);
+                x[0] = exp2_approx(x[0] - r0_), x[1] = exp2_approx(x[1] - r1_), x[2] = exp2_approx(x[2] - r0_), x[3] = exp2_approx(x[3] - r1_);
+                l[0] += x[0] + x[2];  // of this lane's positions
+                l[1] += x[1] + x[3];
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    split_pack<T>(x[2 * k], x[2 * k + 1], hi[k], lo[k]);
+                    hi[k] = transpose_8x8(hi[k]), lo[k] = transpose_8x8(lo[k]);  // positions 8 k + 2 t, + 1 of row g
+                }
             }
             asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
             team_sync();  // the values of tile j are here, and its keys are done with
@@ -382,66 +394,51 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             if (((ahead + 1) & 31) == 0) strips = strips_next, strips_next = strips_of(ahead + 33 + lane);
             strip = __shfl_sync(0xffffffffu, strips, (ahead + 1) & 31);
             if (strip < 0) row = row_of(ahead + 1);
-            const uint8_t *V = ring + cur;
+            const uint32_t V = ring_at + cur;
             free_entry = cur;
             cur = cur + Shape::ENTRY == STAGES * Shape::ENTRY ? 0 : cur + Shape::ENTRY;
-            // ---- O^T += V^T P^T: o[4 v + i] is dimensions 64 v + 8 g + 2 i (registers 0, 1) and + 1 (2, 3) of rows 2 t and 2 t + 1 ----
-            bool special = false;
+            // ---- O^T += V^T P^T: o[i] is dimensions 16 i + g (registers 0, 1) and + 8 (2, 3) of rows 2 t and 2 t + 1 ----
+            if (busy) {
 #pragma unroll
-            for (int v = 0; v < VH; v++) {
-                uint32_t vr[4][4];
+                for (int i = 0; i < DP / 16; i++) {
+                    uint32_t a[4];
+                    const int vrow = (lane & 7) + (lane >> 4) * 8;
+                    ldsm4t_at(a, V + vrow * (DP * 2) + (i >> 2) * 128 + paged_swizzle(vrow, 2 * (i & 3) + (lane >> 3 & 1)) * 16);
+                    if (!full && p.S > 1) {
+                        // Values that are no numbers, in a tile that not every row sees all of: they are taken out of the product and added position by
+                        // position where they are seen, so that the other rows keep their bits.
+                        uint32_t sp_[4];
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int vrow = 2 * t + (r & 1) + 8 * (r >> 1);
-                    const uint4 u = *reinterpret_cast<const uint4 *>(V + vrow * (DP * 2) + v * 128 + paged_swizzle(vrow, g) * 16);
-                    vr[r][0] = u.x, vr[r][1] = u.y, vr[r][2] = u.z, vr[r][3] = u.w;
-                }
-                if (!full && p.S > 1) {
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) special |= has_special<T>(vr[r][i]);
-                    special = __any_sync(0xffffffffu, special);
-                }
-                if (special) {
-                    // A value that is no number, which not every row sees: position by position, added only where it is seen.  (What stands in
-                    // `special` from the slab in front does no harm.)
-                    const int at0 = last_seen(2 * t), at1 = last_seen(2 * t + 1);
+                        for (int c = 0; c < 4; c++) sp_[c] = special_mask<T>(a[c]);
+                        if (__any_sync(0xffffffffu, (sp_[0] | sp_[1] | sp_[2] | sp_[3]) != 0u)) {
 #pragma unroll 1
-                    for (int k = 0; k < TILE; k++) {
-                        const bool s0 = (exist[0] >> k & 1) && sees(at0, base + k), s1 = (exist[0] >> k & 1) && sees(at1, base + k);
+                            for (int k = 0; k < TILE; k++) {
+                                const uint32_t one = (k & 7) >> 1 == t ? (k & 1 ? 0xffff0000u : 0xffffu) : 0u, first = k < 8 ? one : 0u, second = k < 8 ? 0u : one;
+                                const uint32_t b0 = a[0] & sp_[0] & first, b1 = a[1] & sp_[1] & first, b2 = a[2] & sp_[2] & second, b3 = a[3] & sp_[3] & second;
+                                float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                                mma_kv<T>(acc, b0, b1, b2, b3, hi[0], hi[1]);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            uint32_t one[4];
+                                for (int e = 0; e < 2; e++)
+                                    if ((exist[0] >> k & 1) && sees(at[e], base + k)) o[i][e] += acc[e], o[i][2 + e] += acc[2 + e];
+                            }
 #pragma unroll
-                            for (int r = 0; r < 4; r++) one[r] = 2 * t + (r & 1) + 8 * (r >> 1) == k ? vr[r][i] : 0u;
-                            const uint32_t a0 = __byte_perm(one[0], one[1], 0x5410u), a1 = __byte_perm(one[0], one[1], 0x7632u);
-                            const uint32_t a2 = __byte_perm(one[2], one[3], 0x5410u), a3 = __byte_perm(one[2], one[3], 0x7632u);
-                            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma_kv<T>(acc, a0, a1, a2, a3, hi[0], hi[1]);
-                            mma_kv<T>(acc, a0, a1, a2, a3, lo[0], lo[1]);
-                            float(&to)[4] = o[4 * v + i];
-                            if (s0) to[0] += acc[0], to[2] += acc[2];
-                            if (s1) to[1] += acc[1], to[3] += acc[3];
+                            for (int c = 0; c < 4; c++) a[c] &= ~sp_[c];
                         }
                     }
-                    continue;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint32_t a0 = __byte_perm(vr[0][i], vr[1][i], 0x5410u), a1 = __byte_perm(vr[0][i], vr[1][i], 0x7632u);
-                    const uint32_t a2 = __byte_perm(vr[2][i], vr[3][i], 0x5410u), a3 = __byte_perm(vr[2][i], vr[3][i], 0x7632u);
-                    mma_kv<T>(o[4 * v + i], a0, a1, a2, a3, hi[0], hi[1]);
-                    mma_kv<T>(o[4 * v + i], a0, a1, a2, a3, lo[0], lo[1]);
+                    mma_kv<T>(o[i], a[0], a[1], a[2], a[3], hi[0], hi[1]);
+                    mma_kv<T>(o[i], a[0], a[1], a[2], a[3], lo[0], lo[1]);
                 }
             }
 #pragma unroll
             for (int i = 0; i < AHEAD; i++) exist[i] = exist[i + 1];
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (at < 0) m = -INFINITY, l = 0.f;  // a row that is no query, which tiles that all see are not masked for
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+#pragma unroll
+            for (int s = 4; s < 32; s <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], s);
+            if (at[e] < 0) m[e] = -INFINITY, l[e] = 0.f;  // a row that is no query, which tiles that all see are not masked for
+        }
         // ---- the teams meet: half of them hand their sums to the other half, register by register ----
         if constexpr (TEAMS > 1) __syncthreads();  // the rings are idle
 #pragma unroll
@@ -449,24 +446,30 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             const int slot = (team - half) * RW + member;
             if (team >= half && team < 2 * half) {
 #pragma unroll
-                for (int i = 0; i < VH * 4; i++) peers[(slot * (Shape::ACC / 4) + i) * 32 + lane] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
-                if (t == 0) peer_m[slot][g] = m, peer_l[slot][g] = l;
+                for (int i = 0; i < DP / 16; i++) peers[(slot * (Shape::ACC / 4) + i) * 32 + lane] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+                if (g == 0) {
+#pragma unroll
+                    for (int e = 0; e < 2; e++) peer_m[slot][2 * t + e] = m[e], peer_l[slot][2 * t + e] = l[e];
+                }
             }
             __syncthreads();
             if (team < half) {
                 const int from = team * RW + member;
-                const float m2 = peer_m[from][g], now = fmaxf(m, m2), ref = merge_reference(now), f = exp2_approx(m - ref), f2 = exp2_approx(m2 - ref);
-                m = now;
-                l = l * f + peer_l[from][g] * f2;
-                const float a = __shfl_sync(0xffffffffu, f, 8 * t), c = __shfl_sync(0xffffffffu, f, 8 * t + 4);
-                const float a2 = __shfl_sync(0xffffffffu, f2, 8 * t), c2 = __shfl_sync(0xffffffffu, f2, 8 * t + 4);
+                float f[2], f2[2];
 #pragma unroll
-                for (int i = 0; i < VH * 4; i++) {
+                for (int e = 0; e < 2; e++) {
+                    const float m2 = peer_m[from][2 * t + e], now = fmaxf(m[e], m2), ref = merge_reference(now);
+                    f[e] = exp2_approx(m[e] - ref), f2[e] = exp2_approx(m2 - ref);
+                    m[e] = now;
+                    l[e] = l[e] * f[e] + peer_l[from][2 * t + e] * f2[e];
+                }
+#pragma unroll
+                for (int i = 0; i < DP / 16; i++) {
                     const float4 u = peers[(from * (Shape::ACC / 4) + i) * 32 + lane];
-                    o[i][0] = o[i][0] * a + u.x * a2;
-                    o[i][1] = o[i][1] * c + u.y * c2;
-                    o[i][2] = o[i][2] * a + u.z * a2;
-                    o[i][3] = o[i][3] * c + u.w * c2;
+                    o[i][0] = o[i][0] * f[0] + u.x * f2[0];
+                    o[i][1] = o[i][1] * f[1] + u.y * f2[1];
+                    o[i][2] = o[i][2] * f[0] + u.z * f2[0];
+                    o[i][3] = o[i][3] * f[1] + u.w * f2[1];
                 }
             }
             __syncthreads();
@@ -476,35 +479,22 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             float *part = p.ws + (((size_t)blockIdx.y * ctas + cta) * 2 + (run.first ? 0 : 1)) * Shape::ROWS * (D + 2);
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const float L = __shfl_sync(0xffffffffu, l, 8 * t + 4 * e);
                 const int i0 = member * 8 + 2 * t + e, r = r0 + 2 * t + e;
                 if (r >= R) continue;
                 if (whole) {
                     T *to = reinterpret_cast<T *>(p.out) + (((size_t)b * p.S + r % p.S) * p.Hq + h * p.group + r / p.S) * D;
 #pragma unroll
-                    for (int v = 0; v < VH; v++) {
-                        __align__(16) T y[8];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            y[2 * i] = from_f32<T>(paged_quotient(o[4 * v + i][e], L));
-                            y[2 * i + 1] = from_f32<T>(paged_quotient(o[4 * v + i][2 + e], L));
-                        }
-                        if (64 * v + 8 * g < D) *reinterpret_cast<uint4 *>(to + 64 * v + 8 * g) = *reinterpret_cast<const uint4 *>(y);
-                    }
+                    for (int i = 0; i < DP / 8; i++)
+                        if (8 * i < D) to[8 * i + g] = from_f32<T>(paged_quotient(o[i >> 1][2 * (i & 1) + e], l[e]));
                 } else {
 #pragma unroll
-                    for (int v = 0; v < VH; v++) {
-                        float4 *to = reinterpret_cast<float4 *>(part + (size_t)i0 * D + 64 * v + 8 * g);
-                        if (64 * v + 8 * g < D) {
-                            to[0] = make_float4(o[4 * v][e], o[4 * v][2 + e], o[4 * v + 1][e], o[4 * v + 1][2 + e]);
-                            to[1] = make_float4(o[4 * v + 2][e], o[4 * v + 2][2 + e], o[4 * v + 3][e], o[4 * v + 3][2 + e]);
-                        }
+                    for (int i = 0; i < DP / 8; i++)
+                        if (8 * i < D) part[(size_t)i0 * D + 8 * i + g] = o[i >> 1][2 * (i & 1) + e];
+                    if (g == 0) {
+                        part[Shape::ROWS * D + i0] = m[e] * kLn2;
+                        part[Shape::ROWS * D + Shape::ROWS + i0] = l[e];
                     }
                 }
-            }
-            if (!whole && t == 0) {
-                part[Shape::ROWS * D + member * 8 + g] = m * kLn2;
-                part[Shape::ROWS * D + Shape::ROWS + member * 8 + g] = l;
             }
         }
     }
