@@ -29,7 +29,7 @@ struct PagedAttention {
     int B, S, Hq, G, group, D;
     int page, pages, width;  // rows of a page, pages of the cache, pages in a row of the table
     int row_blocks, block_rows;  // the group * S query rows of a pair, row r = head * S + s, in blocks
-    int round;                   // shares are multiples of it: the tiles that the warps of a CTA take at a time
+    int round, toll;             // shares are multiples of `round`, the tiles that the warps of a CTA take at a time; toll: see PagedRun
     int4 *records;               // per CTA the pair that begins in it and ends in another: {b, h, last CTA, slot}, or b == -1
     float *ws;                   // [row block][CTA][2] parts of block_rows * (D + 2) floats: rows, then maxima, then sums
     int whole;                   // each pair is left to a CTA of its own
@@ -85,50 +85,61 @@ __device__ __forceinline__ long long paged_share(long long total, int ctas, int 
     return max((s + round - 1) / round, 1ll) * round;
 }
 
-// What a CTA takes one after the other: tiles t0 .. t1 - 1 of pair (b, h).
+// What a CTA takes one after the other: tiles t0 .. t1 - 1 of pair (b, h).  To begin with a pair takes time as well, so a pair counts as `toll` tiles more: they lie in front
+// of its tiles, v0 .. v1 - 1 counts both.
 struct PagedRun {
-    int b, h, t0, t1;
+    int b, h, t0, t1, v0, v1;
     long long share, left;
     int4 record;
     bool first;
-    __device__ __forceinline__ void begin(const PagedAttention &p, const PagedShare &s) {
-        b = s.b, h = s.h, t0 = s.t;
+    __device__ __forceinline__ void begin(const PagedShare &s) {
+        b = s.b, h = s.h, v0 = s.t;
         share = left = s.share;
         record = make_int4(-1, 0, 0, 0);
         first = true;
     }
     // On to the next pair that has tiles; false: there is none.
     __device__ __forceinline__ bool more(const PagedAttention &p, PagedSpan &sp) {
-        for (; b < p.B && left > 0; b++, h = t0 = 0) {
+        for (; b < p.B && left > 0; b++, h = v0 = 0) {
             sp = paged_span(p, b);
             if (sp.tiles == 0) continue;
-            t1 = (int)min((long long)sp.tiles, t0 + left);
-            if (t0 == 0 && t1 < sp.tiles) record = make_int4(b, h, blockIdx.x + (int)((sp.tiles - t1 + share - 1) / share), first ? 0 : 1);
+            const int cost = sp.tiles + p.toll;
+            v1 = (int)min((long long)cost, v0 + left);
+            t0 = max(v0 - p.toll, 0);
+            t1 = max(v1 - p.toll, 0);
+            if (t1 <= t0) break;  // the run ends in the toll: the pair is the next CTA's
+            if (t0 == 0 && v1 < cost) record = make_int4(b, h, blockIdx.x + (int)((cost - v1 + share - 1) / share), first ? 0 : 1);
             return true;
         }
+        left = 0;
         return false;
     }
     __device__ __forceinline__ void advance(const PagedAttention &p) {
-        left -= t1 - t0;
-        t0 = 0;
+        left -= v1 - v0;
+        v0 = 0;
         first = false;
         if (++h == p.G) h = 0, b++;
     }
 };
 
-// Called by all threads of a CTA: the total number of tiles and the place of tile cta * share.  Each thread sums a run of sequences.
+__device__ __forceinline__ long long paged_cost(const PagedAttention &p, int b) {
+    const int n = paged_span(p, b).tiles;
+    return n > 0 ? n + p.toll : 0;
+}
+
+// Called by all threads of a CTA: the total cost and the place cta * share in it.  Each thread sums a run of sequences.
 template <int THREADS>
 __device__ __forceinline__ PagedShare paged_find(const PagedAttention &p, int cta, int ctas) {
     __shared__ long long warp_sums[THREADS / 32];
     __shared__ PagedShare found;
     if (p.whole) {
-        const int b = cta / p.G, n = paged_span(p, b).tiles;
-        return {0, n, b, cta - b * p.G, 0};
+        const int b = cta / p.G;
+        return {0, paged_cost(p, b), b, cta - b * p.G, 0};
     }
     const int per = (p.B + THREADS - 1) / THREADS, b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     long long mine = 0;
-    for (int b = b0; b < b1; b++) mine += (long long)paged_span(p, b).tiles * p.G;
+    for (int b = b0; b < b1; b++) mine += paged_cost(p, b) * p.G;
     long long incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -148,13 +159,13 @@ __device__ __forceinline__ PagedShare paged_find(const PagedAttention &p, int ct
     if (threadIdx.x == 0 && begin >= total) found = {total, share, p.B, 0, 0};
     if (begin >= at && begin < end) {
         for (int b = b0; b < b1; b++) {
-            const int n = paged_span(p, b).tiles;
-            if (begin < at + (long long)n * p.G) {
+            const long long n = paged_cost(p, b);
+            if (begin < at + n * p.G) {
                 const long long rest = begin - at;
                 found = {total, share, b, (int)(rest / n), (int)(rest % n)};
                 break;
             }
-            at += (long long)n * p.G;
+            at += n * p.G;
         }
     }
     __syncthreads();

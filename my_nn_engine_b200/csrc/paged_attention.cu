@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32) paged_attention_plain_ke
             for (int i = threadIdx.x; i < p.G * rows * D; i += W * 32)
                 reinterpret_cast<T *>(p.out)[place(b, i / (rows * D), r0 + i / D % rows, i % D)] = from_f32<T>(0.f);
     PagedRun run;
-    run.begin(p, paged_find<W * 32>(p, cta, ctas));
+    run.begin(paged_find<W * 32>(p, cta, ctas));
     PagedSpan sp;
     for (; run.more(p, sp); run.advance(p)) {
         const int b = run.b, h = run.h, t0 = run.t0, t1 = run.t1;
@@ -198,9 +198,8 @@ struct MmaShape {
     static constexpr int CTAS = DP > 128 ? 1 : 2;  // per SM
     static constexpr int FIT = (CTAS == 2 ? 96 : 192) * 1024 / TEAMS / ENTRY;
     static constexpr int AHEAD = FIT >= 9 ? 4 : (FIT - 1) / 2, STAGES = 2 * AHEAD + 1;  // tiles on their way while one is worked on
-    static constexpr int ACC = DP / 4;  // accumulators of a lane
-    static constexpr size_t RING = (size_t)TEAMS * STAGES * ENTRY, PEERS = TEAMS == 1 ? 0 : (size_t)W / 2 * ACC * 32 * 4;
-    static constexpr size_t SMEM = RING > PEERS ? RING : PEERS;
+    static constexpr size_t RING = (size_t)TEAMS * STAGES * ENTRY;
+    static constexpr size_t SMEM = RING + W * 8 * 64 * sizeof(float);  // and 64 dimensions of all warps' sums
 };
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -231,13 +230,13 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
     constexpr int W = Shape::W, TEAMS = Shape::TEAMS, STAGES = Shape::STAGES, AHEAD = Shape::AHEAD, TILE = kPagedTile, KCH = DP / 32, CPR = DP / 8;
     constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
     extern __shared__ __align__(128) uint8_t raw[];
-    __shared__ float peer_m[W / 2][8], peer_l[W / 2][8];
+    __shared__ float part_m[W][8], part_l[W][8];
     pdl_trigger();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, team = warp / RW, member = warp % RW;
     const int cta = blockIdx.x, ctas = gridDim.x, D = p.D, R = p.group * p.S, r0 = blockIdx.y * Shape::ROWS + member * 8;
     uint8_t *ring = raw + (size_t)team * STAGES * Shape::ENTRY;
-    float4 *peers = reinterpret_cast<float4 *>(raw);  // over the rings, when they are idle
+    float *sums = reinterpret_cast<float *>(raw + Shape::RING);
     const uint32_t ring_at = smem_u32(ring);
     const bool busy = r0 < R;  // a warp without rows of its own only helps to copy
     for (int b = cta; b < p.B; b += ctas)  // sequences that see nothing at all are in no CTA's run
@@ -249,11 +248,17 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
     };
     const float unit = p.scale * kLog2e;
     PagedRun run;
-    run.begin(p, paged_find<W * 32>(p, cta, ctas));
+    run.begin(paged_find<W * 32>(p, cta, ctas));
     PagedSpan sp;
-    for (; run.more(p, sp); run.advance(p)) {
+    // the pair that was worked on last, whose sums are still the warps' own
+    int done_b = -1, done_h = 0;
+    bool whole = false;
+    float *part = nullptr;
+    float o[DP / 16][4], m[2], l[2];
+    for (;;) {
+        const bool more = run.more(p, sp);
         const int b = run.b, h = run.h, t0 = run.t0, t1 = run.t1;
-        const int mine = t0 + team < t1 ? (t1 - t0 - team + TEAMS - 1) / TEAMS : 0;
+        const int mine = more && t0 + team < t1 ? (t1 - t0 - team + TEAMS - 1) / TEAMS : 0;
         const int oldest = sp.len - sp.count;
         // last position that row r0 + i sees, -1: it is no query
         auto last_seen = [&](int i) {
@@ -297,22 +302,21 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
         uint32_t exist[AHEAD + 1];  // which rows of the next tiles there are
-        team_sync();                // the ring is free
-        int strips = strips_of(lane), strips_next = strips_of(lane + 32), strip, row = -1;
-#pragma unroll
-        for (int j = 0; j < AHEAD; j++) {
-            strip = __shfl_sync(0xffffffffu, strips, j);
-            if (strip < 0) row = row_of(j);
-            exist[j] = strip >= 0 ? 0xffffu : __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
-            issue(p.k, ring_at + 2 * j * Shape::ENTRY, j < mine, strip, row);
-            issue(p.v, ring_at + (2 * j + 1) * Shape::ENTRY, j < mine, strip, row);
-        }
-        strip = __shfl_sync(0xffffffffu, strips, AHEAD);
-        if (strip < 0) row = row_of(AHEAD);
-        uint32_t cur = 0, free_entry = (STAGES - 1) * Shape::ENTRY;  // offsets: the entry that is read next, the one that is empty
-
+        int strips = -1, strips_next = -1, strip = -1, row = -1;
         uint32_t qb[2 * KCH][2];  // row g, dimensions 16 i + 2 t and + 8
-        {
+        if (more) {
+            team_sync();  // the ring is free
+            strips = strips_of(lane), strips_next = strips_of(lane + 32);
+#pragma unroll
+            for (int j = 0; j < AHEAD; j++) {
+                strip = __shfl_sync(0xffffffffu, strips, j);
+                if (strip < 0) row = row_of(j);
+                exist[j] = strip >= 0 ? 0xffffu : __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+                issue(p.k, ring_at + 2 * j * Shape::ENTRY, j < mine, strip, row);
+                issue(p.v, ring_at + (2 * j + 1) * Shape::ENTRY, j < mine, strip, row);
+            }
+            strip = __shfl_sync(0xffffffffu, strips, AHEAD);
+            if (strip < 0) row = row_of(AHEAD);
             const int r = min(r0 + g, R - 1);
             const bool in = r0 + g < R && r % p.S < sp.count;
             const T *qr = reinterpret_cast<const T *>(p.q) + (((size_t)b * p.Hq + h * p.group + r / p.S) * p.S + r % p.S) * D;
@@ -324,7 +328,64 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
                     qb[i][e] = in && d < D ? *reinterpret_cast<const uint32_t *>(qr + d) : 0u;
                 }
         }
-        float o[DP / 16][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        // ---- the teams meet, while the first tiles of the next pair are on their way: 64 dimensions of all warps' sums at a time ----
+        if (done_b >= 0) {
+            const int rows = min(R - (int)blockIdx.y * Shape::ROWS, Shape::ROWS);
+            __syncthreads();  // nobody reads what the pair in front left any more
+            if (g == 0) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) part_m[warp][2 * t + e] = m[e], part_l[warp][2 * t + e] = l[e];
+            }
+            __syncthreads();
+            float f[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < TEAMS; w++) top = fmaxf(top, part_m[w * RW + member][2 * t + e]);
+                f[e] = exp2_approx(m[e] - merge_reference(top));
+            }
+#pragma unroll
+            for (int s = 0; s < DP / 64; s++) {
+                if (s > 0) __syncthreads();
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++)  // (dimensions 8 apart for neighbouring t: all banks)
+                        sums[(warp * 8 + 2 * t + (k & 1)) * 64 + ((16 * i + 8 * (k >> 1) + g) ^ (t * 8))] = o[4 * s + i][k] * f[k & 1];
+                __syncthreads();
+                for (int i = threadIdx.x; i < rows * 32; i += W * 32) {
+                    const int r = i >> 5, d = 2 * (i & 31), w0 = r >> 3, at = ((w0 * 8 + (r & 7)) * 64) + (d ^ ((r >> 1 & 3) * 8));
+                    float2 O = make_float2(0.f, 0.f);
+                    float top = -INFINITY, L = 0.f;
+#pragma unroll
+                    for (int w = 0; w < TEAMS; w++) {
+                        const float2 u = *reinterpret_cast<const float2 *>(sums + at + w * RW * 512);
+                        O.x += u.x, O.y += u.y;
+                        top = fmaxf(top, part_m[w * RW + w0][r & 7]);
+                    }
+#pragma unroll
+                    for (int w = 0; w < TEAMS; w++) L += part_l[w * RW + w0][r & 7] * exp2_approx(part_m[w * RW + w0][r & 7] - merge_reference(top));
+                    if (64 * s + d >= D) continue;
+                    if (whole) {
+                        const int q = blockIdx.y * Shape::ROWS + r;
+                        T *to = reinterpret_cast<T *>(p.out) + (((size_t)done_b * p.S + q % p.S) * p.Hq + done_h * p.group + q / p.S) * D + 64 * s + d;
+                        __align__(4) T y[2] = {from_f32<T>(paged_quotient(O.x, L)), from_f32<T>(paged_quotient(O.y, L))};
+                        *reinterpret_cast<uint32_t *>(to) = *reinterpret_cast<const uint32_t *>(y);
+                    } else {
+                        *reinterpret_cast<float2 *>(part + (size_t)r * D + 64 * s + d) = O;
+                        if (s == 0 && d == 0) {
+                            part[Shape::ROWS * D + r] = top * kLn2;
+                            part[Shape::ROWS * D + Shape::ROWS + r] = L;
+                        }
+                    }
+                }
+            }
+        }
+        if (!more) break;
+        uint32_t cur = 0, free_entry = (STAGES - 1) * Shape::ENTRY;  // offsets: the entry that is read next, the one that is empty
+#pragma unroll
+        for (int e = 0; e < 2; e++) m[e] = -INFINITY, l[e] = 0.f;
 #pragma unroll
         for (int i = 0; i < DP / 16; i++)
 #pragma unroll
@@ -439,64 +500,10 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             for (int s = 4; s < 32; s <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], s);
             if (at[e] < 0) m[e] = -INFINITY, l[e] = 0.f;  // a row that is no query, which tiles that all see are not masked for
         }
-        // ---- the teams meet: half of them hand their sums to the other half, register by register ----
-        if constexpr (TEAMS > 1) __syncthreads();  // the rings are idle
-#pragma unroll
-        for (int half = TEAMS / 2; half > 0; half >>= 1) {
-            const int slot = (team - half) * RW + member;
-            if (team >= half && team < 2 * half) {
-#pragma unroll
-                for (int i = 0; i < DP / 16; i++) peers[(slot * (Shape::ACC / 4) + i) * 32 + lane] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
-                if (g == 0) {
-#pragma unroll
-                    for (int e = 0; e < 2; e++) peer_m[slot][2 * t + e] = m[e], peer_l[slot][2 * t + e] = l[e];
-                }
-            }
-            __syncthreads();
-            if (team < half) {
-                const int from = team * RW + member;
-                float f[2], f2[2];
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const float m2 = peer_m[from][2 * t + e], now = fmaxf(m[e], m2), ref = merge_reference(now);
-                    f[e] = exp2_approx(m[e] - ref), f2[e] = exp2_approx(m2 - ref);
-                    m[e] = now;
-                    l[e] = l[e] * f[e] + peer_l[from][2 * t + e] * f2[e];
-                }
-#pragma unroll
-                for (int i = 0; i < DP / 16; i++) {
-                    const float4 u = peers[(from * (Shape::ACC / 4) + i) * 32 + lane];
-                    o[i][0] = o[i][0] * f[0] + u.x * f2[0];
-                    o[i][1] = o[i][1] * f[1] + u.y * f2[1];
-                    o[i][2] = o[i][2] * f[0] + u.z * f2[0];
-                    o[i][3] = o[i][3] * f[1] + u.w * f2[1];
-                }
-            }
-            __syncthreads();
-        }
-        if (team == 0) {
-            const bool whole = t0 == 0 && t1 == sp.tiles;
-            float *part = p.ws + (((size_t)blockIdx.y * ctas + cta) * 2 + (run.first ? 0 : 1)) * Shape::ROWS * (D + 2);
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int i0 = member * 8 + 2 * t + e, r = r0 + 2 * t + e;
-                if (r >= R) continue;
-                if (whole) {
-                    T *to = reinterpret_cast<T *>(p.out) + (((size_t)b * p.S + r % p.S) * p.Hq + h * p.group + r / p.S) * D;
-#pragma unroll
-                    for (int i = 0; i < DP / 8; i++)
-                        if (8 * i < D) to[8 * i + g] = from_f32<T>(paged_quotient(o[i >> 1][2 * (i & 1) + e], l[e]));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < DP / 8; i++)
-                        if (8 * i < D) part[(size_t)i0 * D + 8 * i + g] = o[i >> 1][2 * (i & 1) + e];
-                    if (g == 0) {
-                        part[Shape::ROWS * D + i0] = m[e] * kLn2;
-                        part[Shape::ROWS * D + Shape::ROWS + i0] = l[e];
-                    }
-                }
-            }
-        }
+        done_b = b, done_h = h;
+        whole = t0 == 0 && t1 == sp.tiles;
+        part = p.ws + (((size_t)blockIdx.y * ctas + cta) * 2 + (run.first ? 0 : 1)) * Shape::ROWS * (D + 2);
+        run.advance(p);
     }
     if (blockIdx.y == 0 && threadIdx.x == 0 && !p.whole) p.records[cta] = run.record;
 }
@@ -706,6 +713,7 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
     p.page = page, p.pages = pages, p.width = table_pages;
     p.row_blocks = n.row_blocks, p.block_rows = n.block_rows, p.round = n.round;
     p.whole = n.whole;
+    p.toll = n.mma ? 16 : 2 * n.round;
     p.strips = n.mma && page % kPagedTile == 0 && D == n.dim;
     p.records = reinterpret_cast<int4 *>(workspace);
     p.ws = reinterpret_cast<float *>(p.records + (n.whole ? 0 : n.ctas));
