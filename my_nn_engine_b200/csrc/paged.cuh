@@ -5,7 +5,7 @@
 // of the sequence with its new tokens, counts[b] the new tokens: query s of the sequence sits at position lengths[b] - counts[b] + s.
 //
 // Sequences of a batch have lengths of their own, so a fixed number of CTAs per sequence would leave most of the GPU waiting for the longest one.
-// The visible rows are cut into tiles of kPagedTile positions, and all tiles of all (sequence, kv head) pairs, one pair behind the other, are
+// The visible rows are cut into tiles of 16 or 32 positions (p.tile), and all tiles of all (sequence, kv head) pairs, one pair behind the other, are
 // dealt out evenly: each CTA takes one run of `share` tiles, which may end one pair, hold a few whole ones and begin another.  A pair that
 // lies in one CTA is finished there; the parts of the others go to a workspace and are joined by a second kernel.  A CTA has at most two parts:
 // the pair its run begins inside of (slot 0) and the pair it ends inside of (slot 1); it records the one that begins in it and ends elsewhere.  The lengths are on
@@ -17,7 +17,6 @@
 
 namespace mynn {
 
-constexpr int kPagedTile = 16;
 constexpr int kPagedWindow = INT_MAX - (1 << 17);
 
 struct PagedAttention {
@@ -29,18 +28,18 @@ struct PagedAttention {
     int B, S, Hq, G, group, D;
     int page, pages, width;  // rows of a page, pages of the cache, pages in a row of the table
     int row_blocks, block_rows;  // the group * S query rows of a pair, row r = head * S + s, in blocks
-    int round, toll;             // shares are multiples of `round`, the tiles that the warps of a CTA take at a time; toll: see PagedRun
+    int tile, round, toll;             // shares are multiples of `round`, the tiles that the warps of a CTA take at a time; toll: see PagedRun
     int4 *records;               // per CTA the pair that begins in it and ends in another: {b, h, last CTA, slot}, or b == -1
     float *ws;                   // [row block][CTA][2] parts of block_rows * (D + 2) floats: rows, then maxima, then sums
     int whole;                   // each pair is left to a CTA of its own
-    int strips;                  // tiles lie in one page each, and rows are as long on the chip as in the cache
+    int strips;                  // tiles of 16 lie in one page each, and rows are as long on the chip as in the cache
 };
 
 // What the new queries of a sequence see: the tiles of the first tokens, then those from the oldest query's window on.
 struct PagedSpan {
     int len, count, rows;         // rows: positions that the block table has entries for
     int sink_tiles, skip, tiles;  // skip: tiles between the two parts
-    __device__ __forceinline__ int base(int t) const { return (t + (t < sink_tiles ? 0 : skip)) * kPagedTile; }
+    __device__ __forceinline__ int at(int t) const { return t + (t < sink_tiles ? 0 : skip); }  // in tiles from the first position
 };
 
 __device__ __forceinline__ PagedSpan paged_span(const PagedAttention &p, int b) {
@@ -49,9 +48,10 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttention &p, int b) 
     s.rows = min(s.len, p.width * p.page);
     s.count = p.counts ? min(max(p.counts[b], 0), p.S) : p.S;
     const int oldest = s.len - s.count;
-    const int all = (s.rows + kPagedTile - 1) / kPagedTile;
-    const int lo = p.window > 0 ? min(max(0, oldest - p.window + 1) / kPagedTile, all) : 0;  // the tile that the windows begin in
-    s.sink_tiles = min((min(p.sinks, s.rows) + kPagedTile - 1) / kPagedTile, lo);
+    const int shift = p.tile == 16 ? 4 : 5, up = p.tile - 1;
+    const int all = (s.rows + up) >> shift;
+    const int lo = p.window > 0 ? min(max(0, oldest - p.window + 1) >> shift, all) : 0;  // the tile that the windows begin in
+    s.sink_tiles = min((min(p.sinks, s.rows) + up) >> shift, lo);
     s.skip = lo - s.sink_tiles;
     s.tiles = s.count > 0 ? all - s.skip : 0;
     return s;
@@ -71,8 +71,8 @@ __device__ __forceinline__ int paged_row(const PagedAttention &p, const PagedSpa
 }
 // All queries of the sequence see all of the tile (what a tile holds that only some see has to be kept from the others, not only weighted by zero: it may
 // be infinite).
-__device__ __forceinline__ bool paged_tile_full(const PagedAttention &p, const PagedSpan &sp, int base) {
-    return base + kPagedTile - 1 <= sp.len - sp.count && (p.window <= 0 || sp.len - 1 - base < p.window || base + kPagedTile <= p.sinks);
+__device__ __forceinline__ bool paged_tile_full(const PagedAttention &p, const PagedSpan &sp, int base, int tile) {
+    return base + tile - 1 <= sp.len - sp.count && (p.window <= 0 || sp.len - 1 - base < p.window || base + tile <= p.sinks);
 }
 
 struct PagedShare {

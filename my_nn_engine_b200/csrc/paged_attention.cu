@@ -10,6 +10,8 @@ namespace mynn {
 // of -inf, and adds nothing.
 __device__ __forceinline__ float paged_quotient(float O, float L) { return L == 0.f ? 0.f : O / L; }
 
+constexpr int kPagedTile = 16;  // of the kernel for any sizes
+
 // ---- any sizes ----------------------------------------------------------------------------------------------------------
 // f32 caches, heads that are no multiple of 8 numbers, unaligned tensors.  Each warp takes tiles of 16 positions into shared memory as f32; in the first product
 // a lane has one key and half of the dimensions, in the second the dimensions lane, lane + 32, ...
@@ -63,7 +65,7 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32) paged_attention_plain_ke
 #pragma unroll
             for (int i = 0; i < DL; i++) o[r][i] = 0.f;
         }
-        auto row_of = [&](int t) { return t < t1 ? paged_row(p, sp, b, h, sp.base(t) + key) : -1; };
+        auto row_of = [&](int t) { return t < t1 ? paged_row(p, sp, b, h, sp.at(t) * TILE + key) : -1; };
         auto issue = [&](int row, int stage) {
             float *to = ring + stage * 2 * TILE * PITCH;
 #pragma unroll 4
@@ -106,7 +108,7 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32) paged_attention_plain_ke
                     x[r] += a.x * c.x + a.y * c.y + a.z * c.z + a.w * c.w;
                 }
             }
-            const int j = sp.base(t) + key;
+            const int j = sp.at(t) * TILE + key;
 #pragma unroll
             for (int r = 0; r < RB; r++) {
                 x[r] += __shfl_xor_sync(0xffffffffu, x[r], 16);
@@ -124,7 +126,7 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32) paged_attention_plain_ke
                 for (int i = 0; i < DL; i++) o[r][i] *= keep;
             }
             __syncwarp();
-            const bool full = p.S == 1 || paged_tile_full(p, sp, sp.base(t));
+            const bool full = p.S == 1 || paged_tile_full(p, sp, sp.at(t) * TILE, TILE);
 #pragma unroll 2
             for (int k = 0; k < TILE; k++) {
                 float w[RB];
@@ -191,13 +193,14 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32) paged_attention_plain_ke
 // zeros, on the chip only.
 // The chain of one tile is long (two products, a softmax) and each warp walks it alone, so warps are what hides it: sixteen per SM, eight query rows each, rather than
 // eight with sixteen rows (96 mixed sequences of heads of 64: eight warps per SM 97 us).
+// A tile is 32 positions where three entries of that size fit, else 16: what goes on around the products takes as long as they do.
 template <int DP, int RW>
 struct MmaShape {
     static constexpr int W = 8, TEAMS = W / RW, ROWS = 8 * RW;
-    static constexpr int ENTRY = kPagedTile * DP * 2;
     static constexpr int CTAS = DP > 128 ? 1 : 2;  // per SM
-    static constexpr int FIT = (CTAS == 2 ? 96 : 192) * 1024 / TEAMS / ENTRY;
-    static constexpr int AHEAD = FIT >= 9 ? 4 : (FIT - 1) / 2, STAGES = 2 * AHEAD + 1;  // tiles on their way while one is worked on
+    static constexpr int SPACE = (CTAS == 2 ? 96 : 192) * 1024 / TEAMS;
+    static constexpr int TILE = SPACE / (32 * DP * 2) >= 3 ? 32 : 16, ENTRY = TILE * DP * 2;
+    static constexpr int FIT = (SPACE / ENTRY - 1) / 2, AHEAD = FIT < 3 ? FIT : 3, STAGES = 2 * AHEAD + 1;  // tiles on their way while one is worked on
     static constexpr size_t RING = (size_t)TEAMS * STAGES * ENTRY;
     static constexpr size_t SMEM = RING + W * 8 * 64 * sizeof(float);  // and 64 dimensions of all warps' sums
 };
@@ -227,7 +230,7 @@ __device__ __forceinline__ uint32_t special_mask(uint32_t x) {  // all ones over
 template <typename T, int DP, int RW>
 __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_mma_kernel(const PagedAttention p) {
     using Shape = MmaShape<DP, RW>;
-    constexpr int W = Shape::W, TEAMS = Shape::TEAMS, STAGES = Shape::STAGES, AHEAD = Shape::AHEAD, TILE = kPagedTile, KCH = DP / 32, CPR = DP / 8;
+    constexpr int W = Shape::W, TEAMS = Shape::TEAMS, STAGES = Shape::STAGES, AHEAD = Shape::AHEAD, TILE = Shape::TILE, KT = TILE / 16, KS = DP / 16, CPR = DP / 8;
     constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
     extern __shared__ __align__(128) uint8_t raw[];
     __shared__ float part_m[W][8], part_l[W][8];
@@ -239,6 +242,15 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
     float *sums = reinterpret_cast<float *>(raw + Shape::RING);
     const uint32_t ring_at = smem_u32(ring);
     const bool busy = r0 < R;  // a warp without rows of its own only helps to copy
+    // this lane's places: of its first copy in the cache and in an entry, of the first piece of a row of keys (row lane % 16) and, transposed, of values.  Entries
+    // begin on 128 bytes, so that another piece or row is an exclusive or away.
+    constexpr int COPIES = (TILE * CPR + 32 * RW - 1) / (32 * RW), STEP = 32 * RW / CPR;
+    constexpr bool EVEN = 32 * RW % CPR == 0;
+    constexpr uint32_t ALL = 0xffffffffu >> (32 - TILE);
+    const char *k_rows = reinterpret_cast<const char *>(p.k) + (member * 32 + lane) * 16, *v_rows = reinterpret_cast<const char *>(p.v) + (member * 32 + lane) * 16;
+    const int copy_row = (member * 32 + lane) / CPR, copy_piece = (member * 32 + lane) % CPR, k_row = lane & 15, v_row = (lane & 7) + (lane >> 4) * 8;
+    const uint32_t copy_lane = copy_row * (DP * 2) + (copy_piece >> 3) * 128 + paged_swizzle(copy_row, copy_piece & 7) * 16;
+    const uint32_t k_lane = ring_at + k_row * (DP * 2) + paged_swizzle(k_row, lane >> 4) * 16, v_lane = ring_at + v_row * (DP * 2) + paged_swizzle(v_row, lane >> 3 & 1) * 16;
     for (int b = cta; b < p.B; b += ctas)  // sequences that see nothing at all are in no CTA's run
         if (blockIdx.y == 0 && paged_span(p, b).tiles == 0)
             for (size_t n = (size_t)p.S * p.Hq * D / 8, i = threadIdx.x; i < n; i += W * 32) reinterpret_cast<uint4 *>(p.out)[b * n + i] = make_uint4(0, 0, 0, 0);
@@ -254,7 +266,7 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
     int done_b = -1, done_h = 0;
     bool whole = false;
     float *part = nullptr;
-    float o[DP / 16][4], m[2], l[2];
+    float o[KS][4], m[2], l[2], ref[2], limit[2];  // ref, limit: what weights are relative to, and the score that moves it
     for (;;) {
         const bool more = run.more(p, sp);
         const int b = run.b, h = run.h, t0 = run.t0, t1 = run.t1;
@@ -267,61 +279,87 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
         };
         const int at[2] = {last_seen(2 * t), last_seen(2 * t + 1)};  // this lane's two rows
         auto sees = [&](int last, int j) { return j <= last && (p.window <= 0 || last - j < p.window || j < p.sinks); };
-        auto base_of = [&](int j) { return sp.base(t0 + team + TEAMS * j); };
-        // The first row of a tile whose sixteen rows lie one behind the other and are all seen, for 32 tiles at once, one per lane; -1 for others.
-        auto strips_of = [&](int j) {
-            const int pos = base_of(j);
-            if (j >= mine || !p.strips || pos + TILE > sp.rows || (p.window > 0 && oldest - pos >= p.window && pos + TILE > p.sinks)) return -1;
+        auto base_of = [&](int j) { return sp.at(t0 + team + TEAMS * j) * TILE; };
+        // The first row of a sixteenth position and the fifteen behind it where these lie one behind the other and are all seen, for 32 of them at once, one
+        // per lane; -1 for others.
+        auto strips_of = [&](int i) {
+            const int j = i / KT, pos = base_of(j) + i % KT * 16;
+            if (j >= mine || !p.strips || pos + 16 > sp.rows || (p.window > 0 && oldest - pos >= p.window && pos + 16 > p.sinks)) return -1;
             return paged_row(p, sp, b, h, pos);
         };
-        auto row_of = [&](int j) { return j < mine ? paged_row(p, sp, b, h, base_of(j) + (lane & 15)) : -1; };
-        // The keys or the values of a tile to an entry of the ring.  strip: uniform; row: of position lane % 16, where strip < 0.
-        auto issue = [&](const void *rows, uint32_t entry, bool in_run, int strip, int row) {
-            constexpr int COPIES = (TILE * CPR + 32 * RW - 1) / (32 * RW);
+        auto row_of = [&](int j) { return j < mine ? paged_row(p, sp, b, h, base_of(j) + (lane & (TILE - 1))) : -1; };
+        // The keys or the values of a tile to an entry of the ring, from strips (uniform) where there are any, else row by row (row: of position lane % TILE).
+        auto issue = [&](const char *rows, uint32_t entry, bool in_run, bool fast, const int (&strip)[KT], int row, uint32_t there) {
             if (in_run) {
-                if (strip >= 0) {
-                    const char *src = reinterpret_cast<const char *>(rows) + (size_t)(uint32_t)strip * (DP * 2) + (member * 32 + lane) * 16;
+                const uint32_t to = ring_at + entry + copy_lane;
+                if (fast) {
+                    const char *src[KT];
+#pragma unroll
+                    for (int k = 0; k < KT; k++) src[k] = rows + (size_t)(uint32_t)strip[k] * (DP * 2);
 #pragma unroll
                     for (int i = 0; i < COPIES; i++) {
-                        const int idx = (i * RW + member) * 32 + lane, r = idx / CPR, c = idx % CPR;
-                        if (TILE * CPR % (32 * RW) != 0 && idx >= TILE * CPR) break;
-                        copy16_now(entry + r * (DP * 2) + (c >> 3) * 128 + paged_swizzle(r, c & 7) * 16, src + i * RW * 512);
+                        if constexpr (EVEN) {  // the lane's row moves on by STEP rows, its piece stays
+                            const char *from = KT == 1 || i < COPIES / 2 ? src[0] + i * RW * 512 : src[KT - 1] + (i - COPIES / 2) * RW * 512;
+                            if (KT == 2 && COPIES == 1) from = member * 32 < 16 * CPR ? src[0] : src[1] - 16 * DP * 2;
+                            copy16_now((to ^ (STEP * i & 7) << 4) + STEP * i * DP * 2, from);
+                        } else {
+                            const int idx = (i * RW + member) * 32 + lane, r = idx / CPR, c = idx % CPR;
+                            if (TILE * CPR % (32 * RW) != 0 && idx >= TILE * CPR) break;
+                            const char *from = KT == 1 || r < 16 ? src[0] + i * RW * 512 : src[KT - 1] + i * RW * 512 - 16 * DP * 2;
+                            copy16_now(ring_at + entry + r * (DP * 2) + (c >> 3) * 128 + paged_swizzle(r, c & 7) * 16, from);
+                        }
                     }
                 } else {
 #pragma unroll
                     for (int i = 0; i < COPIES; i++) {
                         const int idx = (i * RW + member) * 32 + lane, r = idx / CPR, c = idx % CPR;
-                        if (TILE * CPR % (32 * RW) != 0 && idx >= TILE * CPR) break;
-                        const int from = __shfl_sync(0xffffffffu, row, r & 15);
-                        const bool in = from >= 0 && 8 * c < D;
-                        const char *src = reinterpret_cast<const char *>(rows) + (size_t)(uint32_t)(in ? from : 0) * (uint32_t)(2 * D) + (in ? 16 * c : 0);
-                        copy16_at(entry + r * (DP * 2) + (c >> 3) * 128 + paged_swizzle(r, c & 7) * 16, src, in);
+                        if (TILE * CPR % (32 * RW) != 0 && idx >= TILE * CPR) break;  // (a whole warp)
+                        const int from = __shfl_sync(0xffffffffu, row, r);
+                        const bool in = (there >> r & 1) && 8 * c < D;
+                        const char *src = rows - (member * 32 + lane) * 16 + (size_t)(uint32_t)from * (uint32_t)(2 * D) + (8 * c < D ? 16 * c : 0);
+                        copy16_at(EVEN ? (to ^ (STEP * i & 7) << 4) + STEP * i * DP * 2 : ring_at + entry + r * (DP * 2) + (c >> 3) * 128 + paged_swizzle(r, c & 7) * 16, src, in);
                     }
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
+        // What issue() needs for tile j, and which rows of it there are.
+        int strips = -1, strips_next = -1, strip[KT], row = -1;
+        uint32_t there = 0;
+        bool fast = false;
+        auto look_up = [&](int j) {
+            if (j > 0 && (j * KT & 31) == 0) strips = strips_next, strips_next = strips_of(j * KT + 32 + lane);
+            fast = true;
+#pragma unroll
+            for (int k = 0; k < KT; k++) {
+                strip[k] = __shfl_sync(0xffffffffu, strips, (j * KT + k) & 31);
+                fast &= strip[k] >= 0;
+            }
+            there = ALL;
+            if (!fast) {
+                row = row_of(j);
+                there = __ballot_sync(0xffffffffu, row >= 0) & ALL;
+                row = max(row, 0);
+            }
+        };
         uint32_t exist[AHEAD + 1];  // which rows of the next tiles there are
-        int strips = -1, strips_next = -1, strip = -1, row = -1;
-        uint32_t qb[2 * KCH][2];  // row g, dimensions 16 i + 2 t and + 8
+        uint32_t qb[KS][2];  // row g, dimensions 16 i + 2 t and + 8
         if (more) {
             team_sync();  // the ring is free
             strips = strips_of(lane), strips_next = strips_of(lane + 32);
 #pragma unroll
             for (int j = 0; j < AHEAD; j++) {
-                strip = __shfl_sync(0xffffffffu, strips, j);
-                if (strip < 0) row = row_of(j);
-                exist[j] = strip >= 0 ? 0xffffu : __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
-                issue(p.k, ring_at + 2 * j * Shape::ENTRY, j < mine, strip, row);
-                issue(p.v, ring_at + (2 * j + 1) * Shape::ENTRY, j < mine, strip, row);
+                look_up(j);
+                exist[j] = there;
+                issue(k_rows, 2 * j * Shape::ENTRY, j < mine, fast, strip, row, there);
+                issue(v_rows, (2 * j + 1) * Shape::ENTRY, j < mine, fast, strip, row, there);
             }
-            strip = __shfl_sync(0xffffffffu, strips, AHEAD);
-            if (strip < 0) row = row_of(AHEAD);
+            look_up(AHEAD);
             const int r = min(r0 + g, R - 1);
             const bool in = r0 + g < R && r % p.S < sp.count;
             const T *qr = reinterpret_cast<const T *>(p.q) + (((size_t)b * p.Hq + h * p.group + r / p.S) * p.S + r % p.S) * D;
 #pragma unroll
-            for (int i = 0; i < 2 * KCH; i++)
+            for (int i = 0; i < KS; i++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     const int d = 16 * i + 8 * e + 2 * t;
@@ -370,7 +408,8 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
                     if (whole) {
                         const int q = blockIdx.y * Shape::ROWS + r;
                         T *to = reinterpret_cast<T *>(p.out) + (((size_t)done_b * p.S + q % p.S) * p.Hq + done_h * p.group + q / p.S) * D + 64 * s + d;
-                        __align__(4) T y[2] = {from_f32<T>(paged_quotient(O.x, L)), from_f32<T>(paged_quotient(O.y, L))};
+                        const float inv = __frcp_rn(L);  // (a second rounding of 2^-24 in front of one of 2^-9 or 2^-11)
+                        __align__(4) T y[2] = {from_f32<T>(L == 0.f ? 0.f : O.x * inv), from_f32<T>(L == 0.f ? 0.f : O.y * inv)};
                         *reinterpret_cast<uint32_t *>(to) = *reinterpret_cast<const uint32_t *>(y);
                     } else {
                         *reinterpret_cast<float2 *>(part + (size_t)r * D + 64 * s + d) = O;
@@ -385,7 +424,7 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
         if (!more) break;
         uint32_t cur = 0, free_entry = (STAGES - 1) * Shape::ENTRY;  // offsets: the entry that is read next, the one that is empty
 #pragma unroll
-        for (int e = 0; e < 2; e++) m[e] = -INFINITY, l[e] = 0.f;
+        for (int e = 0; e < 2; e++) m[e] = limit[e] = -INFINITY, ref[e] = l[e] = 0.f;
 #pragma unroll
         for (int i = 0; i < DP / 16; i++)
 #pragma unroll
@@ -395,100 +434,123 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
             team_sync();  // the keys of tile j are here, and the values of tile j - 1 are done with
             const int ahead = j + AHEAD;
-            exist[AHEAD] = strip >= 0 ? 0xffffu : __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
-            issue(p.k, ring_at + free_entry, ahead < mine, strip, row);
+            exist[AHEAD] = there;
+            issue(k_rows, free_entry, ahead < mine, fast, strip, row, there);
             const int base = base_of(j);
-            const uint32_t K = ring_at + cur;
+            const uint32_t K = k_lane + cur;
             free_entry = cur;
             cur = cur + Shape::ENTRY == STAGES * Shape::ENTRY ? 0 : cur + Shape::ENTRY;
-            // ---- S^T = K Q^T: x[2 k + e] is position base + g + 8 k, row 2 t + e ----
-            float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-            uint32_t hi[2], lo[2];
-            const bool full = exist[0] == 0xffffu && (p.S == 1 || paged_tile_full(p, sp, base));
+            // ---- S^T = K Q^T: x[k][2 c + e] is position base + 16 k + g + 8 c, row 2 t + e ----
+            float x[KT][4], y[KT][4];
+            uint32_t hi[KT][2], lo[KT][2];
+            const bool full = exist[0] == ALL && (p.S == 1 || paged_tile_full(p, sp, base, TILE));
             if (busy) {
 #pragma unroll
-                for (int i = 0; i < 2 * KCH; i++) {
-                    uint32_t a[4];
-                    const int krow = lane & 15;
-                    ldsm4_at(a, K + krow * (DP * 2) + (i >> 2) * 128 + paged_swizzle(krow, 2 * (i & 3) + (lane >> 4)) * 16);
-                    mma_kv<T>(i & 1 ? y : x, a[0], a[1], a[2], a[3], qb[i][0], qb[i][1]);
-                }
+                for (int k = 0; k < KT; k++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    x[i] += y[i];
-                    if (p.softcap > 0.f) x[i] = kLog2e * fast_soft_cap(x[i] * p.scale, p.softcap);
-                    else x[i] *= unit;
+                    for (int i = 0; i < 4; i++) x[k][i] = y[k][i] = 0.f;
+#pragma unroll
+                for (int i = 0; i < KS; i++)
+#pragma unroll
+                    for (int k = 0; k < KT; k++) {
+                        uint32_t a[4];
+                        ldsm4_at(a, (K ^ (i & 3) << 5) + (i >> 2) * 128 + k * 16 * DP * 2);
+                        mma_kv<T>(KT == 1 && (i & 1) ? y[k] : x[k], a[0], a[1], a[2], a[3], qb[i][0], qb[i][1]);
+                    }
+                float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int k = 0; k < KT; k++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if (KT == 1) x[k][i] += y[k][i];
+                        x[k][i] *= unit;
+                    }
+                if (p.softcap > 0.f) {
+#pragma unroll
+                    for (int k = 0; k < KT; k++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) x[k][i] = kLog2e * fast_soft_cap(x[k][i] * kLn2, p.softcap);
                 }
                 if (!full) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int bit = g + 8 * (i >> 1);
-                        if (!((exist[0] >> bit & 1) && sees(at[i & 1], base + bit))) x[i] = -INFINITY;
-                    }
+                    for (int k = 0; k < KT; k++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int bit = 16 * k + g + 8 * (i >> 1);
+                            if (!((exist[0] >> bit & 1) && sees(at[i & 1], base + bit))) x[k][i] = -INFINITY;
+                        }
                 }
-                if (__any_sync(0xffffffffu, fmaxf(x[0], x[2]) > m[0] + 8.f || fmaxf(x[1], x[3]) > m[1] + 8.f)) {
+#pragma unroll
+                for (int k = 0; k < KT; k++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) most[i & 1] = fmaxf(most[i & 1], x[k][i]);
+                if (__any_sync(0xffffffffu, most[0] > limit[0] || most[1] > limit[1])) {
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        float top = fmaxf(x[e], x[2 + e]);
+                        float top = most[e];
 #pragma unroll
                         for (int s = 4; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
                         const float now = fmaxf(m[e], top), keep = exp2_approx(m[e] - merge_reference(now));
                         m[e] = now;
+                        ref[e] = merge_reference(now);
+                        limit[e] = now + 8.f;
                         l[e] *= keep;
 #pragma unroll
-                        for (int i = 0; i < DP / 16; i++) o[i][e] *= keep, o[i][2 + e] *= keep;
+                        for (int i = 0; i < KS; i++) o[i][e] *= keep, o[i][2 + e] *= keep;
                     }
                 }
-                const float r0_ = merge_reference(m[0]), r1_ = merge_reference(m[1]);
-                x[0] = exp2_approx(x[0] - r0_), x[1] = exp2_approx(x[1] - r1_), x[2] = exp2_approx(x[2] - r0_), x[3] = exp2_approx(x[3] - r1_);
-                l[0] += x[0] + x[2];  // of this lane's positions
-                l[1] += x[1] + x[3];
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    split_pack<T>(x[2 * k], x[2 * k + 1], hi[k], lo[k]);
-                    hi[k] = transpose_8x8(hi[k]), lo[k] = transpose_8x8(lo[k]);  // positions 8 k + 2 t, + 1 of row g
+                for (int k = 0; k < KT; k++) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[k][i] = exp2_approx(x[k][i] - ref[i & 1]);
+                    l[0] += x[k][0] + x[k][2];  // of this lane's positions
+                    l[1] += x[k][1] + x[k][3];
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        split_pack<T>(x[k][2 * c], x[k][2 * c + 1], hi[k][c], lo[k][c]);
+                        hi[k][c] = transpose_8x8(hi[k][c]), lo[k][c] = transpose_8x8(lo[k][c]);  // positions 16 k + 8 c + 2 t, + 1 of row g
+                    }
                 }
             }
             asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
             team_sync();  // the values of tile j are here, and its keys are done with
-            issue(p.v, ring_at + free_entry, ahead < mine, strip, row);
-            if (((ahead + 1) & 31) == 0) strips = strips_next, strips_next = strips_of(ahead + 33 + lane);
-            strip = __shfl_sync(0xffffffffu, strips, (ahead + 1) & 31);
-            if (strip < 0) row = row_of(ahead + 1);
-            const uint32_t V = ring_at + cur;
+            issue(v_rows, free_entry, ahead < mine, fast, strip, row, there);
+            look_up(ahead + 1);
+            const uint32_t V = v_lane + cur;
             free_entry = cur;
             cur = cur + Shape::ENTRY == STAGES * Shape::ENTRY ? 0 : cur + Shape::ENTRY;
             // ---- O^T += V^T P^T: o[i] is dimensions 16 i + g (registers 0, 1) and + 8 (2, 3) of rows 2 t and 2 t + 1 ----
             if (busy) {
+                const bool guarded = !full && p.S > 1;
 #pragma unroll
-                for (int i = 0; i < DP / 16; i++) {
-                    uint32_t a[4];
-                    const int vrow = (lane & 7) + (lane >> 4) * 8;
-                    ldsm4t_at(a, V + vrow * (DP * 2) + (i >> 2) * 128 + paged_swizzle(vrow, 2 * (i & 3) + (lane >> 3 & 1)) * 16);
-                    if (!full && p.S > 1) {
-                        // Values that are no numbers, in a tile that not every row sees all of: they are taken out of the product and added position by
-                        // position where they are seen, so that the other rows keep their bits.
-                        uint32_t sp_[4];
+                for (int i = 0; i < KS; i++)
 #pragma unroll
-                        for (int c = 0; c < 4; c++) sp_[c] = special_mask<T>(a[c]);
-                        if (__any_sync(0xffffffffu, (sp_[0] | sp_[1] | sp_[2] | sp_[3]) != 0u)) {
+                    for (int k = 0; k < KT; k++) {
+                        uint32_t a[4];
+                        ldsm4t_at(a, (V ^ (i & 3) << 5) + (i >> 2) * 128 + k * 16 * DP * 2);
+                        if (guarded) {
+                            // Values that are no numbers, in a tile that not every row sees all of: they are taken out of the product and added position by
+                            // position where they are seen, so that the other rows keep their bits.
+                            uint32_t odd[4];
+#pragma unroll
+                            for (int c = 0; c < 4; c++) odd[c] = special_mask<T>(a[c]);
+                            if (__any_sync(0xffffffffu, (odd[0] | odd[1] | odd[2] | odd[3]) != 0u)) {
 #pragma unroll 1
-                            for (int k = 0; k < TILE; k++) {
-                                const uint32_t one = (k & 7) >> 1 == t ? (k & 1 ? 0xffff0000u : 0xffffu) : 0u, first = k < 8 ? one : 0u, second = k < 8 ? 0u : one;
-                                const uint32_t b0 = a[0] & sp_[0] & first, b1 = a[1] & sp_[1] & first, b2 = a[2] & sp_[2] & second, b3 = a[3] & sp_[3] & second;
-                                float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                                mma_kv<T>(acc, b0, b1, b2, b3, hi[0], hi[1]);
+                                for (int n = 0; n < 16; n++) {
+                                    const uint32_t one = (n & 7) >> 1 == t ? (n & 1 ? 0xffff0000u : 0xffffu) : 0u, first = n < 8 ? one : 0u, second = n < 8 ? 0u : one;
+                                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                                    mma_kv<T>(acc, a[0] & odd[0] & first, a[1] & odd[1] & first, a[2] & odd[2] & second, a[3] & odd[3] & second, hi[k][0], hi[k][1]);
 #pragma unroll
-                                for (int e = 0; e < 2; e++)
-                                    if ((exist[0] >> k & 1) && sees(at[e], base + k)) o[i][e] += acc[e], o[i][2 + e] += acc[2 + e];
+                                    for (int e = 0; e < 2; e++)
+                                        if ((exist[0] >> (16 * k + n) & 1) && sees(at[e], base + 16 * k + n)) o[i][e] += acc[e], o[i][2 + e] += acc[2 + e];
+                                }
+#pragma unroll
+                                for (int c = 0; c < 4; c++) a[c] &= ~odd[c];
                             }
-#pragma unroll
-                            for (int c = 0; c < 4; c++) a[c] &= ~sp_[c];
                         }
+                        mma_kv<T>(o[i], a[0], a[1], a[2], a[3], hi[k][0], hi[k][1]);
+                        mma_kv<T>(o[i], a[0], a[1], a[2], a[3], lo[k][0], lo[k][1]);
                     }
-                    mma_kv<T>(o[i], a[0], a[1], a[2], a[3], hi[0], hi[1]);
-                    mma_kv<T>(o[i], a[0], a[1], a[2], a[3], lo[0], lo[1]);
-                }
             }
 #pragma unroll
             for (int i = 0; i < AHEAD; i++) exist[i] = exist[i + 1];
@@ -596,14 +658,22 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attention_join_kernel(c
 // How the launch is cut: kernel, query rows of a block, CTAs.
 struct PagedPlan {
     bool mma;
+    int tile;
     int dim, team;  // padded head dimension, warps of a team
     int ctas, block_rows, row_blocks, round;
     bool whole;
     size_t bytes(int D) const { return whole ? 16 : (size_t)ctas * sizeof(int4) + (size_t)ctas * row_blocks * 2 * block_rows * (D + 2) * sizeof(float); }
 };
 
-// Tiles of a pair up to which it is not cut.
-constexpr int kPagedWhole = 32;
+// Positions of a block table up to which pairs are not cut.
+constexpr int kPagedWhole = 512;
+
+template <int DP>
+static int mma_tile(int team) {
+    return team == 1 ? MmaShape<DP, 1>::TILE : team == 2 ? MmaShape<DP, 2>::TILE : team == 4 ? MmaShape<DP, 4>::TILE : MmaShape<DP, 8>::TILE;
+}
+static int paged_mma_tile(int dim, int team) { return dim == 64 ? mma_tile<64>(team) : dim == 128 ? mma_tile<128>(team) : dim == 192 ? mma_tile<192>(team) : mma_tile<256>(team); }
+
 
 static int paged_sms(int *sms) {
     int dev = 0;
@@ -621,8 +691,9 @@ static PagedPlan paged_plan(int B, int S, int Hq, int Hkv, int D, int page, int 
     n.block_rows = mma ? 8 * n.team : kPlainRows;
     n.row_blocks = (R + n.block_rows - 1) / n.block_rows;
     n.round = mma ? 8 / n.team : D <= 128 ? 4 : kPlainWarps<8>;
-    const long long tiles = ((long long)width * page + kPagedTile - 1) / kPagedTile, most = mma && n.dim <= 128 ? 2 * sms : sms;
-    n.whole = tiles <= kPagedWhole;
+    n.tile = mma ? paged_mma_tile(n.dim, n.team) : kPagedTile;
+    const long long tiles = ((long long)width * page + n.tile - 1) / n.tile, most = mma && n.dim <= 128 ? 2 * sms : sms;
+    n.whole = (long long)width * page <= kPagedWhole;
     n.ctas = n.whole ? B * Hkv : (int)std::min<long long>(most, std::max<long long>(1, (tiles * Hkv * B + n.round - 1) / n.round));
     return n;
 }
@@ -713,8 +784,9 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
     p.page = page, p.pages = pages, p.width = table_pages;
     p.row_blocks = n.row_blocks, p.block_rows = n.block_rows, p.round = n.round;
     p.whole = n.whole;
-    p.toll = n.mma ? 16 : 2 * n.round;
-    p.strips = n.mma && page % kPagedTile == 0 && D == n.dim;
+    p.tile = n.tile;
+    p.toll = n.mma ? 256 / n.tile : 2 * n.round;
+    p.strips = n.mma && page % 16 == 0 && D == n.dim;
     p.records = reinterpret_cast<int4 *>(workspace);
     p.ws = reinterpret_cast<float *>(p.records + (n.whole ? 0 : n.ctas));
     const cudaStream_t st = (cudaStream_t)stream;
