@@ -520,36 +520,47 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             free_entry = cur;
             cur = cur + Shape::ENTRY == STAGES * Shape::ENTRY ? 0 : cur + Shape::ENTRY;
             // ---- O^T += V^T P^T: o[i] is dimensions 16 i + g (registers 0, 1) and + 8 (2, 3) of rows 2 t and 2 t + 1 ----
-            if (busy) {
-                const bool guarded = !full && p.S > 1;
+            // Values that are no numbers, in a tile that not every row sees all of?
+            bool odd = false;
+            if (!full && p.S > 1) {
+#pragma unroll 1
+                for (int i = lane; i < TILE * CPR; i += 32) {
+                    const uint4 u = *reinterpret_cast<const uint4 *>(ring + free_entry + i * 16);
+                    odd |= (special_mask<T>(u.x) | special_mask<T>(u.y) | special_mask<T>(u.z) | special_mask<T>(u.w)) != 0u;
+                }
+                odd = __any_sync(0xffffffffu, odd);
+            }
+            if (busy && !odd) {
 #pragma unroll
                 for (int i = 0; i < KS; i++)
 #pragma unroll
                     for (int k = 0; k < KT; k++) {
                         uint32_t a[4];
                         ldsm4t_at(a, (V ^ (i & 3) << 5) + (i >> 2) * 128 + k * 16 * DP * 2);
-                        if (guarded) {
-                            // Values that are no numbers, in a tile that not every row sees all of: they are taken out of the product and added position by
-                            // position where they are seen, so that the other rows keep their bits.
-                            uint32_t odd[4];
-#pragma unroll
-                            for (int c = 0; c < 4; c++) odd[c] = special_mask<T>(a[c]);
-                            if (__any_sync(0xffffffffu, (odd[0] | odd[1] | odd[2] | odd[3]) != 0u)) {
-#pragma unroll 1
-                                for (int n = 0; n < 16; n++) {
-                                    const uint32_t one = (n & 7) >> 1 == t ? (n & 1 ? 0xffff0000u : 0xffffu) : 0u, first = n < 8 ? one : 0u, second = n < 8 ? 0u : one;
-                                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                                    mma_kv<T>(acc, a[0] & odd[0] & first, a[1] & odd[1] & first, a[2] & odd[2] & second, a[3] & odd[3] & second, hi[k][0], hi[k][1]);
-#pragma unroll
-                                    for (int e = 0; e < 2; e++)
-                                        if ((exist[0] >> (16 * k + n) & 1) && sees(at[e], base + 16 * k + n)) o[i][e] += acc[e], o[i][2 + e] += acc[2 + e];
-                                }
-#pragma unroll
-                                for (int c = 0; c < 4; c++) a[c] &= ~odd[c];
-                            }
-                        }
                         mma_kv<T>(o[i], a[0], a[1], a[2], a[3], hi[k][0], hi[k][1]);
                         mma_kv<T>(o[i], a[0], a[1], a[2], a[3], lo[k][0], lo[k][1]);
+                    }
+            } else if (busy) {
+                // They are taken out of the product and added position by position where they are seen, so that the other rows keep their bits.
+#pragma unroll
+                for (int i = 0; i < KS; i++)
+#pragma unroll
+                    for (int k = 0; k < KT; k++) {
+                        uint32_t a[4], c[4];
+                        ldsm4t_at(a, (V ^ (i & 3) << 5) + (i >> 2) * 128 + k * 16 * DP * 2);
+#pragma unroll
+                        for (int n = 0; n < 4; n++) c[n] = a[n] & special_mask<T>(a[n]), a[n] &= ~special_mask<T>(a[n]);
+                        mma_kv<T>(o[i], a[0], a[1], a[2], a[3], hi[k][0], hi[k][1]);
+                        mma_kv<T>(o[i], a[0], a[1], a[2], a[3], lo[k][0], lo[k][1]);
+#pragma unroll 1
+                        for (int n = 0; n < 16; n++) {
+                            const uint32_t one = (n & 7) >> 1 == t ? (n & 1 ? 0xffff0000u : 0xffffu) : 0u, first = n < 8 ? one : 0u, second = n < 8 ? 0u : one;
+                            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma_kv<T>(acc, c[0] & first, c[1] & first, c[2] & second, c[3] & second, hi[k][0], hi[k][1]);
+#pragma unroll
+                            for (int e = 0; e < 2; e++)
+                                if ((exist[0] >> (16 * k + n) & 1) && sees(at[e], base + 16 * k + n)) o[i][e] += acc[e], o[i][2 + e] += acc[2 + e];
+                        }
                     }
             }
 #pragma unroll
