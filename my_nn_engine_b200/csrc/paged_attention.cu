@@ -274,8 +274,8 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
         const int oldest = sp.len - sp.count;
         // last position that row r0 + i sees, -1: it is no query
         auto last_seen = [&](int i) {
-            const int r = r0 + i;
-            return r < R && r % p.S < sp.count ? oldest + r % p.S : -1;
+            const int r = r0 + i, s = p.by_S.mod(r, p.by_S.div(r));
+            return r < R && s < sp.count ? oldest + s : -1;
         };
         const int at[2] = {last_seen(2 * t), last_seen(2 * t + 1)};  // this lane's two rows
         auto sees = [&](int last, int j) { return j <= last && (p.window <= 0 || last - j < p.window || j < p.sinks); };
@@ -355,9 +355,9 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
                 issue(v_rows, (2 * j + 1) * Shape::ENTRY, j < mine, fast, strip, row, there);
             }
             look_up(AHEAD);
-            const int r = min(r0 + g, R - 1);
-            const bool in = r0 + g < R && r % p.S < sp.count;
-            const T *qr = reinterpret_cast<const T *>(p.q) + (((size_t)b * p.Hq + h * p.group + r / p.S) * p.S + r % p.S) * D;
+            const int r = min(r0 + g, R - 1), head = p.by_S.div(r), s = p.by_S.mod(r, head);
+            const bool in = r0 + g < R && s < sp.count;
+            const T *qr = reinterpret_cast<const T *>(p.q) + (((size_t)b * p.Hq + h * p.group + head) * p.S + s) * D;
 #pragma unroll
             for (int i = 0; i < KS; i++)
 #pragma unroll
@@ -406,8 +406,8 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
                     for (int w = 0; w < TEAMS; w++) L += part_l[w * RW + w0][r & 7] * exp2_approx(part_m[w * RW + w0][r & 7] - merge_reference(top));
                     if (64 * s + d >= D) continue;
                     if (whole) {
-                        const int q = blockIdx.y * Shape::ROWS + r;
-                        T *to = reinterpret_cast<T *>(p.out) + (((size_t)done_b * p.S + q % p.S) * p.Hq + done_h * p.group + q / p.S) * D + 64 * s + d;
+                        const int q = blockIdx.y * Shape::ROWS + r, head = p.by_S.div(q);
+                        T *to = reinterpret_cast<T *>(p.out) + (((size_t)done_b * p.S + p.by_S.mod(q, head)) * p.Hq + done_h * p.group + head) * D + 64 * s + d;
                         const float inv = __frcp_rn(L);  // (a second rounding of 2^-24 in front of one of 2^-9 or 2^-11)
                         __align__(4) T y[2] = {from_f32<T>(L == 0.f ? 0.f : O.x * inv), from_f32<T>(L == 0.f ? 0.f : O.y * inv)};
                         *reinterpret_cast<uint32_t *>(to) = *reinterpret_cast<const uint32_t *>(y);
@@ -658,7 +658,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attention_join_kernel(c
         }
     }
     if (!in) return;
-    T *out = reinterpret_cast<T *>(p.out) + (((size_t)rec.x * p.S + r % p.S) * p.Hq + rec.y * p.group + r / p.S) * D;
+    const int head = p.by_S.div(r);
+    T *out = reinterpret_cast<T *>(p.out) + (((size_t)rec.x * p.S + p.by_S.mod(r, head)) * p.Hq + rec.y * p.group + head) * D;
 #pragma unroll
     for (int k = 0; k < ITEMS; k++)
 #pragma unroll
@@ -793,6 +794,7 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
     p.scale = scale, p.softcap = softcap, p.window = std::min(window, kPagedWindow), p.sinks = sinks;
     p.B = B, p.S = S, p.Hq = Hq, p.G = Hkv, p.group = Hq / Hkv, p.D = D;
     p.page = page, p.pages = pages, p.width = table_pages;
+    p.by_page = FixedDivisor(page), p.by_S = FixedDivisor(S);
     p.row_blocks = n.row_blocks, p.block_rows = n.block_rows, p.round = n.round;
     p.whole = n.whole;
     p.tile = n.tile;
