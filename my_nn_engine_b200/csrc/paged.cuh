@@ -39,11 +39,12 @@ struct PagedAttention {
     int window, sinks;  // window: at most kPagedWindow (positions are below 2^31, and new tokens may lie before the first one)
     int B, S, Hq, G, group, D;
     int page, pages, width;  // rows of a page, pages of the cache, pages in a row of the table
-    FixedDivisor by_page, by_S;
+    FixedDivisor by_page, by_S, by_pieces;  // by_pieces: copies of a row, of the kernel for any sizes
     int row_blocks, block_rows;  // the group * S query rows of a pair, row r = head * S + s, in blocks
     int tile, round, toll;             // shares are multiples of `round`, the tiles that the warps of a CTA take at a time; toll: see PagedRun
     int4 *records;               // per CTA the pair that begins in it and ends in another: {b, h, last CTA, slot}, or b == -1
-    float *ws;                   // [row block][CTA][2] parts of block_rows * (D + 2) floats: rows, then maxima, then sums
+    float *ws;                   // [row block][CTA][2] parts of part_floats floats: block_rows rows of D, then maxima, then sums
+    int part_floats;             // a multiple of 4
     int whole;                   // each pair is left to a CTA of its own
     int strips;                  // tiles of 16 lie in one page each, and rows are as long on the chip as in the cache
 };

@@ -15,47 +15,78 @@ constexpr int kPagedTile = 16;  // of the kernel for any sizes
 // ---- any sizes ----------------------------------------------------------------------------------------------------------
 // f32 caches, heads that are no multiple of 8 numbers, unaligned tensors.  Each warp takes tiles of 16 positions into shared memory as f32; in the first product
 // a lane has one key and half of the dimensions, in the second the dimensions lane, lane + 32, ...
+// RB: query rows of a CTA (one head per kv head: with eight rows where one is needed 7 sequences of 1 to 1501, 12 heads of 80, took 46 us).
 // VEC: elements of a copy to shared memory (cp.async, f32); 0: 16-bit elements, converted on the way.
-constexpr int kPlainRows = 8;
 template <int DL>
 constexpr int kPlainWarps = DL > 4 ? 2 : 4;
-template <int DL>
-constexpr size_t plain_smem() {
-    constexpr int pitch = DL * 32 + 4, warps = kPlainWarps<DL>;
-    return sizeof(float) * (size_t)(warps * (2 * 2 * kPagedTile * pitch + kPagedTile * kPlainRows) + kPlainRows * pitch);
-}
+template <int DL, int RB>
+struct PlainShape {
+    static constexpr int W = kPlainWarps<DL>, PITCH = DL * 32 + 4;
+    static constexpr int RING = 2 * 2 * kPagedTile * PITCH;  // floats of a warp: two stages, keys and values
+    static constexpr int WEIGHTS = kPagedTile * (RB < 4 ? 4 : RB), SUMS = RB * DL * 32;
+    static constexpr size_t SMEM = sizeof(float) * (size_t)(RB * PITCH + W * (RING + WEIGHTS + SUMS));
+    static constexpr int CTAS = SMEM <= 112 * 1024 ? 2 : 1;  // per SM
+};
 
 template <int BYTES>
 __device__ __forceinline__ void copy_async(void *smem, const void *gmem, bool in) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(smem_u32(smem)), "l"(gmem), "n"(BYTES), "r"(in ? BYTES : 0) : "memory");
 }
 
-template <typename T, int DL, int VEC>
-__global__ void __launch_bounds__(kPlainWarps<DL> * 32) paged_attention_plain_kernel(const PagedAttention p) {
-    constexpr int RB = kPlainRows, W = kPlainWarps<DL>, PITCH = DL * 32 + 4, TILE = kPagedTile;
+template <typename T, int DL, int RB, int VEC>
+__global__ void __launch_bounds__(kPlainWarps<DL> * 32, PlainShape<DL, RB>::CTAS) paged_attention_plain_kernel(const PagedAttention p) {
+    using Shape = PlainShape<DL, RB>;
+    constexpr int W = Shape::W, PITCH = Shape::PITCH, TILE = kPagedTile, WR = Shape::WEIGHTS / TILE;
     extern __shared__ __align__(16) float sm[];
     __shared__ float part_m[W][RB], part_l[W][RB];
     pdl_trigger();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, key = lane & 15, side = lane >> 4;
     const int cta = blockIdx.x, ctas = gridDim.x, r0 = blockIdx.y * RB, rows = min(p.group * p.S - r0, RB), D = p.D;
-    float *sq = sm, *ring = sm + RB * PITCH + warp * (2 * 2 * TILE * PITCH), *weights = sm + RB * PITCH + W * (2 * 2 * TILE * PITCH) + warp * TILE * RB;
+    float *sq = sm, *ring = sm + RB * PITCH + warp * Shape::RING, *weights = sm + RB * PITCH + W * Shape::RING + warp * Shape::WEIGHTS;
+    float *sums = sm + RB * PITCH + W * (Shape::RING + Shape::WEIGHTS);
     for (int i = threadIdx.x; i < RB * PITCH; i += W * 32) sq[i] = 0.f;
-    for (int i = lane; i < 2 * 2 * TILE * PITCH; i += 32) ring[i] = 0.f;  // what lies behind D is never written again
-    auto place = [&](int b, int h, int r, int d) { return (((size_t)b * p.S + r % p.S) * p.Hq + h * p.group + r / p.S) * D + d; };
+    for (int i = lane; i < Shape::RING; i += 32) ring[i] = 0.f;  // what lies behind D is never written again
+    auto place = [&](int b, int h, int r, int d) {
+        const int head = p.by_S.div(r);
+        return (((size_t)b * p.S + p.by_S.mod(r, head)) * p.Hq + h * p.group + head) * D + d;
+    };
     for (int b = cta; b < p.B; b += ctas)  // sequences that see nothing at all are in no CTA's run
         if (paged_span(p, b).tiles == 0)
-            for (int i = threadIdx.x; i < p.G * rows * D; i += W * 32)
-                reinterpret_cast<T *>(p.out)[place(b, i / (rows * D), r0 + i / D % rows, i % D)] = from_f32<T>(0.f);
+            for (int h = 0; h < p.G; h++)
+                for (int i = threadIdx.x; i < rows * D; i += W * 32) reinterpret_cast<T *>(p.out)[place(b, h, r0 + i / D, i % D)] = from_f32<T>(0.f);
     PagedRun run;
     run.begin(paged_find<W * 32>(p, cta, ctas));
     PagedSpan sp;
     for (; run.more(p, sp); run.advance(p)) {
         const int b = run.b, h = run.h, t0 = run.t0, t1 = run.t1;
-        __syncthreads();
+        auto row_of = [&](int t) { return t < t1 ? paged_row(p, sp, b, h, sp.at(t) * TILE + key) : -1; };
+        auto issue = [&](int row, int stage) {
+            float *to = ring + stage * 2 * TILE * PITCH;
+            const int pieces = VEC > 0 ? D / VEC : D;
+#pragma unroll 2
+            for (int i = lane; i < (TILE * pieces + 31) / 32 * 32; i += 32) {
+                const int r = p.by_pieces.div(i), d = (i - r * pieces) * (VEC > 0 ? VEC : 1);
+                const int from = __shfl_sync(0xffffffffu, row, r & 15);
+                if (r >= TILE) continue;
+                const size_t at = (size_t)(uint32_t)max(from, 0) * (uint32_t)D + d;
+                float *dst = to + r * PITCH + d;
+                if constexpr (VEC > 0) {
+                    copy_async<4 * VEC>(dst, reinterpret_cast<const float *>(p.k) + at, from >= 0);
+                    copy_async<4 * VEC>(dst + TILE * PITCH, reinterpret_cast<const float *>(p.v) + at, from >= 0);
+                } else {
+                    dst[0] = from >= 0 ? to_f32<T>(reinterpret_cast<const T *>(p.k)[at]) : 0.f;
+                    dst[TILE * PITCH] = from >= 0 ? to_f32<T>(reinterpret_cast<const T *>(p.v)[at]) : 0.f;
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        int row = row_of(t0 + warp), next = row_of(t0 + warp + W);
+        if (t0 + warp < t1) issue(row, 0);
+        __syncthreads();  // the queries and sums of the pair in front are done with
         for (int i = threadIdx.x; i < rows * D; i += W * 32) {
-            const int r = r0 + i / D;
-            sq[i / D * PITCH + i % D] = to_f32<T>(reinterpret_cast<const T *>(p.q)[(((size_t)b * p.Hq + h * p.group + r / p.S) * p.S + r % p.S) * D + i % D]);
+            const int r = r0 + i / D, head = p.by_S.div(r);
+            sq[i / D * PITCH + i % D] = to_f32<T>(reinterpret_cast<const T *>(p.q)[(((size_t)b * p.Hq + h * p.group + head) * p.S + p.by_S.mod(r, head)) * D + i % D]);
         }
         __syncthreads();
         float m[RB], l[RB], o[RB][DL];
@@ -65,29 +96,6 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32) paged_attention_plain_ke
 #pragma unroll
             for (int i = 0; i < DL; i++) o[r][i] = 0.f;
         }
-        auto row_of = [&](int t) { return t < t1 ? paged_row(p, sp, b, h, sp.at(t) * TILE + key) : -1; };
-        auto issue = [&](int row, int stage) {
-            float *to = ring + stage * 2 * TILE * PITCH;
-#pragma unroll 4
-            for (int r = 0; r < TILE; r++) {
-                const int from = __shfl_sync(0xffffffffu, row, r);
-                const size_t at = (size_t)max(from, 0) * D;
-                if constexpr (VEC > 0) {
-                    for (int d = lane * VEC; d < D; d += 32 * VEC) {
-                        copy_async<4 * VEC>(to + r * PITCH + d, reinterpret_cast<const float *>(p.k) + at + d, from >= 0);
-                        copy_async<4 * VEC>(to + (TILE + r) * PITCH + d, reinterpret_cast<const float *>(p.v) + at + d, from >= 0);
-                    }
-                } else {
-                    for (int d = lane; d < D; d += 32) {
-                        to[r * PITCH + d] = from >= 0 ? to_f32<T>(reinterpret_cast<const T *>(p.k)[at + d]) : 0.f;
-                        to[(TILE + r) * PITCH + d] = from >= 0 ? to_f32<T>(reinterpret_cast<const T *>(p.v)[at + d]) : 0.f;
-                    }
-                }
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-        int row = row_of(t0 + warp), next = row_of(t0 + warp + W);
-        if (t0 + warp < t1) issue(row, 0);
         for (int t = t0 + warp, stage = 0; t < t1; t += W, stage ^= 1) {
             const int after = row_of(t + 2 * W);
             if (t + W < t1) {
@@ -100,6 +108,7 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32) paged_attention_plain_ke
             const float *K = ring + stage * 2 * TILE * PITCH, *V = K + TILE * PITCH;
             float x[RB] = {};
             const int half = (D + 7) / 8 * 4;
+#pragma unroll 4
             for (int d = side * half; d < (side + 1) * half; d += 4) {
                 const float4 a = *reinterpret_cast<const float4 *>(K + key * PITCH + d);
 #pragma unroll
@@ -114,24 +123,27 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32) paged_attention_plain_ke
                 x[r] += __shfl_xor_sync(0xffffffffu, x[r], 16);
                 x[r] *= p.scale;
                 if (p.softcap > 0.f) x[r] = p.softcap * tanhf(x[r] / p.softcap);
-                if (r >= rows || row < 0 || !paged_sees(p, sp, (r0 + r) % p.S, j)) x[r] = -INFINITY;
+                if (r >= rows || row < 0 || !paged_sees(p, sp, p.by_S.mod(r0 + r, p.by_S.div(r0 + r)), j)) x[r] = -INFINITY;
                 float top = x[r];
 #pragma unroll
                 for (int s = 8; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
                 const float now = fmaxf(m[r], top), ref = merge_reference(now), keep = expf(m[r] - ref), w = expf(x[r] - ref);
                 m[r] = now;
                 l[r] = l[r] * keep + (side ? 0.f : w);
-                if (!side) weights[key * RB + r] = w;
+                if (!side) weights[key * WR + r] = w;
 #pragma unroll
                 for (int i = 0; i < DL; i++) o[r][i] *= keep;
             }
             __syncwarp();
             const bool full = p.S == 1 || paged_tile_full(p, sp, sp.at(t) * TILE, TILE);
-#pragma unroll 2
+#pragma unroll(RB > 4 ? 2 : 8)
             for (int k = 0; k < TILE; k++) {
-                float w[RB];
+                float w[WR];
 #pragma unroll
-                for (int r = 0; r < RB; r += 4) *reinterpret_cast<float4 *>(w + r) = *reinterpret_cast<const float4 *>(weights + k * RB + r);
+                for (int r = 0; r < WR; r += 4) {
+                    const float4 u = *reinterpret_cast<const float4 *>(weights + k * WR + r);
+                    w[r] = u.x, w[r + 1] = u.y, w[r + 2] = u.z, w[r + 3] = u.w;
+                }
 #pragma unroll
                 for (int i = 0; i < DL; i++) {
                     const float v = V[k * PITCH + lane + 32 * i];
@@ -144,21 +156,19 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32) paged_attention_plain_ke
             row = next;
             next = after;
         }
-        // the warps' parts meet in their (idle) stages
-        __syncwarp();
+        // the warps' parts meet
 #pragma unroll
         for (int r = 0; r < RB; r++) {
             l[r] = warp_sum(l[r]);
             if (lane == 0) part_m[warp][r] = m[r], part_l[warp][r] = l[r];
 #pragma unroll
-            for (int i = 0; i < DL; i++)
-                if (lane + 32 * i < D) ring[r * D + lane + 32 * i] = o[r][i];
+            for (int i = 0; i < DL; i++) sums[warp * Shape::SUMS + r * DL * 32 + lane + 32 * i] = o[r][i];
         }
         __syncthreads();
         const bool whole = t0 == 0 && t1 == sp.tiles;
-        float *part = p.ws + (((size_t)blockIdx.y * ctas + cta) * 2 + (run.first ? 0 : 1)) * RB * (D + 2);
+        float *part = p.ws + (((size_t)blockIdx.y * ctas + cta) * 2 + (run.first ? 0 : 1)) * p.part_floats;
         for (int i = threadIdx.x; i < rows * D; i += W * 32) {
-            const int r = i / D;
+            const int r = i / D, d = i - r * D;
             float top = -INFINITY, L = 0.f, O = 0.f;
 #pragma unroll
             for (int w = 0; w < W; w++) top = fmaxf(top, part_m[w][r]);
@@ -167,18 +177,15 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32) paged_attention_plain_ke
             for (int w = 0; w < W; w++) {
                 const float f = expf(part_m[w][r] - ref);
                 L += part_l[w][r] * f;
-                O += sm[RB * PITCH + w * (2 * 2 * TILE * PITCH) + i] * f;
+                O += sums[w * Shape::SUMS + r * DL * 32 + d] * f;
             }
             if (whole) {
-                reinterpret_cast<T *>(p.out)[place(b, h, r0 + r, i - r * D)] = from_f32<T>(paged_quotient(O, L));
+                reinterpret_cast<T *>(p.out)[place(b, h, r0 + r, d)] = from_f32<T>(paged_quotient(O, L));
             } else {
                 part[i] = O;
-                if (i == r * D) part[RB * D + r] = top, part[RB * D + RB + r] = L;
+                if (d == 0) part[RB * D + r] = top, part[RB * D + RB + r] = L;
             }
         }
-        __syncthreads();
-        // the stages' columns behind D are zeros again
-        for (int i = lane; i < 2 * 2 * TILE * PITCH; i += 32) ring[i] = 0.f;
     }
     if (blockIdx.y == 0 && threadIdx.x == 0 && !p.whole) p.records[cta] = run.record;
 }
@@ -575,7 +582,7 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
         }
         done_b = b, done_h = h;
         whole = t0 == 0 && t1 == sp.tiles;
-        part = p.ws + (((size_t)blockIdx.y * ctas + cta) * 2 + (run.first ? 0 : 1)) * Shape::ROWS * (D + 2);
+        part = p.ws + (((size_t)blockIdx.y * ctas + cta) * 2 + (run.first ? 0 : 1)) * p.part_floats;
         run.advance(p);
     }
     if (blockIdx.y == 0 && threadIdx.x == 0 && !p.whole) p.records[cta] = run.record;
@@ -597,8 +604,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attention_join_kernel(c
     const int c0 = blockIdx.x, n = rec.z - c0 + 1, R = p.block_rows, D = p.D;
     const int r = blockIdx.y * rows + warp / per, block = r / R, i0 = r - block * R;
     const bool in = r < p.group * p.S;
-    const float *parts = p.ws + (size_t)block * ctas * 2 * R * (D + 2);
-    auto part = [&](int c) { return parts + ((size_t)(c0 + c) * 2 + (c == 0 ? rec.w : 0)) * R * (D + 2); };
+    const float *parts = p.ws + (size_t)block * ctas * 2 * p.part_floats;
+    auto part = [&](int c) { return parts + ((size_t)(c0 + c) * 2 + (c == 0 ? rec.w : 0)) * p.part_floats; };
     float top = -INFINITY, L = 0.f, O[ITEMS][V] = {};
     if (in) {
         for (int c = lane; c < n; c += 32) top = fmaxf(top, part(c)[R * D + i0]);
@@ -674,7 +681,8 @@ struct PagedPlan {
     int dim, team;  // padded head dimension, warps of a team
     int ctas, block_rows, row_blocks, round;
     bool whole;
-    size_t bytes(int D) const { return whole ? 16 : (size_t)ctas * sizeof(int4) + (size_t)ctas * row_blocks * 2 * block_rows * (D + 2) * sizeof(float); }
+    size_t bytes(int D) const { return whole ? 16 : (size_t)ctas * sizeof(int4) + (size_t)ctas * row_blocks * 2 * part_floats(D) * sizeof(float); }
+    int part_floats(int D) const { return (block_rows * (D + 2) + 3) / 4 * 4; }  // 16-byte pieces of them are read
 };
 
 // Positions of a block table up to which pairs are not cut.
@@ -694,17 +702,23 @@ static int paged_sms(int *sms) {
     return MYNN_OK;
 }
 
-static PagedPlan paged_plan(int B, int S, int Hq, int Hkv, int D, int page, int width, int sms, bool mma) {
+static int plain_rows(int R, int dtype) { return dtype != MYNN_F32 ? (R == 1 ? 1 : 8) : R == 1 ? 1 : R == 2 ? 2 : R <= 4 ? 4 : 8; }
+template <int DL>
+static int plain_ctas(int rows) {
+    return rows == 1 ? PlainShape<DL, 1>::CTAS : rows == 2 ? PlainShape<DL, 2>::CTAS : rows == 4 ? PlainShape<DL, 4>::CTAS : PlainShape<DL, 8>::CTAS;
+}
+
+static PagedPlan paged_plan(int B, int S, int Hq, int Hkv, int D, int page, int width, int sms, bool mma, int dtype) {
     PagedPlan n;
     const int R = Hq / Hkv * S;
     n.mma = mma;
     n.dim = D <= 64 ? 64 : D <= 128 ? 128 : D <= 192 ? 192 : 256;
     n.team = R <= 8 ? 1 : R <= 16 ? 2 : R <= 32 ? 4 : 8;
-    n.block_rows = mma ? 8 * n.team : kPlainRows;
+    n.block_rows = mma ? 8 * n.team : plain_rows(R, dtype);
     n.row_blocks = (R + n.block_rows - 1) / n.block_rows;
     n.round = mma ? 8 / n.team : D <= 128 ? 4 : kPlainWarps<8>;
     n.tile = mma ? paged_mma_tile(n.dim, n.team) : kPagedTile;
-    const long long tiles = ((long long)width * page + n.tile - 1) / n.tile, most = mma && n.dim <= 128 ? 2 * sms : sms;
+    const long long tiles = ((long long)width * page + n.tile - 1) / n.tile, most = sms * (mma ? (n.dim <= 128 ? 2 : 1) : D <= 32 ? plain_ctas<1>(n.block_rows) : D <= 64 ? plain_ctas<2>(n.block_rows) : D <= 96 ? plain_ctas<3>(n.block_rows) : D <= 128 ? plain_ctas<4>(n.block_rows) : plain_ctas<8>(n.block_rows));
     n.whole = (long long)width * page <= kPagedWhole;
     n.ctas = n.whole ? B * Hkv : (int)std::min<long long>(most, std::max<long long>(1, (tiles * Hkv * B + n.round - 1) / n.round));
     return n;
@@ -737,18 +751,22 @@ static int launch_mma_any(cudaStream_t st, const PagedAttention &p, const PagedP
     }
 }
 
+template <typename T, int DL, int RB, int VEC>
+static int launch_plain(cudaStream_t st, const PagedAttention &p, int ctas) {
+    static SmemLimit limit;
+    MYNN_CUDA_OK(limit.raise((const void *)paged_attention_plain_kernel<T, DL, RB, VEC>, PlainShape<DL, RB>::SMEM));
+    MYNN_CUDA_OK(launch_dependent(paged_attention_plain_kernel<T, DL, RB, VEC>, dim3(ctas, p.row_blocks), dim3(kPlainWarps<DL> * 32), PlainShape<DL, RB>::SMEM, st, p));
+    MYNN_LAUNCH_OK("paged_attention_plain_kernel");
+    return MYNN_OK;
+}
 template <typename T, int DL>
-static int launch_plain(cudaStream_t st, const PagedAttention &p, int ctas, int vec) {
-    const dim3 grid(ctas, p.row_blocks), block(kPlainWarps<DL> * 32);
-    static SmemLimit limits[2];
-    auto go = [&](auto kern) -> int {
-        MYNN_CUDA_OK(limits[vec == 4].raise((const void *)kern, plain_smem<DL>()));
-        MYNN_CUDA_OK(launch_dependent(kern, grid, block, plain_smem<DL>(), st, p));
-        MYNN_LAUNCH_OK("paged_attention_plain_kernel");
-        return MYNN_OK;
-    };
-    if constexpr (std::is_same<T, float>::value) return vec == 4 ? go(paged_attention_plain_kernel<T, DL, 4>) : go(paged_attention_plain_kernel<T, DL, 1>);
-    else return go(paged_attention_plain_kernel<T, DL, 0>);
+static int launch_plain_rows(cudaStream_t st, const PagedAttention &p, int ctas, int vec) {
+    if constexpr (!std::is_same<T, float>::value) {
+        return p.block_rows == 1 ? launch_plain<T, DL, 1, 0>(st, p, ctas) : launch_plain<T, DL, 8, 0>(st, p, ctas);
+    } else {
+        if (vec == 1) return p.block_rows == 1 ? launch_plain<T, DL, 1, 1>(st, p, ctas) : p.block_rows == 2 ? launch_plain<T, DL, 2, 1>(st, p, ctas) : p.block_rows == 4 ? launch_plain<T, DL, 4, 1>(st, p, ctas) : launch_plain<T, DL, 8, 1>(st, p, ctas);
+        return p.block_rows == 1 ? launch_plain<T, DL, 1, 4>(st, p, ctas) : p.block_rows == 2 ? launch_plain<T, DL, 2, 4>(st, p, ctas) : p.block_rows == 4 ? launch_plain<T, DL, 4, 4>(st, p, ctas) : launch_plain<T, DL, 8, 4>(st, p, ctas);
+    }
 }
 
 }  // namespace mynn
@@ -768,7 +786,10 @@ static int paged_check(int B, int S, int Hq, int Hkv, int D, int page, int width
 extern "C" size_t mynn_b200_paged_attention_workspace_bytes(int B, int S, int Hq, int Hkv, int D, int page, int table_pages) {
     int sms = 0;
     if (paged_check(B, S, Hq, Hkv, D, page, table_pages) != MYNN_OK || B == 0 || paged_sms(&sms) != MYNN_OK) return 0;
-    return std::max(paged_plan(B, S, Hq, Hkv, D, page, table_pages, sms, true).bytes(D), paged_plan(B, S, Hq, Hkv, D, page, table_pages, sms, false).bytes(D));
+    size_t most = 0;  // of the kernels that the tensors' type and alignment may ask for
+    for (const int dtype : {(int)MYNN_F32, (int)MYNN_BF16})
+        for (const bool mma : {false, true}) most = std::max(most, paged_plan(B, S, Hq, Hkv, D, page, table_pages, sms, mma, dtype).bytes(D));
+    return most;
 }
 
 extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q, const void *k_pages, const void *v_pages, const int32_t *block_table,
@@ -783,10 +804,11 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
     int sms = 0;
     if (const int e = paged_sms(&sms)) return e;
     const bool mma = dtype != MYNN_F32 && D % 8 == 0 && ((uintptr_t)out | (uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0;
-    const PagedPlan n = paged_plan(B, S, Hq, Hkv, D, page, table_pages, sms, mma);
+    const PagedPlan n = paged_plan(B, S, Hq, Hkv, D, page, table_pages, sms, mma, dtype);
     const size_t need = n.bytes(D);
     if (!workspace || workspace_bytes < need) return fail(MYNN_E_ARG, "paged_attention: workspace of %zu bytes, %zu are needed", workspace_bytes, need);
     if ((uintptr_t)workspace % 16) return fail(MYNN_E_ARG, "paged_attention: the workspace is not aligned to 16 bytes");
+    const int vec = D % 4 == 0 && ((uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0 ? 4 : 1;
     PagedAttention p;
     p.out = out, p.q = q;
     p.k = pages ? k_pages : q, p.v = pages ? v_pages : q;  // (a copy of nothing has an address too)
@@ -794,8 +816,8 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
     p.scale = scale, p.softcap = softcap, p.window = std::min(window, kPagedWindow), p.sinks = sinks;
     p.B = B, p.S = S, p.Hq = Hq, p.G = Hkv, p.group = Hq / Hkv, p.D = D;
     p.page = page, p.pages = pages, p.width = table_pages;
-    p.by_page = FixedDivisor(page), p.by_S = FixedDivisor(S);
-    p.row_blocks = n.row_blocks, p.block_rows = n.block_rows, p.round = n.round;
+    p.by_page = FixedDivisor(page), p.by_S = FixedDivisor(S), p.by_pieces = FixedDivisor(dtype == MYNN_F32 ? D / vec : D);
+    p.row_blocks = n.row_blocks, p.block_rows = n.block_rows, p.part_floats = n.part_floats(D), p.round = n.round;
     p.whole = n.whole;
     p.tile = n.tile;
     p.toll = n.mma ? 256 / n.tile : 2 * n.round;
@@ -803,16 +825,15 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
     p.records = reinterpret_cast<int4 *>(workspace);
     p.ws = reinterpret_cast<float *>(p.records + (n.whole ? 0 : n.ctas));
     const cudaStream_t st = (cudaStream_t)stream;
-    const int vec = D % 4 == 0 && ((uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0 ? 4 : 1;
     MYNN_DISPATCH_DTYPE(dtype, T, {
         int e = MYNN_OK;
         if (n.mma) {
             if constexpr (!std::is_same<T, float>::value) e = launch_mma_any<T>(st, p, n);
-        } else if (D <= 32) e = launch_plain<T, 1>(st, p, n.ctas, vec);
-        else if (D <= 64) e = launch_plain<T, 2>(st, p, n.ctas, vec);
-        else if (D <= 96) e = launch_plain<T, 3>(st, p, n.ctas, vec);
-        else if (D <= 128) e = launch_plain<T, 4>(st, p, n.ctas, vec);
-        else e = launch_plain<T, 8>(st, p, n.ctas, vec);
+        } else if (D <= 32) e = launch_plain_rows<T, 1>(st, p, n.ctas, vec);
+        else if (D <= 64) e = launch_plain_rows<T, 2>(st, p, n.ctas, vec);
+        else if (D <= 96) e = launch_plain_rows<T, 3>(st, p, n.ctas, vec);
+        else if (D <= 128) e = launch_plain_rows<T, 4>(st, p, n.ctas, vec);
+        else e = launch_plain_rows<T, 8>(st, p, n.ctas, vec);
         if (e != MYNN_OK) return e;
         if (n.whole) return MYNN_OK;
         const int R = p.group * S, rows = R == 1 ? 1 : R == 2 ? 2 : R <= 4 ? 4 : 8;

@@ -112,6 +112,14 @@ def test_long_and_short_sequences_in_one_batch(dt, page):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("H,G,D", [(2, 2, 80), (3, 3, 33), (4, 2, 20), (8, 2, 36), (2, 1, 250), (12, 2, 72), (2, 2, 256), (18, 1, 100)])
+def test_parts_of_every_number_of_rows(dt, H, G, D):
+    """Pairs that lie in several CTAs, for one, two, four and more query heads per kv head and heads of odd sizes."""
+    run_attention(D, dt, [3000, 7, 1501, 900], H, G, D, 16)
+    run_attention(D, dt, [2000, 33], H, G, D, 10, S=2)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
 @pytest.mark.parametrize("H,G,D,S", [(8, 2, 64, 2), (32, 8, 128, 5), (7, 1, 128, 3), (4, 4, 80, 8), (16, 2, 64, 8), (32, 1, 64, 5), (4, 2, 33, 4)])
 def test_drafted_tokens(dt, H, G, D, S):
     lengths = [S, 40, 333, 1, 0, 700, 17]
