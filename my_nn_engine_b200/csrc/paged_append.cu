@@ -75,6 +75,15 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const PagedAppend p, 
     const int d0 = split ? 8 * sub : 16 * sub, d1 = split ? d0 + half : d0 + 8;
     const T *src = reinterpret_cast<const T *>(p.proj) + ((size_t)b * p.S + s) * heads * p.D;
     Piece<T> x0, x1;
+    // A place without a token is not read, and only its queries are written.
+    if (p.counts && s >= p.counts[b]) {
+        const uint4 z = make_uint4(0, 0, 0, 0);
+        T *dst = reinterpret_cast<T *>(p.q_out) + ((size_t)b * p.Hq * p.S + s) * p.D;
+        for (int i = 0; i < Piece<T>::N; i++) x0.raw[i] = z;
+        if (in)
+            for (int head = group; head < p.Hq; head += groups) x0.store(dst + (size_t)head * p.S * p.D + d0), x0.store(dst + (size_t)head * p.S * p.D + d1);
+        return;
+    }
     if (in && group < heads) x0.load(src + (size_t)group * p.D + d0), x1.load(src + (size_t)group * p.D + d1);
     const AppendToken k = append_token(p, b, s);
     // angles of the pairs in the two pieces: halves (d0 + i, d1 + i), else (d0 + 2 i, d0 + 2 i + 1) and the same in the second piece

@@ -1,5 +1,6 @@
 // Attention of the new tokens of each sequence over a paged cache (paged.cuh says how the work is dealt out).
 #include <algorithm>
+#include <atomic>
 
 #include "attention_internal.cuh"
 #include "paged.cuh"
@@ -681,7 +682,7 @@ struct PagedPlan {
     int dim, team;  // padded head dimension, warps of a team
     int ctas, block_rows, row_blocks, round;
     bool whole;
-    size_t bytes(int D) const { return whole ? 16 : (size_t)ctas * sizeof(int4) + (size_t)ctas * row_blocks * 2 * part_floats(D) * sizeof(float); }
+    size_t bytes(int D) const { return whole ? 0 : (size_t)ctas * sizeof(int4) + (size_t)ctas * row_blocks * 2 * part_floats(D) * sizeof(float); }
     int part_floats(int D) const { return (block_rows * (D + 2) + 3) / 4 * 4; }  // 16-byte pieces of them are read
 };
 
@@ -696,9 +697,14 @@ static int paged_mma_tile(int dim, int team) { return dim == 64 ? mma_tile<64>(t
 
 
 static int paged_sms(int *sms) {
+    static std::atomic<int> known[64];  // of a device, once asked for
     int dev = 0;
     MYNN_CUDA_OK(cudaGetDevice(&dev));
-    MYNN_CUDA_OK(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+    *sms = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+    if (*sms == 0) {
+        MYNN_CUDA_OK(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+        if (dev < 64) known[dev].store(*sms, std::memory_order_relaxed);
+    }
     return MYNN_OK;
 }
 
@@ -806,7 +812,7 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
     const bool mma = dtype != MYNN_F32 && D % 8 == 0 && ((uintptr_t)out | (uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0;
     const PagedPlan n = paged_plan(B, S, Hq, Hkv, D, page, table_pages, sms, mma, dtype);
     const size_t need = n.bytes(D);
-    if (!workspace || workspace_bytes < need) return fail(MYNN_E_ARG, "paged_attention: workspace of %zu bytes, %zu are needed", workspace_bytes, need);
+    if (need && (!workspace || workspace_bytes < need)) return fail(MYNN_E_ARG, "paged_attention: workspace of %zu bytes, %zu are needed", workspace_bytes, need);
     if ((uintptr_t)workspace % 16) return fail(MYNN_E_ARG, "paged_attention: the workspace is not aligned to 16 bytes");
     const int vec = D % 4 == 0 && ((uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0 ? 4 : 1;
     PagedAttention p;

@@ -608,36 +608,45 @@ def dense_matmul_ex(act, w, act_fn=ffi.ACT_NONE, f32_columns=0, block=0, status=
 
 
 # ---- paged caches and drafted tokens ----------------------------------------------------------------------------------
-def _int32(name, t, shape):
-    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != shape):
-        raise ValueError(f"{name} must be an int32 tensor of shape {shape}, not {t.dtype} {tuple(t.shape)}")
-    return t
-
-
-def _on_device_of(first, *others):
-    """The tensors' device as a context, after a check that it is one device: the operators of this section run on their tensors' device and its
-    current stream, whichever device is current."""
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"tensors on {first.device} and {t.device}")
-    if not first.is_cuda:
+def _pointers(*tensors):
+    """Addresses of contiguous tensors of one CUDA device (None: a tensor that is left out), and that device's number."""
+    device, out = tensors[0].get_device(), []
+    for t in tensors:
+        if t is None:
+            out.append(None)
+            continue
+        if t.get_device() != device:
+            raise ValueError(f"tensors on {tensors[0].device} and {t.device}")
+        if not t.is_contiguous():
+            raise ValueError("mynn_b200 operators need contiguous tensors")
+        out.append(t.data_ptr())
+    if device < 0:
         raise ValueError("mynn_b200 operators need CUDA tensors (there is no CPU path)")
-    return _HERE if _device is not None and first.device.index == _device() else torch.cuda.device(first.device)
+    return device, out
 
 
 _HERE = contextlib.nullcontext()
 
 
+def _on(device):
+    """The operators of this section run on their tensors' device and its current stream, whichever device is current."""
+    return _HERE if _device is not None and device == _device() else torch.cuda.device(device)
+
+
 def _pages(k_pages, v_pages, dtype, block_table, lengths, counts, batch):
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
-        raise ValueError(f"k_pages and v_pages must have one shape [pages, kv heads, page, D], not {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    """[pages, kv heads, rows of a page, D] and the pages in a row of the table."""
+    shape, table = k_pages.shape, block_table.shape
+    if len(shape) != 4 or shape != v_pages.shape:
+        raise ValueError(f"k_pages and v_pages must have one shape [pages, kv heads, page, D], not {tuple(shape)} and {tuple(v_pages.shape)}")
     if k_pages.dtype != dtype or v_pages.dtype != dtype:
         raise TypeError("the pages must have the dtype of the queries")
-    if block_table.dim() != 2:
-        raise ValueError("block_table must be [B, pages of a sequence]")
-    _int32("block_table", block_table, (batch, block_table.shape[1]))
-    _int32("lengths", lengths, (batch,))
-    _int32("counts", counts, (batch,))
+    if len(table) != 2 or table[0] != batch or block_table.dtype != torch.int32:
+        raise ValueError(f"block_table must be an int32 tensor [{batch}, pages of a sequence], not {block_table.dtype} {tuple(table)}")
+    if lengths.dtype != torch.int32 or lengths.shape != (batch,):
+        raise ValueError(f"lengths must be an int32 tensor of shape ({batch},), not {lengths.dtype} {tuple(lengths.shape)}")
+    if counts is not None and (counts.dtype != torch.int32 or counts.shape != (batch,)):
+        raise ValueError(f"counts must be an int32 tensor of shape ({batch},), not {counts.dtype} {tuple(counts.shape)}")
+    return *shape, table[1]
 
 
 def paged_rotary_append(proj, lengths, block_table, k_pages, v_pages, heads, cos=None, sin=None, counts=None, halves=True, qk_norm=False, eps=1e-6):
@@ -647,17 +656,17 @@ def paged_rotary_append(proj, lengths, block_table, k_pages, v_pages, heads, cos
     // page].  A place without a token gets a zero query, a position without a page (an entry outside the cache, such as -1) is not stored.  lengths, counts,
     block_table: int32 CUDA tensors.  cos / sin: f32 [positions, rotated / 2], None: no rotation."""
     B, S, C = proj.shape
-    _pages(k_pages, v_pages, proj.dtype, block_table, lengths, counts, B)
-    n, G, page, D = k_pages.shape
+    n, G, page, D, width = _pages(k_pages, v_pages, proj.dtype, block_table, lengths, counts, B)
     if C != (heads + 2 * G) * D:
         raise ValueError(f"proj has {C} columns, {heads} query and 2 x {G} cached heads of {D} need {(heads + 2 * G) * D}")
-    if (cos is None) != (sin is None) or (cos is not None and (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape)):
+    positions, half = (0, 0) if cos is None else cos.shape
+    if (cos is None) != (sin is None) or (cos is not None and (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape)):
         raise ValueError("cos and sin must be f32 tensors of one shape [positions, rotated / 2], or both None")
-    with _on_device_of(proj, lengths, block_table, k_pages, v_pages, cos, sin, counts):
-        q = torch.empty(B, heads, S, D, dtype=proj.dtype, device=proj.device)
-        ffi.check(ffi.lib().mynn_b200_paged_rotary_append(
-            _stream(), _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(proj), _ptr(cos), _ptr(sin), _ptr(lengths), _ptr(counts), _ptr(block_table), B, S, heads, G, D,
-            0 if cos is None else 2 * cos.shape[1], int(halves), int(qk_norm), eps, page, n, block_table.shape[1], 0 if cos is None else cos.shape[0], _dt(proj)))
+    device, (proj_p, lengths_p, table_p, k_p, v_p, cos_p, sin_p, counts_p) = _pointers(proj, lengths, block_table, k_pages, v_pages, cos, sin, counts)
+    with _on(device):
+        q = torch.empty((B, heads, S, D), dtype=proj.dtype, device=proj.device)
+        ffi.check(ffi.lib().mynn_b200_paged_rotary_append(_stream(), q.data_ptr(), k_p, v_p, proj_p, cos_p, sin_p, lengths_p, counts_p, table_p, B, S, heads, G, D, 2 * half,
+                                                          int(halves), int(qk_norm), eps, page, n, width, positions, _dt(proj)))
     return q
 
 
@@ -672,20 +681,21 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale, counts=Non
     up to its own, and the first ``sinks`` ones of the sequence; pages that hold none of these may have been given back.  softcap: cap on the
     scores (0: none).  A query that sees nothing (an idle sequence, a place without a token) gives zeros."""
     B, Hq, S, D = q.shape
-    _pages(k_pages, v_pages, q.dtype, block_table, lengths, counts, B)
-    n, G, page, width = *k_pages.shape[:3], block_table.shape[1]
-    if k_pages.shape[3] != D:
-        raise ValueError(f"heads of {D} over a cache of heads of {k_pages.shape[3]}")
-    with _on_device_of(q, k_pages, v_pages, block_table, lengths, counts, out):
+    n, G, page, head, width = _pages(k_pages, v_pages, q.dtype, block_table, lengths, counts, B)
+    if head != D:
+        raise ValueError(f"heads of {D} over a cache of heads of {head}")
+    if out is not None and (out.shape != (B, S, Hq, D) or out.dtype != q.dtype):
+        raise ValueError(f"out must be {(B, S, Hq, D)} in the dtype of the queries")
+    device, (q_p, k_p, v_p, table_p, lengths_p, counts_p, out_p) = _pointers(q, k_pages, v_pages, block_table, lengths, counts, out)
+    with _on(device):
         if out is None:
-            out = torch.empty(B, S, Hq, D, dtype=q.dtype, device=q.device)
-        elif out.shape != (B, S, Hq, D) or out.dtype != q.dtype:
-            raise ValueError(f"out must be {(B, S, Hq, D)} in the dtype of the queries")
+            out = torch.empty((B, S, Hq, D), dtype=q.dtype, device=q.device)
+            out_p = out.data_ptr()
         # not kept between calls: two captured graphs, or two streams, never share it
-        size = _paged_ws_bytes(q.device.index, B, S, Hq, G, D, page, width)
-        ws = torch.empty(size, dtype=torch.uint8, device=q.device)
-        ffi.check(ffi.lib().mynn_b200_paged_attention(_stream(), _ptr(out), _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(block_table), _ptr(lengths), _ptr(counts),
-                                                      scale, softcap, window, sinks, B, S, Hq, G, D, page, n, width, _dt(q), _ptr(ws), size))
+        size = _paged_ws_bytes(device, B, S, Hq, G, D, page, width)
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        ffi.check(ffi.lib().mynn_b200_paged_attention(_stream(), out_p, q_p, k_p, v_p, table_p, lengths_p, counts_p, scale, softcap, window, sinks, B, S, Hq, G, D, page, n,
+                                                      width, _dt(q), ws.data_ptr() if size else None, size))
     return out
 
 
@@ -697,15 +707,18 @@ def verify_draft(target, tokens, accept, sample, draft=None, counts=None):
     tokens int32 [B])."""
     B, K1, V = target.shape
     K = K1 - 1
-    _int32("tokens", tokens, (B, K))
-    _int32("counts", counts, (B,))
-    if draft is not None and (draft.dtype != target.dtype or tuple(draft.shape) != (B, K, V)):
+    if tokens.dtype != torch.int32 or tokens.shape != (B, K):
+        raise ValueError(f"tokens must be an int32 tensor of shape {(B, K)}, not {tokens.dtype} {tuple(tokens.shape)}")
+    if counts is not None and (counts.dtype != torch.int32 or counts.shape != (B,)):
+        raise ValueError(f"counts must be an int32 tensor of shape ({B},), not {counts.dtype} {tuple(counts.shape)}")
+    if draft is not None and (draft.dtype != target.dtype or draft.shape != (B, K, V)):
         raise ValueError(f"draft must be {(B, K, V)} in the dtype of target")
-    if accept.dtype != torch.float32 or tuple(accept.shape) != (B, K) or sample.dtype != torch.float32 or tuple(sample.shape) != (B,):
+    if accept.dtype != torch.float32 or accept.shape != (B, K) or sample.dtype != torch.float32 or sample.shape != (B,):
         raise ValueError(f"accept and sample must be f32 tensors of shapes {(B, K)} and {(B,)}")
-    with _on_device_of(target, tokens, accept, sample, draft, counts):
-        out = torch.empty(B, K1, dtype=torch.int32, device=target.device)
-        taken = torch.empty(B, dtype=torch.int32, device=target.device)
-        ffi.check(ffi.lib().mynn_b200_verify_draft(_stream(), _ptr(out), _ptr(taken), _ptr(target), _ptr(draft), _ptr(tokens), _ptr(counts), _ptr(accept),
-                                                   _ptr(sample), B, K, V, _dt(target)))
+    device, (target_p, tokens_p, accept_p, sample_p, draft_p, counts_p) = _pointers(target, tokens, accept, sample, draft, counts)
+    with _on(device):
+        out = torch.empty((B, K1), dtype=torch.int32, device=target.device)
+        taken = torch.empty((B,), dtype=torch.int32, device=target.device)
+        ffi.check(ffi.lib().mynn_b200_verify_draft(_stream(), out.data_ptr(), taken.data_ptr(), target_p, draft_p, tokens_p, counts_p, accept_p, sample_p, B, K, V,
+                                                   _dt(target)))
     return out, taken
