@@ -46,7 +46,7 @@ struct PagedAttention {
     float *ws;                   // [row block][CTA][2] parts of part_floats floats: block_rows rows of D, then maxima, then sums
     int part_floats;             // a multiple of 4
     int whole;                   // each pair is left to a CTA of its own
-    int strips;                  // tiles of 16 lie in one page each, and rows are as long on the chip as in the cache
+    int strips;                  // eight positions lie in one page, and rows are as long on the chip as in the cache
 };
 
 // What the new queries of a sequence see: the tiles of the first tokens, then those from the oldest query's window on.

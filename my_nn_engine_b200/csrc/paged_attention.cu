@@ -244,8 +244,10 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
     __shared__ float part_m[W][8], part_l[W][8];
     pdl_trigger();
     pdl_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, team = warp / RW, member = warp % RW;
-    const int cta = blockIdx.x, ctas = gridDim.x, D = p.D, R = p.group * p.S, r0 = blockIdx.y * Shape::ROWS + member * 8;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, team = warp / RW;
+    const int cta = blockIdx.x, ctas = gridDim.x, D = p.D, R = p.group * p.S;
+    // A warp's number says which of the SM's four schedulers it is on: the members that have fewer rows are spread over them.
+    const int member = warp % RW, mine_at = team * RW + member, r0 = blockIdx.y * Shape::ROWS + member * 8;
     uint8_t *ring = raw + (size_t)team * STAGES * Shape::ENTRY;
     float *sums = reinterpret_cast<float *>(raw + Shape::RING);
     const uint32_t ring_at = smem_u32(ring);
@@ -254,6 +256,7 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
     // begin on 128 bytes, so that another piece or row is an exclusive or away.
     constexpr int COPIES = (TILE * CPR + 32 * RW - 1) / (32 * RW), STEP = 32 * RW / CPR;
     constexpr bool EVEN = 32 * RW % CPR == 0;
+    constexpr int STRIPS = TILE / 8;
     constexpr uint32_t ALL = 0xffffffffu >> (32 - TILE);
     const char *k_rows = reinterpret_cast<const char *>(p.k) + (member * 32 + lane) * 16, *v_rows = reinterpret_cast<const char *>(p.v) + (member * 32 + lane) * 16;
     const int copy_row = (member * 32 + lane) / CPR, copy_piece = (member * 32 + lane) % CPR, k_row = lane & 15, v_row = (lane & 7) + (lane >> 4) * 8;
@@ -288,33 +291,29 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
         const int at[2] = {last_seen(2 * t), last_seen(2 * t + 1)};  // this lane's two rows
         auto sees = [&](int last, int j) { return j <= last && (p.window <= 0 || last - j < p.window || j < p.sinks); };
         auto base_of = [&](int j) { return sp.at(t0 + team + TEAMS * j) * TILE; };
-        // The first row of a sixteenth position and the fifteen behind it where these lie one behind the other and are all seen, for 32 of them at once, one
-        // per lane; -1 for others.
+        // The first row of eight positions whose rows lie one behind the other and are all seen, for 32 such strips at once, one per lane; -1 for others.
         auto strips_of = [&](int i) {
-            const int j = i / KT, pos = base_of(j) + i % KT * 16;
-            if (j >= mine || !p.strips || pos + 16 > sp.rows || (p.window > 0 && oldest - pos >= p.window && pos + 16 > p.sinks)) return -1;
+            const int j = i / STRIPS, pos = base_of(j) + i % STRIPS * 8;
+            if (j >= mine || !p.strips || pos + 8 > sp.rows || (p.window > 0 && oldest - pos >= p.window && pos + 8 > p.sinks)) return -1;
             return paged_row(p, sp, b, h, pos);
         };
         auto row_of = [&](int j) { return j < mine ? paged_row(p, sp, b, h, base_of(j) + (lane & (TILE - 1))) : -1; };
         // The keys or the values of a tile to an entry of the ring, from strips (uniform) where there are any, else row by row (row: of position lane % TILE).
-        auto issue = [&](const char *rows, uint32_t entry, bool in_run, bool fast, const int (&strip)[KT], int row, uint32_t there) {
-            if (in_run) {
+        auto issue = [&](const char *rows, uint32_t entry, int j, bool fast, int strips, int row, uint32_t there) {
+            if (j < mine) {
                 const uint32_t to = ring_at + entry + copy_lane;
                 if (fast) {
-                    const char *src[KT];
-#pragma unroll
-                    for (int k = 0; k < KT; k++) src[k] = rows + (size_t)(uint32_t)strip[k] * (DP * 2);
+                    const char *src = rows;
 #pragma unroll
                     for (int i = 0; i < COPIES; i++) {
-                        if constexpr (EVEN) {  // the lane's row moves on by STEP rows, its piece stays
-                            const char *from = KT == 1 || i < COPIES / 2 ? src[0] + i * RW * 512 : src[KT - 1] + (i - COPIES / 2) * RW * 512;
-                            if (KT == 2 && COPIES == 1) from = member * 32 < 16 * CPR ? src[0] : src[1] - 16 * DP * 2;
-                            copy16_now((to ^ (STEP * i & 7) << 4) + STEP * i * DP * 2, from);
+                        if constexpr (EVEN && STEP <= 8) {  // the lane's row moves on by STEP rows, its piece stays
+                            if (STEP * i % 8 == 0) src = rows + (size_t)(uint32_t)__shfl_sync(0xffffffffu, strips, (j * STRIPS + STEP * i / 8) & 31) * (DP * 2);
+                            copy16_now((to ^ (STEP * i & 7) << 4) + STEP * i * DP * 2, src + STEP * i % 8 * (DP * 2));
                         } else {
                             const int idx = (i * RW + member) * 32 + lane, r = idx / CPR, c = idx % CPR;
-                            if (TILE * CPR % (32 * RW) != 0 && idx >= TILE * CPR) break;
-                            const char *from = KT == 1 || r < 16 ? src[0] + i * RW * 512 : src[KT - 1] + i * RW * 512 - 16 * DP * 2;
-                            copy16_now(ring_at + entry + r * (DP * 2) + (c >> 3) * 128 + paged_swizzle(r, c & 7) * 16, from);
+                            if (TILE * CPR % (32 * RW) != 0 && idx >= TILE * CPR) break;  // (a whole warp)
+                            const int from = __shfl_sync(0xffffffffu, strips, (j * STRIPS + (r >> 3)) & 31) + (r & 7);
+                            copy16_now(ring_at + entry + r * (DP * 2) + (c >> 3) * 128 + paged_swizzle(r, c & 7) * 16, rows + (size_t)(uint32_t)from * (DP * 2) + c * 16 - (member * 32 + lane) * 16);
                         }
                     }
                 } else {
@@ -332,17 +331,16 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
         // What issue() needs for tile j, and which rows of it there are.
-        int strips = -1, strips_next = -1, strip[KT], row = -1;
+        int strips = -1, strips_next = -1, row = -1;
+        uint32_t strips_there = 0;
         uint32_t there = 0;
         bool fast = false;
         auto look_up = [&](int j) {
-            if (j > 0 && (j * KT & 31) == 0) strips = strips_next, strips_next = strips_of(j * KT + 32 + lane);
-            fast = true;
-#pragma unroll
-            for (int k = 0; k < KT; k++) {
-                strip[k] = __shfl_sync(0xffffffffu, strips, (j * KT + k) & 31);
-                fast &= strip[k] >= 0;
+            if ((j * STRIPS & 31) == 0) {
+                strips = strips_next, strips_next = strips_of(j * STRIPS + 32 + lane);
+                strips_there = __ballot_sync(0xffffffffu, strips >= 0);
             }
+            fast = (strips_there >> (j * STRIPS & 31) & ((1u << STRIPS) - 1)) == (1u << STRIPS) - 1;
             there = ALL;
             if (!fast) {
                 row = row_of(j);
@@ -354,13 +352,13 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
         uint32_t qb[KS][2];  // row g, dimensions 16 i + 2 t and + 8
         if (more) {
             team_sync();  // the ring is free
-            strips = strips_of(lane), strips_next = strips_of(lane + 32);
+            strips_next = strips_of(lane);
 #pragma unroll
             for (int j = 0; j < AHEAD; j++) {
                 look_up(j);
                 exist[j] = there;
-                issue(k_rows, 2 * j * Shape::ENTRY, j < mine, fast, strip, row, there);
-                issue(v_rows, (2 * j + 1) * Shape::ENTRY, j < mine, fast, strip, row, there);
+                issue(k_rows, 2 * j * Shape::ENTRY, j, fast, strips, row, there);
+                issue(v_rows, (2 * j + 1) * Shape::ENTRY, j, fast, strips, row, there);
             }
             look_up(AHEAD);
             const int r = min(r0 + g, R - 1), head = p.by_S.div(r), s = p.by_S.mod(r, head);
@@ -380,7 +378,7 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             __syncthreads();  // nobody reads what the pair in front left any more
             if (g == 0) {
 #pragma unroll
-                for (int e = 0; e < 2; e++) part_m[warp][2 * t + e] = m[e], part_l[warp][2 * t + e] = l[e];
+                for (int e = 0; e < 2; e++) part_m[mine_at][2 * t + e] = m[e], part_l[mine_at][2 * t + e] = l[e];
             }
             __syncthreads();
             float f[2];
@@ -398,7 +396,7 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
                 for (int i = 0; i < 4; i++)
 #pragma unroll
                     for (int k = 0; k < 4; k++)  // (dimensions 8 apart for neighbouring t: all banks)
-                        sums[(warp * 8 + 2 * t + (k & 1)) * 64 + ((16 * i + 8 * (k >> 1) + g) ^ (t * 8))] = o[4 * s + i][k] * f[k & 1];
+                        sums[(mine_at * 8 + 2 * t + (k & 1)) * 64 + ((16 * i + 8 * (k >> 1) + g) ^ (t * 8))] = o[4 * s + i][k] * f[k & 1];
                 __syncthreads();
                 for (int i = threadIdx.x; i < rows * 32; i += W * 32) {
                     const int r = i >> 5, d = 2 * (i & 31), w0 = r >> 3, at = ((w0 * 8 + (r & 7)) * 64) + (d ^ ((r >> 1 & 3) * 8));
@@ -443,7 +441,7 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             team_sync();  // the keys of tile j are here, and the values of tile j - 1 are done with
             const int ahead = j + AHEAD;
             exist[AHEAD] = there;
-            issue(k_rows, free_entry, ahead < mine, fast, strip, row, there);
+            issue(k_rows, free_entry, ahead, fast, strips, row, there);
             const int base = base_of(j);
             const uint32_t K = k_lane + cur;
             free_entry = cur;
@@ -522,7 +520,7 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             }
             asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
             team_sync();  // the values of tile j are here, and its keys are done with
-            issue(v_rows, free_entry, ahead < mine, fast, strip, row, there);
+            issue(v_rows, free_entry, ahead, fast, strips, row, there);
             look_up(ahead + 1);
             const uint32_t V = v_lane + cur;
             free_entry = cur;
@@ -827,7 +825,7 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
     p.whole = n.whole;
     p.tile = n.tile;
     p.toll = n.mma ? 256 / n.tile : 2 * n.round;
-    p.strips = n.mma && page % 16 == 0 && D == n.dim;
+    p.strips = n.mma && page % 8 == 0 && D == n.dim;
     p.records = reinterpret_cast<int4 *>(workspace);
     p.ws = reinterpret_cast<float *>(p.records + (n.whole ? 0 : n.ctas));
     const cudaStream_t st = (cudaStream_t)stream;
