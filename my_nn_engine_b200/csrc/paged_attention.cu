@@ -208,7 +208,10 @@ struct MmaShape {
     static constexpr int CTAS = DP > 128 ? 1 : 2;  // per SM
     static constexpr int SPACE = (CTAS == 2 ? 96 : 192) * 1024 / TEAMS;
     static constexpr int TILE = SPACE / (32 * DP * 2) >= 3 ? 32 : 16, ENTRY = TILE * DP * 2;
-    static constexpr int FIT = (SPACE / ENTRY - 1) / 2, AHEAD = FIT < 3 ? FIT : 3, STAGES = 2 * AHEAD + 1;  // tiles on their way while one is worked on
+    // Large teams have room for the keys and values of a tile together, and meet once per tile instead of twice.
+    static constexpr bool JOINT = RW >= 4;
+    static constexpr int FIT = JOINT ? SPACE / ENTRY / 2 - 1 : (SPACE / ENTRY - 1) / 2, AHEAD = FIT < 3 ? FIT : 3;  // tiles on their way while one is worked on
+    static constexpr int STAGES = 2 * AHEAD + (JOINT ? 2 : 1), WAIT = JOINT ? 2 * AHEAD - 2 : STAGES - 2;             // groups of copies that may still be on their way
     static constexpr size_t RING = (size_t)TEAMS * STAGES * ENTRY;
     static constexpr size_t SMEM = RING + W * 8 * 64 * sizeof(float);  // and 64 dimensions of all warps' sums
 };
@@ -238,6 +241,7 @@ __device__ __forceinline__ uint32_t special_mask(uint32_t x) {  // all ones over
 template <typename T, int DP, int RW>
 __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_mma_kernel(const PagedAttention p) {
     using Shape = MmaShape<DP, RW>;
+    constexpr bool JOINT = Shape::JOINT;
     constexpr int W = Shape::W, TEAMS = Shape::TEAMS, STAGES = Shape::STAGES, AHEAD = Shape::AHEAD, TILE = Shape::TILE, KT = TILE / 16, KS = DP / 16, CPR = DP / 8;
     constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
     extern __shared__ __align__(128) uint8_t raw[];
@@ -428,7 +432,12 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             }
         }
         if (!more) break;
-        uint32_t cur = 0, free_entry = (STAGES - 1) * Shape::ENTRY;  // offsets: the entry that is read next, the one that is empty
+        // offsets: the entry that is read next, the one that is empty (JOINT: the first of two)
+        uint32_t cur = 0, free_entry = (STAGES - (JOINT ? 2 : 1)) * Shape::ENTRY;
+        auto step_on = [&]() {
+            free_entry = JOINT ? cur - Shape::ENTRY : cur;  // (JOINT: called behind the values)
+            cur = cur + Shape::ENTRY == STAGES * Shape::ENTRY ? 0 : cur + Shape::ENTRY;
+        };
 #pragma unroll
         for (int e = 0; e < 2; e++) m[e] = limit[e] = -INFINITY, ref[e] = l[e] = 0.f;
 #pragma unroll
@@ -437,15 +446,19 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             for (int e = 0; e < 4; e++) o[i][e] = 0.f;
 #pragma unroll 1
         for (int j = 0; j < mine; j++) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-            team_sync();  // the keys of tile j are here, and the values of tile j - 1 are done with
+            asm volatile("cp.async.wait_group %0;" ::"n"(Shape::WAIT) : "memory");
+            team_sync();  // the keys of tile j are here (JOINT: its values too), and the values of tile j - 1 are done with
             const int ahead = j + AHEAD;
             exist[AHEAD] = there;
             issue(k_rows, free_entry, ahead, fast, strips, row, there);
+            if constexpr (JOINT) {
+                issue(v_rows, free_entry + Shape::ENTRY, ahead, fast, strips, row, there);
+                look_up(ahead + 1);
+            }
             const int base = base_of(j);
             const uint32_t K = k_lane + cur;
-            free_entry = cur;
-            cur = cur + Shape::ENTRY == STAGES * Shape::ENTRY ? 0 : cur + Shape::ENTRY;
+            if constexpr (JOINT) cur += Shape::ENTRY;
+            else step_on();
             // ---- S^T = K Q^T: x[k][2 c + e] is position base + 16 k + g + 8 c, row 2 t + e ----
             float x[KT][4], y[KT][4];
             uint32_t hi[KT][2], lo[KT][2];
@@ -518,20 +531,21 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
                     }
                 }
             }
-            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-            team_sync();  // the values of tile j are here, and its keys are done with
-            issue(v_rows, free_entry, ahead, fast, strips, row, there);
-            look_up(ahead + 1);
-            const uint32_t V = v_lane + cur;
-            free_entry = cur;
-            cur = cur + Shape::ENTRY == STAGES * Shape::ENTRY ? 0 : cur + Shape::ENTRY;
+            if constexpr (!JOINT) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(Shape::WAIT) : "memory");
+                team_sync();  // the values of tile j are here, and its keys are done with
+                issue(v_rows, free_entry, ahead, fast, strips, row, there);
+                look_up(ahead + 1);
+            }
+            const uint32_t V = v_lane + cur, v_entry = cur;
+            step_on();
             // ---- O^T += V^T P^T: o[i] is dimensions 16 i + g (registers 0, 1) and + 8 (2, 3) of rows 2 t and 2 t + 1 ----
             // Values that are no numbers, in a tile that not every row sees all of?
             bool odd = false;
             if (!full && p.S > 1) {
 #pragma unroll 1
                 for (int i = lane; i < TILE * CPR; i += 32) {
-                    const uint4 u = *reinterpret_cast<const uint4 *>(ring + free_entry + i * 16);
+                    const uint4 u = *reinterpret_cast<const uint4 *>(ring + v_entry + i * 16);
                     odd |= (special_mask<T>(u.x) | special_mask<T>(u.y) | special_mask<T>(u.z) | special_mask<T>(u.w)) != 0u;
                 }
                 odd = __any_sync(0xffffffffu, odd);
