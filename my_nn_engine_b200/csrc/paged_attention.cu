@@ -192,28 +192,29 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32, PlainShape<DL, RB>::CTAS
 }
 
 // ---- 16-bit caches on the tensor cores --------------------------------------------------------------------------------
-// Bound by the one pass over the cache.  A team of RW warps takes tiles of 16 positions: cp.async brings a tile's rows, wherever their pages lie, to a ring in shared
-// memory whose entries are the keys or the values of a tile, each warp a share of the rows, and each warp then multiplies the whole tile with eight query rows of its
-// own, so that a row of the cache is read once for up to 64 query rows (all heads of a group, all drafts).  Both products are mma.m16n8k16 on fragments that
-// are whole 8 x 8 blocks from ldmatrix, without a byte moved: S^T = K Q^T, eight query rows as columns, and O^T = V^T P^T, whose second operand is the first
-// product's result behind a transposition of its 8 x 8 blocks.  Weights enter as a 16-bit part and its remainder (16 bits in all); scores, maxima and sums are f32.  The
-// reference of the weights is moved only when a score exceeds it by 2^8, so most tiles need no maximum across lanes and no rescaling.  D is padded to DP with
-// zeros, on the chip only.
-// The chain of one tile is long (two products, a softmax) and each warp walks it alone, so warps are what hides it: sixteen per SM, eight query rows each, rather than
-// eight with sixteen rows (96 mixed sequences of heads of 64: eight warps per SM 97 us).
-// A tile is 32 positions where three entries of that size fit, else 16: what goes on around the products takes as long as they do.
-template <int DP, int RW>
+// Bound by the one pass over the cache.  A team of RW warps takes tiles of 16 or 32 positions: cp.async brings a tile's rows, wherever their pages lie, to a ring in
+// shared memory whose entries are the keys or the values of a tile, each warp a share of the rows, and each warp then multiplies the whole tile with query rows of its
+// own, eight or NT times eight, so that a row of the cache is read once for up to 64 query rows (all heads of a group, all drafts).  Both products are mma.m16n8k16 on
+// fragments that are whole 8 x 8 blocks from ldmatrix, without a byte moved: S^T = K Q^T, eight query rows as columns, and O^T = V^T P^T, whose second operand is
+// the first product's result behind a transposition of its 8 x 8 blocks.  Weights enter as a 16-bit part and its remainder (16 bits in all); scores, maxima and
+// sums are f32.  The reference of the weights is moved only when a score exceeds it by 2^8, so most tiles need no maximum across lanes and no rescaling.  D is padded
+// to DP with zeros, on the chip only.
+// The chain of one tile is long (two products, a softmax) and each warp walks it alone, so warps are what hides it: sixteen per SM with eight query rows each (96 mixed
+// sequences of heads of 64: 81 us, eight warps with sixteen rows 97).  From 17 rows on the instructions bound it, and sixteen rows of a warp share the blocks of keys and values and what goes
+// on around the products.
+template <int DP, int RW, int NT>
 struct MmaShape {
-    static constexpr int W = 8, TEAMS = W / RW, ROWS = 8 * RW;
-    static constexpr int CTAS = DP > 128 ? 1 : 2;  // per SM
-    static constexpr int SPACE = (CTAS == 2 ? 96 : 192) * 1024 / TEAMS;
+    static constexpr int W = 8, TEAMS = W / RW, ROWS = 8 * NT * RW;
+    static constexpr int CTAS = DP > 128 || (DP == 128 && NT == 2) ? 1 : 2;  // per SM
+    static constexpr int SPACE = (CTAS == 1 ? 192 : NT == 2 ? 80 : 96) * 1024 / TEAMS;
+    // A tile is 32 positions where three entries of that size fit, else 16: what goes on around the products takes as long as they do.
     static constexpr int TILE = SPACE / (32 * DP * 2) >= 3 ? 32 : 16, ENTRY = TILE * DP * 2;
     // Large teams have room for the keys and values of a tile together, and meet once per tile instead of twice.
-    static constexpr bool JOINT = RW >= 4;
+    static constexpr bool JOINT = RW > 1 && SPACE / ENTRY >= 5;
     static constexpr int FIT = JOINT ? SPACE / ENTRY / 2 - 1 : (SPACE / ENTRY - 1) / 2, AHEAD = FIT < 3 ? FIT : 3;  // tiles on their way while one is worked on
     static constexpr int STAGES = 2 * AHEAD + (JOINT ? 2 : 1), WAIT = JOINT ? 2 * AHEAD - 2 : STAGES - 2;             // groups of copies that may still be on their way
     static constexpr size_t RING = (size_t)TEAMS * STAGES * ENTRY;
-    static constexpr size_t SMEM = RING + W * 8 * 64 * sizeof(float);  // and 64 dimensions of all warps' sums
+    static constexpr size_t SMEM = RING + W * 8 * NT * 64 * sizeof(float);  // and 64 dimensions of all warps' sums
 };
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -238,24 +239,24 @@ __device__ __forceinline__ uint32_t special_mask(uint32_t x) {  // all ones over
     return ((x & e) == e ? 0xffffu : 0u) | ((x >> 16 & e) == e ? 0xffff0000u : 0u);
 }
 
-template <typename T, int DP, int RW>
-__global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_mma_kernel(const PagedAttention p) {
-    using Shape = MmaShape<DP, RW>;
+template <typename T, int DP, int RW, int NT>
+__global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attention_mma_kernel(const PagedAttention p) {
+    using Shape = MmaShape<DP, RW, NT>;
     constexpr bool JOINT = Shape::JOINT;
     constexpr int W = Shape::W, TEAMS = Shape::TEAMS, STAGES = Shape::STAGES, AHEAD = Shape::AHEAD, TILE = Shape::TILE, KT = TILE / 16, KS = DP / 16, CPR = DP / 8;
     constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
     extern __shared__ __align__(128) uint8_t raw[];
-    __shared__ float part_m[W][8], part_l[W][8];
+    __shared__ float part_m[W][8 * NT], part_l[W][8 * NT];
     pdl_trigger();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, team = warp / RW;
     const int cta = blockIdx.x, ctas = gridDim.x, D = p.D, R = p.group * p.S;
-    // A warp's number says which of the SM's four schedulers it is on: the members that have fewer rows are spread over them.
-    const int member = warp % RW, mine_at = team * RW + member, r0 = blockIdx.y * Shape::ROWS + member * 8;
+    // A warp's number says which of the SM's four schedulers it is on; the last members of a team may have fewer rows, and are spread over them.
+    const int member = (warp + team + (RW == 2 ? team >> 1 : 0)) % RW, slot = team * RW + member, r0 = blockIdx.y * Shape::ROWS + member * 8 * NT;
     uint8_t *ring = raw + (size_t)team * STAGES * Shape::ENTRY;
     float *sums = reinterpret_cast<float *>(raw + Shape::RING);
     const uint32_t ring_at = smem_u32(ring);
-    const bool busy = r0 < R;  // a warp without rows of its own only helps to copy
+    const bool busy = r0 < R, more_rows = NT > 1 && r0 + 8 < R;  // a warp without rows of its own only helps to copy
     // this lane's places: of its first copy in the cache and in an entry, of the first piece of a row of keys (row lane % 16) and, transposed, of values.  Entries
     // begin on 128 bytes, so that another piece or row is an exclusive or away.
     constexpr int COPIES = (TILE * CPR + 32 * RW - 1) / (32 * RW), STEP = 32 * RW / CPR;
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
     int done_b = -1, done_h = 0;
     bool whole = false;
     float *part = nullptr;
-    float o[KS][4], m[2], l[2], ref[2], limit[2];  // ref, limit: what weights are relative to, and the score that moves it
+    float o[NT][KS][4], m[NT][2], l[NT][2], ref[NT][2], limit[NT][2];  // ref, limit: what weights are relative to, and the score that moves it
     for (;;) {
         const bool more = run.more(p, sp);
         const int b = run.b, h = run.h, t0 = run.t0, t1 = run.t1;
@@ -292,7 +293,9 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             const int r = r0 + i, s = p.by_S.mod(r, p.by_S.div(r));
             return r < R && s < sp.count ? oldest + s : -1;
         };
-        const int at[2] = {last_seen(2 * t), last_seen(2 * t + 1)};  // this lane's two rows
+        int at[NT][2];  // of this lane's rows 8 n + 2 t and + 1
+#pragma unroll
+        for (int n = 0; n < NT; n++) at[n][0] = last_seen(8 * n + 2 * t), at[n][1] = last_seen(8 * n + 2 * t + 1);
         auto sees = [&](int last, int j) { return j <= last && (p.window <= 0 || last - j < p.window || j < p.sinks); };
         auto base_of = [&](int j) { return sp.at(t0 + team + TEAMS * j) * TILE; };
         // The first row of eight positions whose rows lie one behind the other and are all seen, for 32 such strips at once, one per lane; -1 for others.
@@ -353,7 +356,7 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             }
         };
         uint32_t exist[AHEAD + 1];  // which rows of the next tiles there are
-        uint32_t qb[KS][2];  // row g, dimensions 16 i + 2 t and + 8
+        uint32_t qb[NT][KS][2];  // row 8 n + g, dimensions 16 i + 2 t and + 8
         if (more) {
             team_sync();  // the ring is free
             strips_next = strips_of(lane);
@@ -365,16 +368,19 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
                 issue(v_rows, (2 * j + 1) * Shape::ENTRY, j, fast, strips, row, there);
             }
             look_up(AHEAD);
-            const int r = min(r0 + g, R - 1), head = p.by_S.div(r), s = p.by_S.mod(r, head);
-            const bool in = r0 + g < R && s < sp.count;
-            const T *qr = reinterpret_cast<const T *>(p.q) + (((size_t)b * p.Hq + h * p.group + head) * p.S + s) * D;
 #pragma unroll
-            for (int i = 0; i < KS; i++)
+            for (int n = 0; n < NT; n++) {
+                const int r = min(r0 + 8 * n + g, R - 1), head = p.by_S.div(r), s = p.by_S.mod(r, head);
+                const bool in = r0 + 8 * n + g < R && s < sp.count;
+                const T *qr = reinterpret_cast<const T *>(p.q) + (((size_t)b * p.Hq + h * p.group + head) * p.S + s) * D;
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int d = 16 * i + 8 * e + 2 * t;
-                    qb[i][e] = in && d < D ? *reinterpret_cast<const uint32_t *>(qr + d) : 0u;
-                }
+                for (int i = 0; i < KS; i++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int d = 16 * i + 8 * e + 2 * t;
+                        qb[n][i][e] = in && d < D ? *reinterpret_cast<const uint32_t *>(qr + d) : 0u;
+                    }
+            }
         }
         // ---- the teams meet, while the first tiles of the next pair are on their way: 64 dimensions of all warps' sums at a time ----
         if (done_b >= 0) {
@@ -382,38 +388,44 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             __syncthreads();  // nobody reads what the pair in front left any more
             if (g == 0) {
 #pragma unroll
-                for (int e = 0; e < 2; e++) part_m[mine_at][2 * t + e] = m[e], part_l[mine_at][2 * t + e] = l[e];
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) part_m[slot][8 * n + 2 * t + e] = m[n][e], part_l[slot][8 * n + 2 * t + e] = l[n][e];
             }
             __syncthreads();
-            float f[2];
+            float f[NT][2];
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                float top = -INFINITY;
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int w = 0; w < TEAMS; w++) top = fmaxf(top, part_m[w * RW + member][2 * t + e]);
-                f[e] = exp2_approx(m[e] - merge_reference(top));
-            }
+                for (int e = 0; e < 2; e++) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < TEAMS; w++) top = fmaxf(top, part_m[w * RW + member][8 * n + 2 * t + e]);
+                    f[n][e] = exp2_approx(m[n][e] - merge_reference(top));
+                }
 #pragma unroll
             for (int s = 0; s < DP / 64; s++) {
                 if (s > 0) __syncthreads();
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+                for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int k = 0; k < 4; k++)  // (dimensions 8 apart for neighbouring t: all banks)
-                        sums[(mine_at * 8 + 2 * t + (k & 1)) * 64 + ((16 * i + 8 * (k >> 1) + g) ^ (t * 8))] = o[4 * s + i][k] * f[k & 1];
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++)  // (dimensions 8 apart for neighbouring t: all banks)
+                            sums[(slot * 8 * NT + 8 * n + 2 * t + (k & 1)) * 64 + ((16 * i + 8 * (k >> 1) + g) ^ (t * 8))] = o[n][4 * s + i][k] * f[n][k & 1];
                 __syncthreads();
                 for (int i = threadIdx.x; i < rows * 32; i += W * 32) {
-                    const int r = i >> 5, d = 2 * (i & 31), w0 = r >> 3, at = ((w0 * 8 + (r & 7)) * 64) + (d ^ ((r >> 1 & 3) * 8));
+                    const int r = i >> 5, d = 2 * (i & 31), w0 = r / (8 * NT), own = r % (8 * NT), at = r * 64 + (d ^ ((r >> 1 & 3) * 8));
                     float2 O = make_float2(0.f, 0.f);
                     float top = -INFINITY, L = 0.f;
 #pragma unroll
                     for (int w = 0; w < TEAMS; w++) {
-                        const float2 u = *reinterpret_cast<const float2 *>(sums + at + w * RW * 512);
+                        const float2 u = *reinterpret_cast<const float2 *>(sums + at + w * RW * 512 * NT);
                         O.x += u.x, O.y += u.y;
-                        top = fmaxf(top, part_m[w * RW + w0][r & 7]);
+                        top = fmaxf(top, part_m[w * RW + w0][own]);
                     }
 #pragma unroll
-                    for (int w = 0; w < TEAMS; w++) L += part_l[w * RW + w0][r & 7] * exp2_approx(part_m[w * RW + w0][r & 7] - merge_reference(top));
+                    for (int w = 0; w < TEAMS; w++) L += part_l[w * RW + w0][own] * exp2_approx(part_m[w * RW + w0][own] - merge_reference(top));
                     if (64 * s + d >= D) continue;
                     if (whole) {
                         const int q = blockIdx.y * Shape::ROWS + r, head = p.by_S.div(q);
@@ -439,11 +451,14 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             cur = cur + Shape::ENTRY == STAGES * Shape::ENTRY ? 0 : cur + Shape::ENTRY;
         };
 #pragma unroll
-        for (int e = 0; e < 2; e++) m[e] = limit[e] = -INFINITY, ref[e] = l[e] = 0.f;
+        for (int n = 0; n < NT; n++) {
 #pragma unroll
-        for (int i = 0; i < DP / 16; i++)
+            for (int e = 0; e < 2; e++) m[n][e] = limit[n][e] = -INFINITY, ref[n][e] = l[n][e] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[i][e] = 0.f;
+            for (int i = 0; i < KS; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[n][i][e] = 0.f;
+        }
 #pragma unroll 1
         for (int j = 0; j < mine; j++) {
             asm volatile("cp.async.wait_group %0;" ::"n"(Shape::WAIT) : "memory");
@@ -459,78 +474,87 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             const uint32_t K = k_lane + cur;
             if constexpr (JOINT) cur += Shape::ENTRY;
             else step_on();
-            // ---- S^T = K Q^T: x[k][2 c + e] is position base + 16 k + g + 8 c, row 2 t + e ----
-            float x[KT][4], y[KT][4];
-            uint32_t hi[KT][2], lo[KT][2];
+            // ---- S^T = K Q^T: x[n][k][2 c + e] is position base + 16 k + g + 8 c, row 8 n + 2 t + e ----
+            uint32_t hi[NT][KT][2], lo[NT][KT][2];
             const bool full = exist[0] == ALL && (p.S == 1 || paged_tile_full(p, sp, base, TILE));
-            if (busy) {
+            auto scores = [&](auto groups) {
+                constexpr int N = decltype(groups)::value;
+                float x[N][KT][4], y[N][KT][4];
 #pragma unroll
-                for (int k = 0; k < KT; k++)
+                for (int n = 0; n < N; n++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) x[k][i] = y[k][i] = 0.f;
+                    for (int k = 0; k < KT; k++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) x[n][k][i] = y[n][k][i] = 0.f;
 #pragma unroll
                 for (int i = 0; i < KS; i++)
 #pragma unroll
                     for (int k = 0; k < KT; k++) {
                         uint32_t a[4];
                         ldsm4_at(a, (K ^ (i & 3) << 5) + (i >> 2) * 128 + k * 16 * DP * 2);
-                        mma_kv<T>(KT == 1 && (i & 1) ? y[k] : x[k], a[0], a[1], a[2], a[3], qb[i][0], qb[i][1]);
+#pragma unroll
+                        for (int n = 0; n < N; n++) mma_kv<T>(KT == 1 && N == 1 && (i & 1) ? y[n][k] : x[n][k], a[0], a[1], a[2], a[3], qb[n][i][0], qb[n][i][1]);
                     }
-                float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int k = 0; k < KT; k++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        if (KT == 1) x[k][i] += y[k][i];
-                        x[k][i] *= unit;
-                    }
-                if (p.softcap > 0.f) {
-#pragma unroll
-                    for (int k = 0; k < KT; k++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) x[k][i] = kLog2e * fast_soft_cap(x[k][i] * kLn2, p.softcap);
-                }
-                if (!full) {
+                for (int n = 0; n < N; n++) {
+                    float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                     for (int k = 0; k < KT; k++)
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            const int bit = 16 * k + g + 8 * (i >> 1);
-                            if (!((exist[0] >> bit & 1) && sees(at[i & 1], base + bit))) x[k][i] = -INFINITY;
+                            if (KT == 1 && N == 1) x[n][k][i] += y[n][k][i];
+                            x[n][k][i] *= unit;
                         }
-                }
+                    if (p.softcap > 0.f) {
 #pragma unroll
-                for (int k = 0; k < KT; k++)
+                        for (int k = 0; k < KT; k++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) most[i & 1] = fmaxf(most[i & 1], x[k][i]);
-                if (__any_sync(0xffffffffu, most[0] > limit[0] || most[1] > limit[1])) {
+                            for (int i = 0; i < 4; i++) x[n][k][i] = kLog2e * fast_soft_cap(x[n][k][i] * kLn2, p.softcap);
+                    }
+                    if (!full) {
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        float top = most[e];
+                        for (int k = 0; k < KT; k++)
 #pragma unroll
-                        for (int s = 4; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-                        const float now = fmaxf(m[e], top), keep = exp2_approx(m[e] - merge_reference(now));
-                        m[e] = now;
-                        ref[e] = merge_reference(now);
-                        limit[e] = now + 8.f;
-                        l[e] *= keep;
+                            for (int i = 0; i < 4; i++) {
+                                const int bit = 16 * k + g + 8 * (i >> 1);
+                                if (!((exist[0] >> bit & 1) && sees(at[n][i & 1], base + bit))) x[n][k][i] = -INFINITY;
+                            }
+                    }
 #pragma unroll
-                        for (int i = 0; i < KS; i++) o[i][e] *= keep, o[i][2 + e] *= keep;
+                    for (int k = 0; k < KT; k++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) most[i & 1] = fmaxf(most[i & 1], x[n][k][i]);
+                    if (__any_sync(0xffffffffu, most[0] > limit[n][0] || most[1] > limit[n][1])) {
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            float top = most[e];
+#pragma unroll
+                            for (int s = 4; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+                            const float now = fmaxf(m[n][e], top), keep = exp2_approx(m[n][e] - merge_reference(now));
+                            m[n][e] = now;
+                            ref[n][e] = merge_reference(now);
+                            limit[n][e] = now + 8.f;
+                            l[n][e] *= keep;
+#pragma unroll
+                            for (int i = 0; i < KS; i++) o[n][i][e] *= keep, o[n][i][2 + e] *= keep;
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < KT; k++) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) x[n][k][i] = exp2_approx(x[n][k][i] - ref[n][i & 1]);
+                        l[n][0] += x[n][k][0] + x[n][k][2];  // of this lane's positions
+                        l[n][1] += x[n][k][1] + x[n][k][3];
+#pragma unroll
+                        for (int c = 0; c < 2; c++) {
+                            split_pack<T>(x[n][k][2 * c], x[n][k][2 * c + 1], hi[n][k][c], lo[n][k][c]);
+                            hi[n][k][c] = transpose_8x8(hi[n][k][c]), lo[n][k][c] = transpose_8x8(lo[n][k][c]);  // positions 16 k + 8 c + 2 t, + 1 of row 8 n + g
+                        }
                     }
                 }
-#pragma unroll
-                for (int k = 0; k < KT; k++) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) x[k][i] = exp2_approx(x[k][i] - ref[i & 1]);
-                    l[0] += x[k][0] + x[k][2];  // of this lane's positions
-                    l[1] += x[k][1] + x[k][3];
-#pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        split_pack<T>(x[k][2 * c], x[k][2 * c + 1], hi[k][c], lo[k][c]);
-                        hi[k][c] = transpose_8x8(hi[k][c]), lo[k][c] = transpose_8x8(lo[k][c]);  // positions 16 k + 8 c + 2 t, + 1 of row g
-                    }
-                }
-            }
+            };
+            if (more_rows) scores(std::integral_constant<int, NT>());
+            else if (busy) scores(std::integral_constant<int, 1>());
             if constexpr (!JOINT) {
                 asm volatile("cp.async.wait_group %0;" ::"n"(Shape::WAIT) : "memory");
                 team_sync();  // the values of tile j are here, and its keys are done with
@@ -539,7 +563,7 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
             }
             const uint32_t V = v_lane + cur, v_entry = cur;
             step_on();
-            // ---- O^T += V^T P^T: o[i] is dimensions 16 i + g (registers 0, 1) and + 8 (2, 3) of rows 2 t and 2 t + 1 ----
+            // ---- O^T += V^T P^T: o[n][i] is dimensions 16 i + g (registers 0, 1) and + 8 (2, 3) of rows 8 n + 2 t and + 1 ----
             // Values that are no numbers, in a tile that not every row sees all of?
             bool odd = false;
             if (!full && p.S > 1) {
@@ -550,49 +574,59 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW>::CTAS) paged_attention_m
                 }
                 odd = __any_sync(0xffffffffu, odd);
             }
-            if (busy && !odd) {
-#pragma unroll
-                for (int i = 0; i < KS; i++)
-#pragma unroll
-                    for (int k = 0; k < KT; k++) {
-                        uint32_t a[4];
-                        ldsm4t_at(a, (V ^ (i & 3) << 5) + (i >> 2) * 128 + k * 16 * DP * 2);
-                        mma_kv<T>(o[i], a[0], a[1], a[2], a[3], hi[k][0], hi[k][1]);
-                        mma_kv<T>(o[i], a[0], a[1], a[2], a[3], lo[k][0], lo[k][1]);
-                    }
-            } else if (busy) {
-                // They are taken out of the product and added position by position where they are seen, so that the other rows keep their bits.
+            auto values = [&](auto groups, auto special) {
+                constexpr int N = decltype(groups)::value;
 #pragma unroll
                 for (int i = 0; i < KS; i++)
 #pragma unroll
                     for (int k = 0; k < KT; k++) {
                         uint32_t a[4], c[4];
                         ldsm4t_at(a, (V ^ (i & 3) << 5) + (i >> 2) * 128 + k * 16 * DP * 2);
+                        if constexpr (decltype(special)::value) {
 #pragma unroll
-                        for (int n = 0; n < 4; n++) c[n] = a[n] & special_mask<T>(a[n]), a[n] &= ~special_mask<T>(a[n]);
-                        mma_kv<T>(o[i], a[0], a[1], a[2], a[3], hi[k][0], hi[k][1]);
-                        mma_kv<T>(o[i], a[0], a[1], a[2], a[3], lo[k][0], lo[k][1]);
+                            for (int q = 0; q < 4; q++) c[q] = a[q] & special_mask<T>(a[q]), a[q] &= ~special_mask<T>(a[q]);
+                        }
+#pragma unroll
+                        for (int n = 0; n < N; n++) {
+                            mma_kv<T>(o[n][i], a[0], a[1], a[2], a[3], hi[n][k][0], hi[n][k][1]);
+                            mma_kv<T>(o[n][i], a[0], a[1], a[2], a[3], lo[n][k][0], lo[n][k][1]);
+                        }
+                        if constexpr (decltype(special)::value) {
 #pragma unroll 1
-                        for (int n = 0; n < 16; n++) {
-                            const uint32_t one = (n & 7) >> 1 == t ? (n & 1 ? 0xffff0000u : 0xffffu) : 0u, first = n < 8 ? one : 0u, second = n < 8 ? 0u : one;
-                            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma_kv<T>(acc, c[0] & first, c[1] & first, c[2] & second, c[3] & second, hi[k][0], hi[k][1]);
+                            for (int q = 0; q < 16; q++) {
+                                const uint32_t one = (q & 7) >> 1 == t ? (q & 1 ? 0xffff0000u : 0xffffu) : 0u, first = q < 8 ? one : 0u, second = q < 8 ? 0u : one;
 #pragma unroll
-                            for (int e = 0; e < 2; e++)
-                                if ((exist[0] >> (16 * k + n) & 1) && sees(at[e], base + 16 * k + n)) o[i][e] += acc[e], o[i][2 + e] += acc[2 + e];
+                                for (int n = 0; n < N; n++) {
+                                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                                    mma_kv<T>(acc, c[0] & first, c[1] & first, c[2] & second, c[3] & second, hi[n][k][0], hi[n][k][1]);
+#pragma unroll
+                                    for (int e = 0; e < 2; e++)
+                                        if ((exist[0] >> (16 * k + q) & 1) && sees(at[n][e], base + 16 * k + q)) o[n][i][e] += acc[e], o[n][i][2 + e] += acc[2 + e];
+                                }
+                            }
                         }
                     }
+            };
+            // Values that are no numbers are taken out of the product and added position by position where they are seen, so that the other rows keep their bits.
+            if (!odd) {
+                if (more_rows) values(std::integral_constant<int, NT>(), std::false_type());
+                else if (busy) values(std::integral_constant<int, 1>(), std::false_type());
+            } else {
+                if (more_rows) values(std::integral_constant<int, NT>(), std::true_type());
+                else if (busy) values(std::integral_constant<int, 1>(), std::true_type());
             }
 #pragma unroll
             for (int i = 0; i < AHEAD; i++) exist[i] = exist[i + 1];
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int s = 4; s < 32; s <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], s);
-            if (at[e] < 0) m[e] = -INFINITY, l[e] = 0.f;  // a row that is no query, which tiles that all see are not masked for
-        }
+            for (int e = 0; e < 2; e++) {
+#pragma unroll
+                for (int s = 4; s < 32; s <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], s);
+                if (at[n][e] < 0) m[n][e] = -INFINITY, l[n][e] = 0.f;  // a row that is no query, which tiles that all see are not masked for
+            }
         done_b = b, done_h = h;
         whole = t0 == 0 && t1 == sp.tiles;
         part = p.ws + (((size_t)blockIdx.y * ctas + cta) * 2 + (run.first ? 0 : 1)) * p.part_floats;
@@ -691,7 +725,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_attention_join_kernel(c
 struct PagedPlan {
     bool mma;
     int tile;
-    int dim, team;  // padded head dimension, warps of a team
+    int dim, team, groups;  // padded head dimension, warps of a team, groups of eight rows of a warp
     int ctas, block_rows, row_blocks, round;
     bool whole;
     size_t bytes(int D) const { return whole ? 0 : (size_t)ctas * sizeof(int4) + (size_t)ctas * row_blocks * 2 * part_floats(D) * sizeof(float); }
@@ -701,12 +735,18 @@ struct PagedPlan {
 // Positions of a block table up to which pairs are not cut.
 constexpr int kPagedWhole = 512;
 
+// Tile and CTAs per SM of the kernel for these sizes.
+template <int DP, int RW, int NT>
+static void mma_shape(int *tile, int *ctas) { *tile = MmaShape<DP, RW, NT>::TILE, *ctas = MmaShape<DP, RW, NT>::CTAS; }
 template <int DP>
-static int mma_tile(int team) {
-    return team == 1 ? MmaShape<DP, 1>::TILE : team == 2 ? MmaShape<DP, 2>::TILE : team == 4 ? MmaShape<DP, 4>::TILE : MmaShape<DP, 8>::TILE;
+static void mma_shape_rows(int team, int groups, int *tile, int *ctas) {
+    if constexpr (DP <= 128) {
+        if (groups == 2) return team == 2 ? mma_shape<DP, 2, 2>(tile, ctas) : mma_shape<DP, 4, 2>(tile, ctas);
+        return team == 1 ? mma_shape<DP, 1, 1>(tile, ctas) : mma_shape<DP, 2, 1>(tile, ctas);
+    } else {
+        return team == 1 ? mma_shape<DP, 1, 1>(tile, ctas) : team == 2 ? mma_shape<DP, 2, 1>(tile, ctas) : team == 4 ? mma_shape<DP, 4, 1>(tile, ctas) : mma_shape<DP, 8, 1>(tile, ctas);
+    }
 }
-static int paged_mma_tile(int dim, int team) { return dim == 64 ? mma_tile<64>(team) : dim == 128 ? mma_tile<128>(team) : dim == 192 ? mma_tile<192>(team) : mma_tile<256>(team); }
-
 
 static int paged_sms(int *sms) {
     static std::atomic<int> known[64];  // of a device, once asked for
@@ -731,32 +771,44 @@ static PagedPlan paged_plan(int B, int S, int Hq, int Hkv, int D, int page, int 
     const int R = Hq / Hkv * S;
     n.mma = mma;
     n.dim = D <= 64 ? 64 : D <= 128 ? 128 : D <= 192 ? 192 : 256;
-    n.team = R <= 8 ? 1 : R <= 16 ? 2 : R <= 32 ? 4 : 8;
-    n.block_rows = mma ? 8 * n.team : plain_rows(R, dtype);
+    n.groups = R > 16 && n.dim <= 128 ? 2 : 1;
+    n.team = (R <= 8 ? 1 : R <= 16 ? 2 : R <= 32 ? 4 : 8) / n.groups;
+    n.block_rows = mma ? 8 * n.team * n.groups : plain_rows(R, dtype);
     n.row_blocks = (R + n.block_rows - 1) / n.block_rows;
     n.round = mma ? 8 / n.team : D <= 128 ? 4 : kPlainWarps<8>;
-    n.tile = mma ? paged_mma_tile(n.dim, n.team) : kPagedTile;
-    const long long tiles = ((long long)width * page + n.tile - 1) / n.tile, most = sms * (mma ? (n.dim <= 128 ? 2 : 1) : D <= 32 ? plain_ctas<1>(n.block_rows) : D <= 64 ? plain_ctas<2>(n.block_rows) : D <= 96 ? plain_ctas<3>(n.block_rows) : D <= 128 ? plain_ctas<4>(n.block_rows) : plain_ctas<8>(n.block_rows));
+    int per_sm = 0;
+    if (mma) {
+        if (n.dim == 64) mma_shape_rows<64>(n.team, n.groups, &n.tile, &per_sm);
+        else if (n.dim == 128) mma_shape_rows<128>(n.team, n.groups, &n.tile, &per_sm);
+        else if (n.dim == 192) mma_shape_rows<192>(n.team, n.groups, &n.tile, &per_sm);
+        else mma_shape_rows<256>(n.team, n.groups, &n.tile, &per_sm);
+    } else {
+        n.tile = kPagedTile;
+        per_sm = D <= 32 ? plain_ctas<1>(n.block_rows) : D <= 64 ? plain_ctas<2>(n.block_rows) : D <= 96 ? plain_ctas<3>(n.block_rows) : D <= 128 ? plain_ctas<4>(n.block_rows) : plain_ctas<8>(n.block_rows);
+    }
+    const long long tiles = ((long long)width * page + n.tile - 1) / n.tile, most = (long long)sms * per_sm;
     n.whole = (long long)width * page <= kPagedWhole;
     n.ctas = n.whole ? B * Hkv : (int)std::min<long long>(most, std::max<long long>(1, (tiles * Hkv * B + n.round - 1) / n.round));
     return n;
 }
 
-template <typename T, int DP, int RW>
+template <typename T, int DP, int RW, int NT>
 static int launch_mma(cudaStream_t st, const PagedAttention &p, int ctas) {
+    using Shape = MmaShape<DP, RW, NT>;
     static SmemLimit limit;
-    MYNN_CUDA_OK(limit.raise((const void *)paged_attention_mma_kernel<T, DP, RW>, MmaShape<DP, RW>::SMEM));
-    MYNN_CUDA_OK(launch_dependent(paged_attention_mma_kernel<T, DP, RW>, dim3(ctas, p.row_blocks), dim3(256), MmaShape<DP, RW>::SMEM, st, p));
+    MYNN_CUDA_OK(limit.raise((const void *)paged_attention_mma_kernel<T, DP, RW, NT>, Shape::SMEM));
+    MYNN_CUDA_OK(launch_dependent(paged_attention_mma_kernel<T, DP, RW, NT>, dim3(ctas, p.row_blocks), dim3(256), Shape::SMEM, st, p));
     MYNN_LAUNCH_OK("paged_attention_mma_kernel");
     return MYNN_OK;
 }
 template <typename T, int DP>
 static int launch_mma_rows(cudaStream_t st, const PagedAttention &p, const PagedPlan &n) {
-    switch (n.team) {
-        case 1: return launch_mma<T, DP, 1>(st, p, n.ctas);
-        case 2: return launch_mma<T, DP, 2>(st, p, n.ctas);
-        case 4: return launch_mma<T, DP, 4>(st, p, n.ctas);
-        default: return launch_mma<T, DP, 8>(st, p, n.ctas);
+    if (n.team == 1) return launch_mma<T, DP, 1, 1>(st, p, n.ctas);
+    if constexpr (DP <= 128) {
+        if (n.groups == 2) return n.team == 2 ? launch_mma<T, DP, 2, 2>(st, p, n.ctas) : launch_mma<T, DP, 4, 2>(st, p, n.ctas);
+        return launch_mma<T, DP, 2, 1>(st, p, n.ctas);
+    } else {
+        return n.team == 2 ? launch_mma<T, DP, 2, 1>(st, p, n.ctas) : n.team == 4 ? launch_mma<T, DP, 4, 1>(st, p, n.ctas) : launch_mma<T, DP, 8, 1>(st, p, n.ctas);
     }
 }
 template <typename T>
