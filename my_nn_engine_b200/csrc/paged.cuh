@@ -5,7 +5,7 @@
 // of the sequence with its new tokens, counts[b] the new tokens: query s of the sequence sits at position lengths[b] - counts[b] + s.
 //
 // Sequences of a batch have lengths of their own, so a fixed number of CTAs per sequence would leave most of the GPU waiting for the longest one.
-// The visible rows are cut into tiles of 16 or 32 positions (p.tile), and all tiles of all (sequence, kv head) pairs, one pair behind the other, are
+// The visible rows are cut into tiles of 8, 16 or 32 positions (p.tile), and all tiles of all (sequence, kv head) pairs, one pair behind the other, are
 // dealt out evenly: each CTA takes one run of `share` tiles, which may end one pair, hold a few whole ones and begin another.  A pair that
 // lies in one CTA is finished there; the parts of the others go to a workspace and are joined by a second kernel.  A CTA has at most two parts:
 // the pair its run begins inside of (slot 0) and the pair it ends inside of (slot 1); it records the one that begins in it and ends elsewhere.  The lengths are on
@@ -62,7 +62,7 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttention &p, int b) 
     s.rows = min(s.len, p.width * p.page);
     s.count = p.counts ? min(max(p.counts[b], 0), p.S) : p.S;
     const int oldest = s.len - s.count;
-    const int shift = p.tile == 16 ? 4 : 5, up = p.tile - 1;
+    const int shift = p.tile == 8 ? 3 : p.tile == 16 ? 4 : 5, up = p.tile - 1;
     const int all = (s.rows + up) >> shift;
     const int lo = p.window > 0 ? min(max(0, oldest - p.window + 1) >> shift, all) : 0;  // the tile that the windows begin in
     s.sink_tiles = min((min(p.sinks, s.rows) + up) >> shift, lo);

@@ -11,20 +11,21 @@ namespace mynn {
 // of -inf, and adds nothing.
 __device__ __forceinline__ float paged_quotient(float O, float L) { return L == 0.f ? 0.f : O / L; }
 
-constexpr int kPagedTile = 16;  // of the kernel for any sizes
+constexpr int kPlainTile = 8;
 
 // ---- any sizes ----------------------------------------------------------------------------------------------------------
-// f32 caches, heads that are no multiple of 8 numbers, unaligned tensors.  Each warp takes tiles of 16 positions into shared memory as f32; in the first product
-// a lane has one key and half of the dimensions, in the second the dimensions lane, lane + 32, ...
+// f32 caches, heads that are no multiple of 8 numbers, unaligned tensors.  Each warp takes tiles of 8 positions into shared memory as f32; in the first product
+// a lane has one key and a quarter of the dimensions, in the second the dimensions lane, lane + 32, ...  Small tiles leave room for many warps, which hide each other's
+// chains: with tiles of 16 and half the warps 64 sequences of 1000, 8 heads of 128, took 192 us.
 // RB: query rows of a CTA (one head per kv head: with eight rows where one is needed 7 sequences of 1 to 1501, 12 heads of 80, took 46 us).
 // VEC: elements of a copy to shared memory (cp.async, f32); 0: 16-bit elements, converted on the way.
 template <int DL>
-constexpr int kPlainWarps = DL > 4 ? 2 : 4;
+constexpr int kPlainWarps = DL > 4 ? 4 : 8;
 template <int DL, int RB>
 struct PlainShape {
     static constexpr int W = kPlainWarps<DL>, PITCH = DL * 32 + 4;
-    static constexpr int RING = 2 * 2 * kPagedTile * PITCH;  // floats of a warp: two stages, keys and values
-    static constexpr int WEIGHTS = kPagedTile * (RB < 4 ? 4 : RB), SUMS = RB * DL * 32;
+    static constexpr int RING = 2 * 2 * kPlainTile * PITCH;  // floats of a warp: two stages, keys and values
+    static constexpr int WEIGHTS = kPlainTile * (RB < 4 ? 4 : RB), SUMS = RB * DL * 32;
     static constexpr size_t SMEM = sizeof(float) * (size_t)(RB * PITCH + W * (RING + WEIGHTS + SUMS));
     static constexpr int CTAS = SMEM <= 112 * 1024 ? 2 : 1;  // per SM
 };
@@ -37,12 +38,12 @@ __device__ __forceinline__ void copy_async(void *smem, const void *gmem, bool in
 template <typename T, int DL, int RB, int VEC>
 __global__ void __launch_bounds__(kPlainWarps<DL> * 32, PlainShape<DL, RB>::CTAS) paged_attention_plain_kernel(const PagedAttention p) {
     using Shape = PlainShape<DL, RB>;
-    constexpr int W = Shape::W, PITCH = Shape::PITCH, TILE = kPagedTile, WR = Shape::WEIGHTS / TILE;
+    constexpr int W = Shape::W, PITCH = Shape::PITCH, TILE = kPlainTile, WR = Shape::WEIGHTS / TILE;
     extern __shared__ __align__(16) float sm[];
     __shared__ float part_m[W][RB], part_l[W][RB];
     pdl_trigger();
     pdl_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, key = lane & 15, side = lane >> 4;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, key = lane & 7, side = lane >> 3;
     const int cta = blockIdx.x, ctas = gridDim.x, r0 = blockIdx.y * RB, rows = min(p.group * p.S - r0, RB), D = p.D;
     float *sq = sm, *ring = sm + RB * PITCH + warp * Shape::RING, *weights = sm + RB * PITCH + W * Shape::RING + warp * Shape::WEIGHTS;
     float *sums = sm + RB * PITCH + W * (Shape::RING + Shape::WEIGHTS);
@@ -68,7 +69,7 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32, PlainShape<DL, RB>::CTAS
 #pragma unroll 2
             for (int i = lane; i < (TILE * pieces + 31) / 32 * 32; i += 32) {
                 const int r = p.by_pieces.div(i), d = (i - r * pieces) * (VEC > 0 ? VEC : 1);
-                const int from = __shfl_sync(0xffffffffu, row, r & 15);
+                const int from = __shfl_sync(0xffffffffu, row, r & 7);
                 if (r >= TILE) continue;
                 const size_t at = (size_t)(uint32_t)max(from, 0) * (uint32_t)D + d;
                 float *dst = to + r * PITCH + d;
@@ -108,9 +109,9 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32, PlainShape<DL, RB>::CTAS
             __syncwarp();
             const float *K = ring + stage * 2 * TILE * PITCH, *V = K + TILE * PITCH;
             float x[RB] = {};
-            const int half = (D + 7) / 8 * 4;
+            const int quarter = (D + 15) / 16 * 4;
 #pragma unroll 4
-            for (int d = side * half; d < (side + 1) * half; d += 4) {
+            for (int d = side * quarter; d < (side + 1) * quarter; d += 4) {
                 const float4 a = *reinterpret_cast<const float4 *>(K + key * PITCH + d);
 #pragma unroll
                 for (int r = 0; r < RB; r++) {
@@ -119,21 +120,33 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32, PlainShape<DL, RB>::CTAS
                 }
             }
             const int j = sp.at(t) * TILE + key;
+            bool moved = false;
 #pragma unroll
             for (int r = 0; r < RB; r++) {
+                x[r] += __shfl_xor_sync(0xffffffffu, x[r], 8);
                 x[r] += __shfl_xor_sync(0xffffffffu, x[r], 16);
                 x[r] *= p.scale;
                 if (p.softcap > 0.f) x[r] = p.softcap * tanhf(x[r] / p.softcap);
-                if (r >= rows || row < 0 || !paged_sees(p, sp, p.by_S.mod(r0 + r, p.by_S.div(r0 + r)), j)) x[r] = -INFINITY;
-                float top = x[r];
+                if (r >= rows || row < 0 || (p.S > 1 && !paged_sees(p, sp, p.by_S.mod(r0 + r, p.by_S.div(r0 + r)), j))) x[r] = -INFINITY;  // (one query sees what there is)
+                moved |= x[r] > m[r];
+            }
+            if (__any_sync(0xffffffffu, moved)) {  // most tiles raise no maximum
 #pragma unroll
-                for (int s = 8; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-                const float now = fmaxf(m[r], top), ref = merge_reference(now), keep = expf(m[r] - ref), w = expf(x[r] - ref);
-                m[r] = now;
-                l[r] = l[r] * keep + (side ? 0.f : w);
-                if (!side) weights[key * WR + r] = w;
+                for (int r = 0; r < RB; r++) {
+                    float top = x[r];
 #pragma unroll
-                for (int i = 0; i < DL; i++) o[r][i] *= keep;
+                    for (int s = 4; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+                    const float now = fmaxf(m[r], top), keep = expf(m[r] - merge_reference(now));
+                    m[r] = now;
+                    l[r] *= keep;
+#pragma unroll
+                    for (int i = 0; i < DL; i++) o[r][i] *= keep;
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < RB; r++) {
+                const float w = expf(x[r] - merge_reference(m[r]));
+                if (side == 0) l[r] += w, weights[key * WR + r] = w;
             }
             __syncwarp();
             const bool full = p.S == 1 || paged_tile_full(p, sp, sp.at(t) * TILE, TILE);
@@ -732,9 +745,6 @@ struct PagedPlan {
     int part_floats(int D) const { return (block_rows * (D + 2) + 3) / 4 * 4; }  // 16-byte pieces of them are read
 };
 
-// Positions of a block table up to which pairs are not cut.
-constexpr int kPagedWhole = 512;
-
 // Tile and CTAs per SM of the kernel for these sizes.
 template <int DP, int RW, int NT>
 static void mma_shape(int *tile, int *ctas) { *tile = MmaShape<DP, RW, NT>::TILE, *ctas = MmaShape<DP, RW, NT>::CTAS; }
@@ -775,7 +785,7 @@ static PagedPlan paged_plan(int B, int S, int Hq, int Hkv, int D, int page, int 
     n.team = (R <= 8 ? 1 : R <= 16 ? 2 : R <= 32 ? 4 : 8) / n.groups;
     n.block_rows = mma ? 8 * n.team * n.groups : plain_rows(R, dtype);
     n.row_blocks = (R + n.block_rows - 1) / n.block_rows;
-    n.round = mma ? 8 / n.team : D <= 128 ? 4 : kPlainWarps<8>;
+    n.round = mma ? 8 / n.team : D <= 128 ? kPlainWarps<4> : kPlainWarps<8>;
     int per_sm = 0;
     if (mma) {
         if (n.dim == 64) mma_shape_rows<64>(n.team, n.groups, &n.tile, &per_sm);
@@ -783,11 +793,11 @@ static PagedPlan paged_plan(int B, int S, int Hq, int Hkv, int D, int page, int 
         else if (n.dim == 192) mma_shape_rows<192>(n.team, n.groups, &n.tile, &per_sm);
         else mma_shape_rows<256>(n.team, n.groups, &n.tile, &per_sm);
     } else {
-        n.tile = kPagedTile;
+        n.tile = kPlainTile;
         per_sm = D <= 32 ? plain_ctas<1>(n.block_rows) : D <= 64 ? plain_ctas<2>(n.block_rows) : D <= 96 ? plain_ctas<3>(n.block_rows) : D <= 128 ? plain_ctas<4>(n.block_rows) : plain_ctas<8>(n.block_rows);
     }
     const long long tiles = ((long long)width * page + n.tile - 1) / n.tile, most = (long long)sms * per_sm;
-    n.whole = (long long)width * page <= kPagedWhole;
+    n.whole = (long long)width * page <= (mma ? 1024 : 256);
     n.ctas = n.whole ? B * Hkv : (int)std::min<long long>(most, std::max<long long>(1, (tiles * Hkv * B + n.round - 1) / n.round));
     return n;
 }

@@ -694,7 +694,7 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale, counts=Non
         # not kept between calls: two captured graphs, or two streams, never share it
         size = _paged_ws_bytes(device, B, S, Hq, G, D, page, width)
         ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-        ffi.check(ffi.lib().mynn_b200_paged_attention(_stream(), out_p, q_p, k_p, v_p, table_p, lengths_p, counts_p, scale, softcap, window, sinks, B, S, Hq, G, D, page, n,
+        ffi.check(ffi.lib().mynn_b200_paged_attention(_stream(), out_p, q_p, k_p, v_p, table_p, lengths_p, counts_p, scale, softcap, min(window, 2**31 - 1), min(sinks, 2**31 - 1), B, S, Hq, G, D, page, n,
                                                       width, _dt(q), ws.data_ptr() if size else None, size))
     return out
 
