@@ -57,6 +57,14 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32, PlainShape<DL, RB>::CTAS
         if (paged_span(p, b).tiles == 0)
             for (int h = 0; h < p.G; h++)
                 for (int i = threadIdx.x; i < rows * D; i += W * 32) reinterpret_cast<T *>(p.out)[place(b, h, r0 + i / D, i % D)] = from_f32<T>(0.f);
+    // this lane's 16-byte pieces of a tile's rows: row and first number, -1: none
+    constexpr int COPIES = VEC == 4 ? TILE * DL * 8 / 32 : 1;
+    int copies[COPIES];
+#pragma unroll
+    for (int u = 0; u < COPIES; u++) {
+        const int i = lane + 32 * u, r = p.by_pieces.div(i);
+        copies[u] = r < TILE ? r << 16 | 4 * (i - r * (D / 4)) : -1;
+    }
     PagedRun run;
     run.begin(paged_find<W * 32>(p, cta, ctas));
     PagedSpan sp;
@@ -65,20 +73,33 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32, PlainShape<DL, RB>::CTAS
         auto row_of = [&](int t) { return t < t1 ? paged_row(p, sp, b, h, sp.at(t) * TILE + key) : -1; };
         auto issue = [&](int row, int stage) {
             float *to = ring + stage * 2 * TILE * PITCH;
-            const int pieces = VEC > 0 ? D / VEC : D;
+            if constexpr (VEC == 4) {
+#pragma unroll
+                for (int u = 0; u < COPIES; u++) {
+                    const int r = copies[u] >> 16 & 7, d = copies[u] & 0xffff;
+                    const int from = __shfl_sync(0xffffffffu, row, r);
+                    if (copies[u] < 0) continue;
+                    const size_t at = (size_t)(uint32_t)max(from, 0) * (uint32_t)(D * 4) + 4 * d;
+                    float *dst = to + r * PITCH + d;
+                    copy_async<16>(dst, reinterpret_cast<const char *>(p.k) + at, from >= 0);
+                    copy_async<16>(dst + TILE * PITCH, reinterpret_cast<const char *>(p.v) + at, from >= 0);
+                }
+            } else {
+                const int pieces = D;
 #pragma unroll 2
-            for (int i = lane; i < (TILE * pieces + 31) / 32 * 32; i += 32) {
-                const int r = p.by_pieces.div(i), d = (i - r * pieces) * (VEC > 0 ? VEC : 1);
-                const int from = __shfl_sync(0xffffffffu, row, r & 7);
-                if (r >= TILE) continue;
-                const size_t at = (size_t)(uint32_t)max(from, 0) * (uint32_t)D + d;
-                float *dst = to + r * PITCH + d;
-                if constexpr (VEC > 0) {
-                    copy_async<4 * VEC>(dst, reinterpret_cast<const float *>(p.k) + at, from >= 0);
-                    copy_async<4 * VEC>(dst + TILE * PITCH, reinterpret_cast<const float *>(p.v) + at, from >= 0);
-                } else {
-                    dst[0] = from >= 0 ? to_f32<T>(reinterpret_cast<const T *>(p.k)[at]) : 0.f;
-                    dst[TILE * PITCH] = from >= 0 ? to_f32<T>(reinterpret_cast<const T *>(p.v)[at]) : 0.f;
+                for (int i = lane; i < (TILE * pieces + 31) / 32 * 32; i += 32) {
+                    const int r = p.by_pieces.div(i), d = i - r * pieces;
+                    const int from = __shfl_sync(0xffffffffu, row, r & 7);
+                    if (r >= TILE) continue;
+                    const size_t at = (size_t)(uint32_t)max(from, 0) * (uint32_t)D + d;
+                    float *dst = to + r * PITCH + d;
+                    if constexpr (VEC == 1) {
+                        copy_async<4>(dst, reinterpret_cast<const float *>(p.k) + at, from >= 0);
+                        copy_async<4>(dst + TILE * PITCH, reinterpret_cast<const float *>(p.v) + at, from >= 0);
+                    } else {
+                        dst[0] = from >= 0 ? to_f32<T>(reinterpret_cast<const T *>(p.k)[at]) : 0.f;
+                        dst[TILE * PITCH] = from >= 0 ? to_f32<T>(reinterpret_cast<const T *>(p.v)[at]) : 0.f;
+                    }
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
@@ -150,22 +171,26 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32, PlainShape<DL, RB>::CTAS
             }
             __syncwarp();
             const bool full = p.S == 1 || paged_tile_full(p, sp, sp.at(t) * TILE, TILE);
-#pragma unroll(RB > 4 ? 2 : 8)
-            for (int k = 0; k < TILE; k++) {
-                float w[WR];
+            auto weigh = [&](auto guarded) {  // guarded: what a row does not see has to be kept from it, not only weighted by zero
 #pragma unroll
-                for (int r = 0; r < WR; r += 4) {
-                    const float4 u = *reinterpret_cast<const float4 *>(weights + k * WR + r);
-                    w[r] = u.x, w[r + 1] = u.y, w[r + 2] = u.z, w[r + 3] = u.w;
+                for (int k = 0; k < TILE; k++) {
+                    float w[WR];
+#pragma unroll
+                    for (int r = 0; r < WR; r += 4) {
+                        const float4 u = *reinterpret_cast<const float4 *>(weights + k * WR + r);
+                        w[r] = u.x, w[r + 1] = u.y, w[r + 2] = u.z, w[r + 3] = u.w;
+                    }
+#pragma unroll
+                    for (int i = 0; i < DL; i++) {
+                        const float v = V[k * PITCH + lane + 32 * i];
+#pragma unroll
+                        for (int r = 0; r < RB; r++)
+                            if (!decltype(guarded)::value || w[r] != 0.f) o[r][i] += w[r] * v;
+                    }
                 }
-#pragma unroll
-                for (int i = 0; i < DL; i++) {
-                    const float v = V[k * PITCH + lane + 32 * i];
-#pragma unroll
-                    for (int r = 0; r < RB; r++)
-                        if (full || w[r] != 0.f) o[r][i] += w[r] * v;
-                }
-            }
+            };
+            if (full) weigh(std::false_type());
+            else weigh(std::true_type());
             __syncwarp();
             row = next;
             next = after;

@@ -128,6 +128,38 @@ def test_drafted_tokens(dt, H, G, D, S):
     run_attention(S + 1, dt, [max(n, S) for n in lengths], H, G, D, 24, S)
 
 
+@pytest.mark.parametrize("dt,D", [("bf16", 64), ("bf16", 128), ("f16", 40), ("f32", 64), ("f32", 33)])
+def test_sequences_shorter_than_their_places(dt, D):
+    """Without counts every place is a token: those of a sequence of fewer positions lie before its first one and see nothing."""
+    for S in (3, 9):
+        run_attention(S, dt, [0, 1, 2, S - 1, S, 700], 8, 2, D, 16, S)
+
+
+@pytest.mark.parametrize("dt,D", [("bf16", 64), ("f16", 128), ("bf16", 192), ("bf16", 256), ("bf16", 96), ("f32", 64)])
+@pytest.mark.parametrize("group,S", [(1, 9), (5, 5), (8, 3), (8, 4), (7, 7), (8, 8), (9, 8), (4, 33)])
+def test_numbers_of_rows_around_the_sizes_of_teams(dt, D, group, S):
+    """9 to 132 query rows per kv head, over pairs that are cut and pairs that are not."""
+    run_attention(group + S, dt, [1500, S, 77], 2 * group, 2, D, 16, S, [S, max(1, S - 2), 1])
+    run_attention(group, dt, [S + 100, S], group, 1, D, 8, S, window=40, sinks=3)
+
+
+def test_one_query_over_a_very_long_cache():
+    """More CTAs than a pair has rows of parts in one go of the joining kernel."""
+    for dt, D in (("bf16", 64), ("f32", 32)):
+        run_attention(D, dt, [100003], 2, 1, D, 64)
+
+
+def test_a_batch_larger_than_the_grid():
+    rng = np.random.default_rng(3)
+    lengths = [int(n) for n in rng.integers(0, 40, 700)]
+    for width in (0, 70):  # a table that pairs are not cut for, and a wide one
+        k, v, table = cache(rng, lengths, 1, 64, 16, "bf16")
+        table = torch.nn.functional.pad(table, (0, width), value=-1).contiguous()
+        q = torch.from_numpy(rng.standard_normal((700, 2, 1, 64))).to("cuda", torch.bfloat16)
+        want, mass = want_attention(q, k, v, table, lengths, [1] * 700, 0.125)
+        close_attention(ops.paged_attention(q, k, v, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), 0.125), want, mass, "bf16")
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (100, 0), (100, 33), (257, 16), (5000, 4), (2 ** 31 - 1, 2 ** 31 - 1)])
 @pytest.mark.parametrize("S", [1, 4])
@@ -494,6 +526,26 @@ def test_calls_on_two_streams_and_repeated_calls_give_the_same_bits():
 
 
 # ---- refusals ------------------------------------------------------------------------------------------------------------
+def test_windows_beyond_32_bits_are_the_whole_past():
+    rng = np.random.default_rng(9)
+    k, v, table = cache(rng, [100], 1, 64, 16, "bf16")
+    q, n = torch.from_numpy(rng.standard_normal((1, 2, 1, 64))).to("cuda", torch.bfloat16), torch.tensor([100], dtype=torch.int32, device="cuda")
+    whole = ops.paged_attention(q, k, v, table, n, 0.1)
+    assert torch.equal(ops.paged_attention(q, k, v, table, n, 0.1, window=2 ** 32 + 5, sinks=2 ** 33), whole)
+    assert torch.equal(ops.paged_attention(q, k, v, table, n, 0.1, window=-1), whole)
+
+
+def test_a_batch_in_which_nobody_has_a_token():
+    k = torch.randn(4, 2, 16, 64, device="cuda", dtype=torch.bfloat16)
+    table, n, c = torch.zeros(3, 200, dtype=torch.int32, device="cuda"), torch.full((3,), 9, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    for dt in (torch.bfloat16, torch.float32):
+        out = torch.full((3, 2, 4, 64), 7.0, device="cuda", dtype=dt)
+        assert not ops.paged_attention(torch.full((3, 4, 2, 64), float("nan"), device="cuda", dtype=dt), k.to(dt), k.to(dt), table, n, 1.0, counts=c, out=out).any()
+    k2, v2 = k.clone(), k.clone()
+    q = ops.paged_rotary_append(torch.full((3, 2, 8 * 64), float("nan"), device="cuda", dtype=torch.bfloat16), n, table, k2, v2, 4, counts=c)
+    assert not q.any() and torch.equal(k2, k) and torch.equal(v2, k)
+
+
 def test_empty_batches():
     k = torch.zeros(2, 1, 16, 64, device="cuda", dtype=torch.bfloat16)
     table, n = torch.zeros(0, 3, dtype=torch.int32, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda")
