@@ -567,7 +567,7 @@ int mynn_b200_paged_attention(void *stream, void *out, const void *q, const void
  * dtype.  Token i is accepted while accept[b, i] * q_i(x_i) < p_i(x_i) (a token outside the vocabulary is not); accepted_out int32 [B] counts
  * them, n.  tokens_out int32 [B, K + 1]: the accepted ones, then one token drawn from max(p_n - q_n, 0), behind all of them from p_n, then -1.  The draw
  * is the first token whose running sum exceeds sample[b] times the whole sum, in 64 bits; where p_n - q_n leaves nothing it is from p_n, and where
- * p_n has nothing either the token is -1.  accept f32 [B, K], sample f32 [B] in [0, 1). */
+ * p_n has nothing either the token is -1.  accept f32 [B, K], sample f32 [B] in [0, 1).  B <= 65535, K <= 1024. */
 int mynn_b200_verify_draft(void *stream, int32_t *tokens_out, int32_t *accepted_out, const void *target, const void *draft, const int32_t *tokens,
                            const int32_t *counts, const float *accept, const float *sample, int B, int K, int V, int dtype);
 

@@ -4,6 +4,8 @@
 // Rotation and norm are f32, the result is rounded once.  A CTA takes one token.  Where heads come in pieces of eight numbers, a thread holds two pieces: piece i of
 // the rotated half and its partner half a rotated range away, or two neighbours; it does so for one head after the other, so a token's angles are read once per
 // thread, and a head's norm is a sum over the few threads that share it.  Other sizes (paged_append_any_kernel): a warp per head, staged in shared memory.
+// Bound by bytes for prompts and by the chain of lengths, table and store for a step: 32 tokens of 48 heads of 128 take 2.4 us (a warp per head: 6.7), 6 prompts of 777
+// places that are mostly padding, whose zero queries are 38 MB, 14 us (read before it was known that they are padding: 24).
 #include <algorithm>
 
 #include "common.cuh"
@@ -231,7 +233,6 @@ extern "C" int mynn_b200_paged_rotary_append(void *stream, void *q_out, void *k_
     const bool pieces = D % 16 == 0 && D <= 512 && rot_dims % (halves ? 16 : 8) == 0 && B <= 65535 &&
                         ((uintptr_t)proj | (uintptr_t)q_out | (uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0;
     if (pieces) {
-        // 32 sequences of one token, 48 heads of 128: 6.7 us with a warp per head
         int lanes = 1;
         while (lanes < D / 16) lanes *= 2;
         const int threads = (int)std::min<long long>(512, ((long long)(Hq + 2 * Hkv) * lanes + 31) / 32 * 32);

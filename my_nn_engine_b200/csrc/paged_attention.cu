@@ -1,4 +1,5 @@
-// Attention of the new tokens of each sequence over a paged cache (paged.cuh says how the work is dealt out).
+// Attention of the new tokens of each sequence over a paged cache: o = softmax(cap(scale q k^T)) v over the positions a query sees, in one pass with a running reference
+// m and sum l of the weights e^(x - m).  paged.cuh says how the work is dealt out; parts of pairs that lie in several CTAs are joined by a second kernel.
 #include <algorithm>
 #include <atomic>
 
@@ -16,7 +17,8 @@ constexpr int kPlainTile = 8;
 // ---- any sizes ----------------------------------------------------------------------------------------------------------
 // f32 caches, heads that are no multiple of 8 numbers, unaligned tensors.  Each warp takes tiles of 8 positions into shared memory as f32; in the first product
 // a lane has one key and a quarter of the dimensions, in the second the dimensions lane, lane + 32, ...  Small tiles leave room for many warps, which hide each other's
-// chains: with tiles of 16 and half the warps 64 sequences of 1000, 8 heads of 128, took 192 us.
+// chains: with tiles of 16 and half the warps 64 sequences of 1000, 8 heads of 128, took 192 us, now 166 = 0.49 of the copy bandwidth.  f32 has no tensor-core
+// form that keeps 24 bits, so the instructions around the 2 RB D multiplications of a position bound it: about 1000 per tile of 8 at four rows.
 // RB: query rows of a CTA (one head per kv head: with eight rows where one is needed 7 sequences of 1 to 1501, 12 heads of 80, took 46 us).
 // VEC: elements of a copy to shared memory (cp.async, f32); 0: 16-bit elements, converted on the way.
 template <int DL>
@@ -237,9 +239,12 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32, PlainShape<DL, RB>::CTAS
 // the first product's result behind a transposition of its 8 x 8 blocks.  Weights enter as a 16-bit part and its remainder (16 bits in all); scores, maxima and
 // sums are f32.  The reference of the weights is moved only when a score exceeds it by 2^8, so most tiles need no maximum across lanes and no rescaling.  D is padded
 // to DP with zeros, on the chip only.
-// The chain of one tile is long (two products, a softmax) and each warp walks it alone, so warps are what hides it: sixteen per SM with eight query rows each (96 mixed
-// sequences of heads of 64: 81 us, eight warps with sixteen rows 97).  From 17 rows on the instructions bound it, and sixteen rows of a warp share the blocks of keys and values and what goes
-// on around the products.
+// The chain of one tile is long (two products, a softmax) and each warp walks it alone, so warps are what hides it: sixteen per SM with eight query rows each (with eight
+// warps of sixteen rows 96 mixed sequences of heads of 64 took a fifth longer).  From 17 rows on the instructions bound it, and sixteen rows of a warp share the blocks
+// of keys and values and what goes on around the products (20 rows over 131072 positions: 110 us with eight rows per warp, 105 with sixteen).
+// Measured with the joining kernel behind it, 8 kv heads of 128, bf16: 32 sequences of 2048 47 us = 0.87 of the copy bandwidth, one of 131071 91 us = 0.90, 16 of 1500 to
+// 4500 with up to 5 queries of 4 heads 55 us = 0.54, 48 with windows of 1000 over pages of 24 41 us = 0.73, one of 300 7 us; 4 kv heads of 64, f16: 96 of 1 to 6000
+// 56 us = 0.81.  What is left is what a launch costs around its pass: to find its run, the first copies, the last sums and the join take some 8 us.
 template <int DP, int RW, int NT>
 struct MmaShape {
     static constexpr int W = 8, TEAMS = W / RW, ROWS = 8 * NT * RW;
@@ -676,6 +681,7 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
 // ---- parts of pairs that lie in several CTAs ------------------------------------------------------------------------------
 // grid (CTAs of the kernel in front, row groups): a CTA takes `rows` rows (1, 2, 4 or 8) of the pair that the CTA of its number recorded, 8 / rows warps
 // each; the parts of a row are dealt out to its warps, eight at a time and loads first.  V: floats of a load.
+// Waits of L2 in a row: the record, the maxima, the rows.
 constexpr int kJoinWarps = 8;
 template <typename T, int V>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_attention_join_kernel(const PagedAttention p, int ctas, int rows) {
@@ -806,7 +812,7 @@ static PagedPlan paged_plan(int B, int S, int Hq, int Hkv, int D, int page, int 
     const int R = Hq / Hkv * S;
     n.mma = mma;
     n.dim = D <= 64 ? 64 : D <= 128 ? 128 : D <= 192 ? 192 : 256;
-    n.groups = R > 16 && n.dim <= 128 ? 2 : 1;
+    n.groups = R > 16 && n.dim <= 128 ? 2 : 1;  // (more would not fit the registers)
     n.team = (R <= 8 ? 1 : R <= 16 ? 2 : R <= 32 ? 4 : 8) / n.groups;
     n.block_rows = mma ? 8 * n.team * n.groups : plain_rows(R, dtype);
     n.row_blocks = (R + n.block_rows - 1) / n.block_rows;
@@ -822,6 +828,8 @@ static PagedPlan paged_plan(int B, int S, int Hq, int Hkv, int D, int page, int 
         per_sm = D <= 32 ? plain_ctas<1>(n.block_rows) : D <= 64 ? plain_ctas<2>(n.block_rows) : D <= 96 ? plain_ctas<3>(n.block_rows) : D <= 128 ? plain_ctas<4>(n.block_rows) : plain_ctas<8>(n.block_rows);
     }
     const long long tiles = ((long long)width * page + n.tile - 1) / n.tile, most = (long long)sms * per_sm;
+    // Tables of so many positions: pairs are not cut, and no second kernel follows.  One sequence, 8 kv heads of 128, 16 bits: 500 positions 8.0 us whole, 10.6 cut, 1000
+    // 11.1 and 11.8; in f32 100 positions 10 us whole, 12 cut, 300 19 and 12.
     n.whole = (long long)width * page <= (mma ? 1024 : 256);
     n.ctas = n.whole ? B * Hkv : (int)std::min<long long>(most, std::max<long long>(1, (tiles * Hkv * B + n.round - 1) / n.round));
     return n;
@@ -906,6 +914,10 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
     if ((long long)pages * Hkv * page > INT_MAX) return fail(MYNN_E_UNSUPPORTED, "paged_attention: a cache of %lld rows", (long long)pages * Hkv * page);
     if (B == 0) return MYNN_OK;
     if (!out || !q || !block_table || !lengths || (pages && (!k_pages || !v_pages))) return fail(MYNN_E_ARG, "paged_attention: null pointer");
+    if (pages == 0) {  // nobody sees anything, and there is no address to copy from
+        MYNN_CUDA_OK(cudaMemsetAsync(out, 0, (size_t)B * S * Hq * D * dtype_size(dtype), (cudaStream_t)stream));
+        return MYNN_OK;
+    }
     int sms = 0;
     if (const int e = paged_sms(&sms)) return e;
     const bool mma = dtype != MYNN_F32 && D % 8 == 0 && ((uintptr_t)out | (uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0;
@@ -916,7 +928,7 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
     const int vec = D % 4 == 0 && ((uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0 ? 4 : 1;
     PagedAttention p;
     p.out = out, p.q = q;
-    p.k = pages ? k_pages : q, p.v = pages ? v_pages : q;  // (a copy of nothing has an address too)
+    p.k = k_pages, p.v = v_pages;
     p.table = block_table, p.lengths = lengths, p.counts = counts;
     p.scale = scale, p.softcap = softcap, p.window = std::min(window, kPagedWindow), p.sinks = sinks;
     p.B = B, p.S = S, p.Hq = Hq, p.G = Hkv, p.group = Hq / Hkv, p.D = D;
@@ -925,6 +937,8 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
     p.row_blocks = n.row_blocks, p.block_rows = n.block_rows, p.part_floats = n.part_floats(D), p.round = n.round;
     p.whole = n.whole;
     p.tile = n.tile;
+    // 96 mixed sequences of 1 to 6000, 4 kv heads of 64: 74 us with no toll, 66 with 8 tiles of 16 positions, 59 with 16, 58 with 32 (16 with drafts 72, 72, 71, 70; one of
+    // 131071 95, 95, 95, 97); f32, 7 of 1 to 1501: 120 with none, 65 with one round of the warps, 64 with two, 72 with four.
     p.toll = n.mma ? 256 / n.tile : 2 * n.round;
     p.strips = n.mma && page % 8 == 0 && D == n.dim;
     p.records = reinterpret_cast<int4 *>(workspace);

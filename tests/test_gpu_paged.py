@@ -556,6 +556,10 @@ def test_empty_batches():
     none = torch.zeros(0, 1, 16, 64, device="cuda", dtype=torch.bfloat16)  # a cache without pages
     table, n = torch.full((2, 1), 0, dtype=torch.int32, device="cuda"), torch.ones(2, dtype=torch.int32, device="cuda")
     assert not ops.paged_attention(torch.ones(2, 4, 1, 64, device="cuda", dtype=torch.bfloat16), none, none, table, n, 1.0).any()
+    for dt in (torch.float32, torch.float16):
+        q = torch.ones(2 * 4 * 64 + 1, device="cuda", dtype=dt)[1:].view(2, 4, 1, 64)
+        assert not ops.paged_attention(q, none.to(dt), none.to(dt), table, n, 1.0, out=torch.ones(2, 1, 4, 64, device="cuda", dtype=dt)).any()
+    assert not ops.paged_rotary_append(torch.ones(2, 1, 6 * 64, device="cuda", dtype=torch.bfloat16), n, table, none, none, 4).eq(0).any()
 
 
 def test_host_tensors_are_refused():
