@@ -7,7 +7,6 @@ tensors and the call raises otherwise.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 
@@ -625,12 +624,9 @@ def _pointers(*tensors):
     return device, out
 
 
-_HERE = contextlib.nullcontext()
-
-
-def _on(device):
-    """The operators of this section run on their tensors' device and its current stream, whichever device is current."""
-    return _HERE if _device is not None and device == _device() else torch.cuda.device(device)
+def _elsewhere(device):
+    """The operators of this section run on their tensors' device and its current stream: is another device current?"""
+    return _device is None or device != _device()
 
 
 def _pages(k_pages, v_pages, dtype, block_table, lengths, counts, batch):
@@ -663,11 +659,16 @@ def paged_rotary_append(proj, lengths, block_table, k_pages, v_pages, heads, cos
     if (cos is None) != (sin is None) or (cos is not None and (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape)):
         raise ValueError("cos and sin must be f32 tensors of one shape [positions, rotated / 2], or both None")
     device, (proj_p, lengths_p, table_p, k_p, v_p, cos_p, sin_p, counts_p) = _pointers(proj, lengths, block_table, k_pages, v_pages, cos, sin, counts)
-    with _on(device):
-        q = torch.empty((B, heads, S, D), dtype=proj.dtype, device=proj.device)
-        ffi.check(ffi.lib().mynn_b200_paged_rotary_append(_stream(), q.data_ptr(), k_p, v_p, proj_p, cos_p, sin_p, lengths_p, counts_p, table_p, B, S, heads, G, D, 2 * half,
-                                                          int(halves), int(qk_norm), eps, page, n, width, positions, _dt(proj)))
+    if _elsewhere(device) and torch.cuda.current_device() != device:
+        with torch.cuda.device(device):
+            return paged_rotary_append(proj, lengths, block_table, k_pages, v_pages, heads, cos, sin, counts, halves, qk_norm, eps)
+    q = torch.empty_strided((B, heads, S, D), (heads * S * D, S * D, D, 1), dtype=proj.dtype, device=proj.device)  # (half the time of torch.empty)
+    ffi.check(ffi.lib().mynn_b200_paged_rotary_append(_stream(), q.data_ptr(), k_p, v_p, proj_p, cos_p, sin_p, lengths_p, counts_p, table_p, B, S, heads, G, D, 2 * half,
+                                                      int(halves), int(qk_norm), eps, page, n, width, positions, _dt(proj)))
     return q
+
+
+_INT_MAX = 2 ** 31 - 1
 
 
 @functools.lru_cache(maxsize=4096)
@@ -687,15 +688,17 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale, counts=Non
     if out is not None and (out.shape != (B, S, Hq, D) or out.dtype != q.dtype):
         raise ValueError(f"out must be {(B, S, Hq, D)} in the dtype of the queries")
     device, (q_p, k_p, v_p, table_p, lengths_p, counts_p, out_p) = _pointers(q, k_pages, v_pages, block_table, lengths, counts, out)
-    with _on(device):
-        if out is None:
-            out = torch.empty((B, S, Hq, D), dtype=q.dtype, device=q.device)
-            out_p = out.data_ptr()
-        # not kept between calls: two captured graphs, or two streams, never share it
-        size = _paged_ws_bytes(device, B, S, Hq, G, D, page, width)
-        ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-        ffi.check(ffi.lib().mynn_b200_paged_attention(_stream(), out_p, q_p, k_p, v_p, table_p, lengths_p, counts_p, scale, softcap, min(window, 2**31 - 1), min(sinks, 2**31 - 1), B, S, Hq, G, D, page, n,
-                                                      width, _dt(q), ws.data_ptr() if size else None, size))
+    if _elsewhere(device) and torch.cuda.current_device() != device:
+        with torch.cuda.device(device):
+            return paged_attention(q, k_pages, v_pages, block_table, lengths, scale, counts, window, sinks, softcap, out)
+    if out is None:
+        out = torch.empty_strided((B, S, Hq, D), (S * Hq * D, Hq * D, D, 1), dtype=q.dtype, device=q.device)
+        out_p = out.data_ptr()
+    # not kept between calls: two captured graphs, or two streams, never share it
+    size = _paged_ws_bytes(device, B, S, Hq, G, D, page, width)
+    ws = torch.empty_strided((size,), (1,), dtype=torch.uint8, device=q.device) if size else None
+    ffi.check(ffi.lib().mynn_b200_paged_attention(_stream(), out_p, q_p, k_p, v_p, table_p, lengths_p, counts_p, scale, softcap, min(window, _INT_MAX), min(sinks, _INT_MAX),
+                                                  B, S, Hq, G, D, page, n, width, _dt(q), ws.data_ptr() if size else None, size))
     return out
 
 
@@ -716,9 +719,10 @@ def verify_draft(target, tokens, accept, sample, draft=None, counts=None):
     if accept.dtype != torch.float32 or accept.shape != (B, K) or sample.dtype != torch.float32 or sample.shape != (B,):
         raise ValueError(f"accept and sample must be f32 tensors of shapes {(B, K)} and {(B,)}")
     device, (target_p, tokens_p, accept_p, sample_p, draft_p, counts_p) = _pointers(target, tokens, accept, sample, draft, counts)
-    with _on(device):
-        out = torch.empty((B, K1), dtype=torch.int32, device=target.device)
-        taken = torch.empty((B,), dtype=torch.int32, device=target.device)
-        ffi.check(ffi.lib().mynn_b200_verify_draft(_stream(), out.data_ptr(), taken.data_ptr(), target_p, draft_p, tokens_p, counts_p, accept_p, sample_p, B, K, V,
-                                                   _dt(target)))
+    if _elsewhere(device) and torch.cuda.current_device() != device:
+        with torch.cuda.device(device):
+            return verify_draft(target, tokens, accept, sample, draft, counts)
+    out = torch.empty_strided((B, K1), (K1, 1), dtype=torch.int32, device=target.device)
+    taken = torch.empty_strided((B,), (1,), dtype=torch.int32, device=target.device)
+    ffi.check(ffi.lib().mynn_b200_verify_draft(_stream(), out.data_ptr(), taken.data_ptr(), target_p, draft_p, tokens_p, counts_p, accept_p, sample_p, B, K, V, _dt(target)))
     return out, taken
