@@ -5,7 +5,8 @@
 // the rotated half and its partner half a rotated range away, or two neighbours; it does so for one head after the other, so a token's angles are read once per
 // thread, and a head's norm is a sum over the few threads that share it.  Other sizes (paged_append_any_kernel): a warp per head, staged in shared memory.
 // Bound by bytes for prompts and by the chain of lengths, table and store for a step: 32 tokens of 48 heads of 128 take 2.4 us (a warp per head: 6.7), 6 prompts of 777
-// places that are mostly padding, whose zero queries are 38 MB, 14 us (read before it was known that they are padding: 24).
+// places that are mostly padding, whose zero queries are 38 MB, 10.6 us (read before it was known that they are padding: 24), 2048 tokens 8.9 us = 0.86 of the copy
+// bandwidth.
 #include <algorithm>
 
 #include "common.cuh"
@@ -65,7 +66,7 @@ struct Piece {
 
 // grid (S, B); a group of `lanes` threads (a power of two) per head, thread i of it with pieces c0 and c1.  D a multiple of 16, rot_dims of 16 (halves) or 8.
 template <typename T>
-__global__ void __launch_bounds__(512) paged_append_kernel(const PagedAppend p, int lanes) {
+__global__ void __launch_bounds__(512, 2) paged_append_kernel(const PagedAppend p, int lanes) {
     pdl_trigger();
     pdl_wait();
     const int s = blockIdx.x, b = blockIdx.y, sub = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = blockDim.x / lanes;
@@ -235,7 +236,10 @@ extern "C" int mynn_b200_paged_rotary_append(void *stream, void *q_out, void *k_
     if (pieces) {
         int lanes = 1;
         while (lanes < D / 16) lanes *= 2;
-        const int threads = (int)std::min<long long>(512, ((long long)(Hq + 2 * Hkv) * lanes + 31) / 32 * 32);
+        // A step wants each head to begin at once, prompts want many CTAs side by side, since each begins with a chain of loads.  48 heads of 128, bf16, with 64 / 128 / 192 / 512
+        // threads: 32 tokens 4.2 / 3.0 / 2.6 / 2.5 us, 512 tokens 6.2 / 5.3 / 4.4 / 4.9, 2048 tokens 9.2 / 8.9 / 10.0 / 15.0, 4662 places that are mostly padding 16 / 12.0 / 10.6 / 14.0.
+        const long long tokens = (long long)B * S;
+        const int threads = (int)std::min<long long>(tokens < 300 ? 512 : tokens < 1024 || counts ? 192 : 128, ((long long)(Hq + 2 * Hkv) * lanes + 31) / 32 * 32);
         MYNN_DISPATCH_DTYPE(dtype, T, { MYNN_CUDA_OK(launch_dependent(paged_append_kernel<T>, dim3(S, B), dim3(threads), 0, st, p, lanes)); });
         MYNN_LAUNCH_OK("paged_append_kernel");
         return MYNN_OK;
