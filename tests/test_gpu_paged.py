@@ -1,5 +1,6 @@
 """Paged caches and drafted tokens against plain restatements in 64 bits (numpy, one sequence at a time)."""
 import itertools
+import threading
 
 import numpy as np
 import pytest
@@ -523,6 +524,44 @@ def test_calls_on_two_streams_and_repeated_calls_give_the_same_bits():
                 results.append(ops.paged_attention(q, k, v, table, n, 0.1))
         torch.cuda.synchronize()
         assert all(torch.equal(r, want) for r in results)
+
+
+def test_a_first_call_inside_a_capture():
+    """Kernels, limits and sizes that no call before has asked for."""
+    for dt, D, H, G, S in ((torch.float16, 192, 8, 2, 3), (torch.float32, 96, 2, 2, 1), (torch.bfloat16, 64, 8, 1, 7)):
+        k = torch.randn(40, G, 16, D, device="cuda", dtype=dt)
+        table = torch.full((2, 120), -1, dtype=torch.int32, device="cuda")
+        table[:, :20] = torch.arange(40, dtype=torch.int32, device="cuda").view(2, 20)
+        q, n = torch.randn(2, H, S, D, device="cuda", dtype=dt), torch.tensor([300, 41], dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = ops.paged_attention(q, k, k, table, n, 0.1)
+        g.replay()
+        assert torch.equal(out, ops.paged_attention(q, k, k, table, n, 0.1))
+        del g
+
+
+def test_calls_from_several_threads():
+    rng = np.random.default_rng(14)
+    k, v, table = cache(rng, [1500, 3, 800], 2, 64, 16, "bf16")
+    q, n = torch.from_numpy(rng.standard_normal((3, 8, 1, 64))).to("cuda", torch.bfloat16), torch.tensor([1500, 3, 800], dtype=torch.int32, device="cuda")
+    want = ops.paged_attention(q, k, v, table, n, 0.1)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                if not torch.equal(ops.paged_attention(q, k, v, table, n, 0.1), want):
+                    wrong.append(1)
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 # ---- refusals ------------------------------------------------------------------------------------------------------------
