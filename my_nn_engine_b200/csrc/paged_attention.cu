@@ -17,8 +17,8 @@ constexpr int kPlainTile = 8;
 // ---- any sizes ----------------------------------------------------------------------------------------------------------
 // f32 caches, heads that are no multiple of 8 numbers, unaligned tensors.  Each warp takes tiles of 8 positions into shared memory as f32; in the first product
 // a lane has one key and a quarter of the dimensions, in the second the dimensions lane, lane + 32, ...  Small tiles leave room for many warps, which hide each other's
-// chains: with tiles of 16 and half the warps 64 sequences of 1000, 8 heads of 128, took 192 us, now 166 = 0.49 of the copy bandwidth.  f32 has no tensor-core
-// form that keeps 24 bits, so the instructions around the 2 RB D multiplications of a position bound it: about 1000 per tile of 8 at four rows.
+// chains: with tiles of 16 and half the warps 64 sequences of 1000, 8 heads of 128, took 192 us, with every lane of a key going on with all rows 166, now 127 = 0.64 of the
+// copy bandwidth.  f32 has no tensor-core form that keeps 24 bits, so the instructions around the 2 RB D multiplications of a position bound it.
 // RB: query rows of a CTA (one head per kv head: with eight rows where one is needed 7 sequences of 1 to 1501, 12 heads of 80, took 46 us).
 // VEC: elements of a copy to shared memory (cp.async, f32); 0: 16-bit elements, converted on the way.
 template <int DL>
@@ -51,6 +51,9 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32, PlainShape<DL, RB>::CTAS
     float *sums = sm + RB * PITCH + W * (Shape::RING + Shape::WEIGHTS);
     for (int i = threadIdx.x; i < RB * PITCH; i += W * 32) sq[i] = 0.f;
     for (int i = lane; i < Shape::RING; i += 32) ring[i] = 0.f;  // what lies behind D is never written again
+    constexpr bool SPREAD = RB >= 4;
+    constexpr int OWN = SPREAD ? RB / 4 : RB;
+    const int own = SPREAD ? side * OWN : 0;  // the first row that this lane goes on with
     auto place = [&](int b, int h, int r, int d) {
         const int head = p.by_S.div(r);
         return (((size_t)b * p.S + p.by_S.mod(r, head)) * p.Hq + h * p.group + head) * D + d;
@@ -114,13 +117,14 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32, PlainShape<DL, RB>::CTAS
             sq[i / D * PITCH + i % D] = to_f32<T>(reinterpret_cast<const T *>(p.q)[(((size_t)b * p.Hq + h * p.group + head) * p.S + p.by_S.mod(r, head)) * D + i % D]);
         }
         __syncthreads();
-        float m[RB], l[RB], o[RB][DL];
+        // The sums of four and more rows are dealt out to the four lanes of a key, each of which goes on with a quarter of the rows; of fewer every lane has all.
+        float m[OWN], l[OWN], o[RB][DL];
 #pragma unroll
-        for (int r = 0; r < RB; r++) {
-            m[r] = -INFINITY, l[r] = 0.f;
+        for (int r = 0; r < OWN; r++) m[r] = -INFINITY, l[r] = 0.f;
+#pragma unroll
+        for (int r = 0; r < RB; r++)
 #pragma unroll
             for (int i = 0; i < DL; i++) o[r][i] = 0.f;
-        }
         for (int t = t0 + warp, stage = 0; t < t1; t += W, stage ^= 1) {
             const int after = row_of(t + 2 * W);
             if (t + W < t1) {
@@ -143,33 +147,52 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32, PlainShape<DL, RB>::CTAS
                 }
             }
             const int j = sp.at(t) * TILE + key;
+            float z[OWN];
+            if constexpr (SPREAD) {
+                float y[RB / 2];
+#pragma unroll
+                for (int r = 0; r < RB / 2; r++) y[r] = (side & 2 ? x[r + RB / 2] : x[r]) + __shfl_xor_sync(0xffffffffu, side & 2 ? x[r] : x[r + RB / 2], 16);
+#pragma unroll
+                for (int r = 0; r < OWN; r++) z[r] = (side & 1 ? y[r + OWN] : y[r]) + __shfl_xor_sync(0xffffffffu, side & 1 ? y[r] : y[r + OWN], 8);
+            } else {
+#pragma unroll
+                for (int r = 0; r < OWN; r++) {
+                    z[r] = x[r] + __shfl_xor_sync(0xffffffffu, x[r], 8);
+                    z[r] += __shfl_xor_sync(0xffffffffu, z[r], 16);
+                }
+            }
             bool moved = false;
 #pragma unroll
-            for (int r = 0; r < RB; r++) {
-                x[r] += __shfl_xor_sync(0xffffffffu, x[r], 8);
-                x[r] += __shfl_xor_sync(0xffffffffu, x[r], 16);
-                x[r] *= p.scale;
-                if (p.softcap > 0.f) x[r] = p.softcap * tanhf(x[r] / p.softcap);
-                if (r >= rows || row < 0 || (p.S > 1 && !paged_sees(p, sp, p.by_S.mod(r0 + r, p.by_S.div(r0 + r)), j))) x[r] = -INFINITY;  // (one query sees what there is)
-                moved |= x[r] > m[r];
+            for (int r = 0; r < OWN; r++) {
+                const int i = own + r;
+                z[r] *= p.scale;
+                if (p.softcap > 0.f) z[r] = p.softcap * tanhf(z[r] / p.softcap);
+                if (i >= rows || row < 0 || (p.S > 1 && !paged_sees(p, sp, p.by_S.mod(r0 + i, p.by_S.div(r0 + i)), j))) z[r] = -INFINITY;  // (one query sees what there is)
+                moved |= z[r] > m[r];
             }
             if (__any_sync(0xffffffffu, moved)) {  // most tiles raise no maximum
+                float keep[OWN];
 #pragma unroll
-                for (int r = 0; r < RB; r++) {
-                    float top = x[r];
+                for (int r = 0; r < OWN; r++) {
+                    float top = z[r];
 #pragma unroll
                     for (int s = 4; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-                    const float now = fmaxf(m[r], top), keep = expf(m[r] - merge_reference(now));
+                    const float now = fmaxf(m[r], top);
+                    keep[r] = expf(m[r] - merge_reference(now));
                     m[r] = now;
-                    l[r] *= keep;
+                    l[r] *= keep[r];
+                }
 #pragma unroll
-                    for (int i = 0; i < DL; i++) o[r][i] *= keep;
+                for (int r = 0; r < RB; r++) {
+                    const float f = SPREAD ? __shfl_sync(0xffffffffu, keep[r % OWN], r / OWN * 8) : keep[r % OWN];
+#pragma unroll
+                    for (int i = 0; i < DL; i++) o[r][i] *= f;
                 }
             }
 #pragma unroll
-            for (int r = 0; r < RB; r++) {
-                const float w = expf(x[r] - merge_reference(m[r]));
-                if (side == 0) l[r] += w, weights[key * WR + r] = w;
+            for (int r = 0; r < OWN; r++) {
+                const float w = expf(z[r] - merge_reference(m[r]));
+                if (SPREAD || side == 0) l[r] += w, weights[key * WR + own + r] = w;
             }
             __syncwarp();
             const bool full = p.S == 1 || paged_tile_full(p, sp, sp.at(t) * TILE, TILE);
@@ -199,12 +222,15 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32, PlainShape<DL, RB>::CTAS
         }
         // the warps' parts meet
 #pragma unroll
-        for (int r = 0; r < RB; r++) {
-            l[r] = warp_sum(l[r]);
-            if (lane == 0) part_m[warp][r] = m[r], part_l[warp][r] = l[r];
+        for (int r = 0; r < OWN; r++) {
+#pragma unroll
+            for (int s = 4; s > 0; s >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], s);
+            if (key == 0 && (SPREAD || side == 0)) part_m[warp][own + r] = m[r], part_l[warp][own + r] = l[r];
+        }
+#pragma unroll
+        for (int r = 0; r < RB; r++)
 #pragma unroll
             for (int i = 0; i < DL; i++) sums[warp * Shape::SUMS + r * DL * 32 + lane + 32 * i] = o[r][i];
-        }
         __syncthreads();
         const bool whole = t0 == 0 && t1 == sp.tiles;
         float *part = p.ws + (((size_t)blockIdx.y * ctas + cta) * 2 + (run.first ? 0 : 1)) * p.part_floats;
