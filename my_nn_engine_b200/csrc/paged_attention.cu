@@ -51,6 +51,7 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32, PlainShape<DL, RB>::CTAS
     float *sums = sm + RB * PITCH + W * (Shape::RING + Shape::WEIGHTS);
     for (int i = threadIdx.x; i < RB * PITCH; i += W * 32) sq[i] = 0.f;
     for (int i = lane; i < Shape::RING; i += 32) ring[i] = 0.f;  // what lies behind D is never written again
+    __syncwarp();  // other lanes copy to these places, and of a table that is left whole no barrier comes before
     constexpr bool SPREAD = RB >= 4;
     constexpr int OWN = SPREAD ? RB / 4 : RB;
     const int own = SPREAD ? side * OWN : 0;  // the first row that this lane goes on with

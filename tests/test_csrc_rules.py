@@ -32,3 +32,10 @@ def test_local_arrays_are_aligned_for_the_pieces_they_are_accessed_in():
             declared = list(re.finditer(r"^.*?\b%s(\[|\b)[^;\n]*" % m.group(1), text[:m.start()], re.M))
             arrays = [d.group(0).strip() for d in declared if re.match(r"\s*(?:__align__\(\d+\) )?%s (?:\w+\[\w+\], )*%s\[" % (element, m.group(1)), d.group(0))]
             assert not arrays or arrays[-1].startswith("__align__"), (name, arrays[-1])
+
+
+def test_a_ring_is_cleared_before_other_lanes_copy_to_it():
+    """Paged attention for any sizes: a warp clears its ring lane by lane, and what brings the first rows writes the same places from other lanes.  Of a table that is
+    left whole paged_find() returns without a barrier, so one stands behind the loop."""
+    text = dict(sources())["paged_attention.cu"]
+    assert re.search(r"ring\[i\] = 0\.f;\s*__syncwarp\(\);", text)
