@@ -263,8 +263,8 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32, PlainShape<DL, RB>::CTAS
 // shared memory whose entries are the keys or the values of a tile, each warp a share of the rows, and each warp then multiplies the whole tile with query rows of its
 // own, eight or NT times eight, so that a row of the cache is read once for up to 64 query rows (all heads of a group, all drafts).  Both products are mma.m16n8k16 on
 // fragments that are whole 8 x 8 blocks from ldmatrix, without a byte moved: S^T = K Q^T, eight query rows as columns, and O^T = V^T P^T, whose second operand is
-// the first product's result behind a transposition of its 8 x 8 blocks.  Weights enter as a 16-bit part and its remainder (16 bits in all); scores, maxima and
-// sums are f32.  The reference of the weights is moved only when a score exceeds it by 2^8, so most tiles need no maximum across lanes and no rescaling.  D is padded
+// the first product's result behind a transposition of its 8 x 8 blocks.  Weights enter as a 16-bit part and its remainder (16 bits in all, kTop says how f16 keeps them); scores, maxima and
+// sums are f32.  The reference of the weights is moved only when a score exceeds it by 2^kLag, so most tiles need no maximum across lanes and no rescaling.  D is padded
 // to DP with zeros, on the chip only.
 // The chain of one tile is long (two products, a softmax) and each warp walks it alone, so warps are what hides it: sixteen per SM with eight query rows each (with eight
 // warps of sixteen rows 96 mixed sequences of heads of 64 took a fifth longer).  From 17 rows on the instructions bound it, and sixteen rows of a warp share the blocks
@@ -309,14 +309,26 @@ __device__ __forceinline__ uint32_t special_mask(uint32_t x) {  // all ones over
     return ((x & e) == e ? 0xffffu : 0u) | ((x >> 16 & e) == e ? 0xffff0000u : 0u);
 }
 
+// Weights of the second product are 2^(x - m + kTop), m lagging behind the largest score by up to kLag, and two 16-bit parts hold them.  bf16 has the range of f32.  Both parts
+// of an f16 number end at 2^-24: with the largest weight near the other end of its range, 2^15, 16 bits are left of one 2^22 times as small as that of m (2^-9).  Where a lane has
+// none as large, the tile is multiplied with weights that are 2^up times as large, its own largest near 2^15, by sums that are brought there and back, powers of two that change no
+// bit.  So behind a key that leads by any number of nats, and whose value may be zero, the others keep 16 bits; those that share its tile are right to 2^-38 of
+// the largest.  Tiles that are all so small take longer: behind a first key that leads by 20 nats 131071 positions, 8 kv heads of 128, 123 us instead of 112 (32 sequences of 2048
+// 71 instead of 64; cold caches).  The check itself costs nothing with eight rows of a warp, 1 to 5 % with sixteen (20 rows of 64 numbers over 60000 positions 55 us without).
+template <typename T>
+constexpr int kTop = std::is_same<T, __half>::value ? 13 : 0;
+template <typename T>
+constexpr int kLag = std::is_same<T, __half>::value ? 2 : 8;
+
 template <typename T, int DP, int RW, int NT>
 __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attention_mma_kernel(const PagedAttention p) {
     using Shape = MmaShape<DP, RW, NT>;
     constexpr bool JOINT = Shape::JOINT;
     constexpr int W = Shape::W, TEAMS = Shape::TEAMS, STAGES = Shape::STAGES, AHEAD = Shape::AHEAD, TILE = Shape::TILE, KT = TILE / 16, KS = DP / 16, CPR = DP / 8;
+    constexpr bool NARROW = kTop<T> != 0;
     constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
     extern __shared__ __align__(128) uint8_t raw[];
-    __shared__ float part_m[W][8 * NT], part_l[W][8 * NT];
+    __shared__ float part_m[W][8 * NT], part_l[W][8 * NT], to_reference[W][8 * NT];
     pdl_trigger();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, team = warp / RW;
@@ -523,7 +535,7 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
 #pragma unroll
         for (int n = 0; n < NT; n++) {
 #pragma unroll
-            for (int e = 0; e < 2; e++) m[n][e] = limit[n][e] = -INFINITY, ref[n][e] = l[n][e] = 0.f;
+            for (int e = 0; e < 2; e++) m[n][e] = limit[n][e] = -INFINITY, ref[n][e] = -kTop<T>, l[n][e] = 0.f;
 #pragma unroll
             for (int i = 0; i < KS; i++)
 #pragma unroll
@@ -546,6 +558,7 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
             else step_on();
             // ---- S^T = K Q^T: x[n][k][2 c + e] is position base + 16 k + g + 8 c, row 8 n + 2 t + e ----
             uint32_t hi[NT][KT][2], lo[NT][KT][2];
+            unsigned small = 0;  // bit n: the tile is multiplied by itself for rows 8 n .. 8 n + 7, and then brought to the reference by to_reference
             const bool full = exist[0] == ALL && (p.S == 1 || paged_tile_full(p, sp, base, TILE));
             auto scores = [&](auto groups) {
                 constexpr int N = decltype(groups)::value;
@@ -594,7 +607,9 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
                     for (int k = 0; k < KT; k++)
 #pragma unroll
                         for (int i = 0; i < 4; i++) most[i & 1] = fmaxf(most[i & 1], x[n][k][i]);
-                    if (__any_sync(0xffffffffu, most[0] > limit[n][0] || most[1] > limit[n][1])) {
+                    auto below = [&](int e) { return NARROW && most[e] < ref[n][e] - 9.f && most[e] > -INFINITY && ref[n][e] < INFINITY; };
+                    if (__any_sync(0xffffffffu, most[0] > limit[n][0] || most[1] > limit[n][1] || below(0) || below(1))) {
+                        float tops[2];
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
                             float top = most[e];
@@ -602,25 +617,41 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
                             for (int s = 4; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
                             const float now = fmaxf(m[n][e], top), keep = exp2_approx(m[n][e] - merge_reference(now));
                             m[n][e] = now;
-                            ref[n][e] = merge_reference(now);
-                            limit[n][e] = now + 8.f;
+                            ref[n][e] = merge_reference(now) - kTop<T>;
+                            limit[n][e] = now + kLag<T>;
+                            tops[e] = top;
                             l[n][e] *= keep;
 #pragma unroll
                             for (int i = 0; i < KS; i++) o[n][i][e] *= keep, o[n][i][2 + e] *= keep;
                         }
+                        if (NARROW && __any_sync(0xffffffffu, below(0) || below(1))) {
+                            small |= 1u << n;
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                // brings the tile's largest weight to 2^14 .. 2^15 (or 2^60 times nearer: the sums have to stay numbers)
+                                const float up = tops[e] > -INFINITY && ref[n][e] < INFINITY ? fminf(floorf(ref[n][e] + 15.f - tops[e]), 60.f) : 0.f;
+#pragma unroll
+                                for (int k = 0; k < KT; k++) x[n][k][e] += up, x[n][k][2 + e] += up;
+                                if (g == 0) to_reference[warp][8 * n + 2 * t + e] = __int_as_float((127 - (int)up) << 23);  // 2^-up
+                            }
+                            __syncwarp();
+                        }
                     }
+                    float mass[2] = {0.f, 0.f};  // of this lane's positions
 #pragma unroll
                     for (int k = 0; k < KT; k++) {
 #pragma unroll
                         for (int i = 0; i < 4; i++) x[n][k][i] = exp2_approx(x[n][k][i] - ref[n][i & 1]);
-                        l[n][0] += x[n][k][0] + x[n][k][2];  // of this lane's positions
-                        l[n][1] += x[n][k][1] + x[n][k][3];
+                        mass[0] += x[n][k][0] + x[n][k][2];
+                        mass[1] += x[n][k][1] + x[n][k][3];
 #pragma unroll
                         for (int c = 0; c < 2; c++) {
                             split_pack<T>(x[n][k][2 * c], x[n][k][2 * c + 1], hi[n][k][c], lo[n][k][c]);
                             hi[n][k][c] = transpose_8x8(hi[n][k][c]), lo[n][k][c] = transpose_8x8(lo[n][k][c]);  // positions 16 k + 8 c + 2 t, + 1 of row 8 n + g
                         }
                     }
+                    if (NARROW && (small >> n & 1)) mass[0] *= to_reference[warp][8 * n + 2 * t], mass[1] *= to_reference[warp][8 * n + 2 * t + 1];
+                    l[n][0] += mass[0], l[n][1] += mass[1];
                 }
             };
             if (more_rows) scores(std::integral_constant<int, NT>());
@@ -644,26 +675,37 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
                 }
                 odd = __any_sync(0xffffffffu, odd);
             }
-            auto values = [&](auto groups, auto special) {
+            auto values = [&](auto groups, auto rare) {
                 constexpr int N = decltype(groups)::value;
+                const bool special = !NARROW || odd;
 #pragma unroll
-                for (int i = 0; i < KS; i++)
+                for (int i = 0; i < KS; i++) {
+                    if constexpr (NARROW && decltype(rare)::value) {
+#pragma unroll
+                        for (int n = 0; n < N; n++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                if (small >> n & 1) o[n][i][e] *= __int_as_float((254 << 23) - __float_as_int(to_reference[warp][8 * n + 2 * t + (e & 1)]));  // 2^up
+                    }
 #pragma unroll
                     for (int k = 0; k < KT; k++) {
                         uint32_t a[4], c[4];
                         ldsm4t_at(a, (V ^ (i & 3) << 5) + (i >> 2) * 128 + k * 16 * DP * 2);
-                        if constexpr (decltype(special)::value) {
+                        if constexpr (decltype(rare)::value) {
 #pragma unroll
-                            for (int q = 0; q < 4; q++) c[q] = a[q] & special_mask<T>(a[q]), a[q] &= ~special_mask<T>(a[q]);
+                            for (int q = 0; q < 4; q++) {
+                                if (special) c[q] = a[q] & special_mask<T>(a[q]), a[q] &= ~special_mask<T>(a[q]);
+                                else c[q] = 0u;
+                            }
                         }
 #pragma unroll
                         for (int n = 0; n < N; n++) {
                             mma_kv<T>(o[n][i], a[0], a[1], a[2], a[3], hi[n][k][0], hi[n][k][1]);
                             mma_kv<T>(o[n][i], a[0], a[1], a[2], a[3], lo[n][k][0], lo[n][k][1]);
                         }
-                        if constexpr (decltype(special)::value) {
+                        if constexpr (decltype(rare)::value) {
 #pragma unroll 1
-                            for (int q = 0; q < 16; q++) {
+                            for (int q = special ? 0 : 16; q < 16; q++) {
                                 const uint32_t one = (q & 7) >> 1 == t ? (q & 1 ? 0xffff0000u : 0xffffu) : 0u, first = q < 8 ? one : 0u, second = q < 8 ? 0u : one;
 #pragma unroll
                                 for (int n = 0; n < N; n++) {
@@ -676,9 +718,17 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
                             }
                         }
                     }
+                    if constexpr (NARROW && decltype(rare)::value) {
+#pragma unroll
+                        for (int n = 0; n < N; n++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                if (small >> n & 1) o[n][i][e] *= to_reference[warp][8 * n + 2 * t + (e & 1)];
+                    }
+                }
             };
             // Values that are no numbers are taken out of the product and added position by position where they are seen, so that the other rows keep their bits.
-            if (!odd) {
+            if (!odd && small == 0) {
                 if (more_rows) values(std::integral_constant<int, NT>(), std::false_type());
                 else if (busy) values(std::integral_constant<int, 1>(), std::false_type());
             } else {
