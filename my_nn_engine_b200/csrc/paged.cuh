@@ -42,7 +42,7 @@ struct PagedAttention {
     FixedDivisor by_page, by_S, by_pieces;  // by_pieces: copies of a row, of the kernel for any sizes
     int row_blocks, block_rows;  // the group * S query rows of a pair, row r = head * S + s, in blocks
     int tile, round, toll;             // shares are multiples of `round`, the tiles that the warps of a CTA take at a time; toll: see PagedRun
-    int4 *records;               // per CTA the pair that begins in it and ends in another: {b, h, last CTA, slot}, or b == -1
+    int4 *records;               // per CTA the pair that begins in it and ends in another: {b, h, last CTA, slot}, or b == -1; null: no pair can end elsewhere
     float *ws;                   // [row block][CTA][2] parts of part_floats floats: block_rows rows of D, then maxima, then sums
     int part_floats;             // a multiple of 4
     int whole;                   // each pair is left to a CTA of its own

@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32, PlainShape<DL, RB>::CTAS
             }
         }
     }
-    if (blockIdx.y == 0 && threadIdx.x == 0 && !p.whole) p.records[cta] = run.record;
+    if (blockIdx.y == 0 && threadIdx.x == 0 && p.records) p.records[cta] = run.record;
 }
 
 // ---- 16-bit caches on the tensor cores --------------------------------------------------------------------------------
@@ -752,7 +752,7 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
         part = p.ws + (((size_t)blockIdx.y * ctas + cta) * 2 + (run.first ? 0 : 1)) * p.part_floats;
         run.advance(p);
     }
-    if (blockIdx.y == 0 && threadIdx.x == 0 && !p.whole) p.records[cta] = run.record;
+    if (blockIdx.y == 0 && threadIdx.x == 0 && p.records) p.records[cta] = run.record;
 }
 
 // ---- parts of pairs that lie in several CTAs ------------------------------------------------------------------------------
@@ -849,7 +849,8 @@ struct PagedPlan {
     int dim, team, groups;  // padded head dimension, warps of a team, groups of eight rows of a warp
     int ctas, block_rows, row_blocks, round;
     bool whole;
-    size_t bytes(int D) const { return whole ? 0 : (size_t)ctas * sizeof(int4) + (size_t)ctas * row_blocks * 2 * part_floats(D) * sizeof(float); }
+    bool cut() const { return !whole && ctas > 1; }  // are there parts to join?
+    size_t bytes(int D) const { return !cut() ? 0 : (size_t)ctas * sizeof(int4) + (size_t)ctas * row_blocks * 2 * part_floats(D) * sizeof(float); }
     int part_floats(int D) const { return (block_rows * (D + 2) + 3) / 4 * 4; }  // 16-byte pieces of them are read
 };
 
@@ -908,7 +909,17 @@ static PagedPlan paged_plan(int B, int S, int Hq, int Hkv, int D, int page, int 
     // Tables of so many positions: pairs are not cut, and no second kernel follows.  One sequence, 8 kv heads of 128, 16 bits: 500 positions 8.0 us whole, 10.6 cut, 1000
     // 11.1 and 11.8; in f32 100 positions 10 us whole, 12 cut, 300 19 and 12.
     n.whole = (long long)width * page <= (mma ? 1024 : 256);
-    n.ctas = n.whole ? B * Hkv : (int)std::min<long long>(most, std::max<long long>(1, (tiles * Hkv * B + n.round - 1) / n.round));
+    // Every block of rows has as many CTAs, all of them together some full waves: one, or as few up to four as leave the least of the GPU idle.  So the parts stay below eight per resident
+    // CTA, 80 MB, whatever the number of rows (a wave per block: 480 MB
+    // for 777 tokens of 4 heads of 128), and pairs are not cut finer than that takes: 6 prompts of 777 tokens 1438 us with a wave per block, 868 so; f32, 8 tokens of 8 heads of 64 over 3000 positions 108 and 68.
+    long long per_block = 1;
+    double busy = 0.0;
+    for (int waves = 1; waves <= 4 && busy < 0.95; waves++) {
+        const long long c = waves * most / n.row_blocks;
+        const double share = (double)(c * n.row_blocks) / (double)(waves * most);
+        if (c > 0 && share > busy + 0.02) per_block = c, busy = share;
+    }
+    n.ctas = n.whole ? B * Hkv : (int)std::min<long long>(per_block, std::max<long long>(1, (tiles * Hkv * B + n.round - 1) / n.round));
     return n;
 }
 
@@ -1018,8 +1029,8 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
     // 131071 95, 95, 95, 97); f32, 7 of 1 to 1501: 120 with none, 65 with one round of the warps, 64 with two, 72 with four.
     p.toll = n.mma ? 256 / n.tile : 2 * n.round;
     p.strips = n.mma && page % 8 == 0 && D == n.dim;
-    p.records = reinterpret_cast<int4 *>(workspace);
-    p.ws = reinterpret_cast<float *>(p.records + (n.whole ? 0 : n.ctas));
+    p.records = n.cut() ? reinterpret_cast<int4 *>(workspace) : nullptr;
+    p.ws = n.cut() ? reinterpret_cast<float *>(p.records + n.ctas) : nullptr;
     const cudaStream_t st = (cudaStream_t)stream;
     MYNN_DISPATCH_DTYPE(dtype, T, {
         int e = MYNN_OK;
@@ -1031,7 +1042,7 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
         else if (D <= 128) e = launch_plain_rows<T, 4>(st, p, n.ctas, vec);
         else e = launch_plain_rows<T, 8>(st, p, n.ctas, vec);
         if (e != MYNN_OK) return e;
-        if (n.whole) return MYNN_OK;
+        if (!n.cut()) return MYNN_OK;
         const int R = p.group * S, rows = R == 1 ? 1 : R == 2 ? 2 : R <= 4 ? 4 : 8;
         const dim3 grid(n.ctas, (R + rows - 1) / rows), block(kJoinWarps * 32);
         if (D % 4 == 0) MYNN_CUDA_OK(launch_dependent(paged_attention_join_kernel<T, 4>, grid, block, 0, st, p, n.ctas, rows));

@@ -1,0 +1,32 @@
+"""Paged attention with many query rows per kv head: prompts and chunks of them, behind tables that pairs are cut for."""
+import pytest
+import torch
+
+from my_nn_engine_b200 import ffi
+from test_gpu_paged import run_attention
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("D", [40, 64, 128, 192, 256])
+@pytest.mark.parametrize("group", [1, 4, 8])
+def test_scratch_is_bounded_whatever_the_number_of_tokens(D, group):
+    """Eight parts of 64 rows of 256 numbers, their maxima and sums per CTA that is resident: 78.3 MB on 148 SMs."""
+    torch.cuda.init()
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    for S in (1, 5, 17, 100, 512, 777, 2048, 65536 // group):
+        n = ffi.lib().mynn_b200_paged_attention_workspace_bytes(6, S, 8 * group, 8, D, 16, 2000)
+        assert n <= sms * 8 * (64 * 258 * 4 + 16), (S, n)
+        assert S > 512 or n > 0
+
+
+@pytest.mark.parametrize("dt,D", [("bf16", 64), ("f16", 128), ("bf16", 192), ("f32", 64), ("f32", 20)])
+@pytest.mark.parametrize("H,G,S", [(4, 1, 50), (8, 1, 150), (6, 2, 333), (8, 1, 601)])
+def test_prompts(dt, D, H, G, S):
+    """4 to 76 blocks of 64 rows, 25 to 601 of eight: cut pairs, whole ones in fewer CTAs than blocks, several waves."""
+    run_attention(S + D, dt, [S + 1400, S, S // 2, 0], H, G, D, 16, S, [S, S - 1, S // 2, 0])
+
+
+def test_a_chunk_behind_a_window():
+    run_attention(5, "bf16", [2500, 700], 8, 2, 128, 24, 260, [260, 130], window=300, sinks=5)
+    run_attention(6, "f32", [1500, 300], 4, 2, 64, 24, 130, [130, 1], window=100, sinks=5)
