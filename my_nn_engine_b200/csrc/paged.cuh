@@ -17,8 +17,6 @@
 
 namespace mynn {
 
-constexpr int kPagedWindow = INT_MAX - (1 << 17);
-
 // Division of a number below 2^31 by a fixed one: (umulhi(n, mul) + n) >> shift with mul = floor(2^32 (2^shift - d) / d) + 1, 2^shift the next power of two.
 struct FixedDivisor {
     unsigned d = 1, mul = 1, shift = 0;
@@ -36,7 +34,7 @@ struct PagedAttention {
     const void *q, *k, *v;
     const int32_t *table, *lengths, *counts;  // counts null: S each
     float scale, softcap;
-    int window, sinks;  // window: at most kPagedWindow (positions are below 2^31, and new tokens may lie before the first one)
+    int window, sinks;
     int B, S, Hq, G, group, D;
     int page, pages, width;  // rows of a page, pages of the cache, pages in a row of the table
     FixedDivisor by_page, by_S, by_pieces;  // by_pieces: copies of a row, of the kernel for any sizes
@@ -64,7 +62,7 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttention &p, int b) 
     const int oldest = s.len - s.count;
     const int shift = p.tile == 8 ? 3 : p.tile == 16 ? 4 : 5, up = p.tile - 1;
     const int all = (s.rows + up) >> shift;
-    const int lo = p.window > 0 ? min(max(0, oldest - p.window + 1) >> shift, all) : 0;  // the tile that the windows begin in
+    const int lo = p.window > 0 ? min(max(0, max(oldest, 0) - p.window + 1) >> shift, all) : 0;  // the tile that the windows begin in (new tokens may lie before position 0)
     s.sink_tiles = min((min(p.sinks, s.rows) + up) >> shift, lo);
     s.skip = lo - s.sink_tiles;
     s.tiles = s.count > 0 ? all - s.skip : 0;

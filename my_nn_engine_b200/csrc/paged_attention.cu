@@ -382,8 +382,10 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
         auto base_of = [&](int j) { return sp.at(t0 + team + TEAMS * j) * TILE; };
         // The first row of eight positions whose rows lie one behind the other and are all seen, for 32 such strips at once, one per lane; -1 for others.
         auto strips_of = [&](int i) {
-            const int j = i / STRIPS, pos = base_of(j) + i % STRIPS * 8;
-            if (j >= mine || !p.strips || pos + 8 > sp.rows || (p.window > 0 && oldest - pos >= p.window && pos + 8 > p.sinks)) return -1;
+            const int j = i / STRIPS;
+            if (j >= mine || !p.strips) return -1;
+            const int pos = base_of(j) + i % STRIPS * 8;
+            if (pos + 8 > sp.rows || (p.window > 0 && oldest - pos >= p.window && pos + 8 > p.sinks)) return -1;
             return paged_row(p, sp, b, h, pos);
         };
         auto row_of = [&](int j) { return j < mine ? paged_row(p, sp, b, h, base_of(j) + (lane & (TILE - 1))) : -1; };
@@ -1018,7 +1020,7 @@ extern "C" int mynn_b200_paged_attention(void *stream, void *out, const void *q,
     p.out = out, p.q = q;
     p.k = k_pages, p.v = v_pages;
     p.table = block_table, p.lengths = lengths, p.counts = counts;
-    p.scale = scale, p.softcap = softcap, p.window = std::min(window, kPagedWindow), p.sinks = sinks;
+    p.scale = scale, p.softcap = softcap, p.window = window, p.sinks = sinks;
     p.B = B, p.S = S, p.Hq = Hq, p.G = Hkv, p.group = Hq / Hkv, p.D = D;
     p.page = page, p.pages = pages, p.width = table_pages;
     p.by_page = FixedDivisor(page), p.by_S = FixedDivisor(S), p.by_pieces = FixedDivisor(dtype == MYNN_F32 ? D / vec : D);

@@ -2,8 +2,8 @@
 import pytest
 import torch
 
-from my_nn_engine_b200 import ffi
-from test_gpu_paged import run_attention
+from my_nn_engine_b200 import ffi, ops
+from test_gpu_paged import DT, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +30,18 @@ def test_prompts(dt, D, H, G, S):
 def test_a_chunk_behind_a_window():
     run_attention(5, "bf16", [2500, 700], 8, 2, 128, 24, 260, [260, 130], window=300, sinks=5)
     run_attention(6, "f32", [1500, 300], 4, 2, 64, 24, 130, [130, 1], window=100, sinks=5)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("S", [1, 3])
+def test_windows_of_nearly_all_positions_there_can_be(dt, S):
+    """The last position a length can have, over a table of 64: what is seen of it follows from the window to the position.  Both sides are rounded once, so they differ by a step at most."""
+    k, v = torch.randn(4, 2, 16, 64, device="cuda").to(DT[dt]), torch.randn(4, 2, 16, 64, device="cuda").to(DT[dt])
+    table, q = torch.arange(4, dtype=torch.int32, device="cuda").view(1, 4), torch.randn(1, 4, S, 64, device="cuda").to(DT[dt])
+    last = torch.tensor([2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    for first in (0, 1, 17, 50, 63):  # the first position that the oldest query sees
+        near = torch.tensor([64], dtype=torch.int32, device="cuda")
+        got = ops.paged_attention(q, k, v, table, last, 0.1, window=2 ** 31 - 1 - S - first + 1)
+        want = torch.cat([ops.paged_attention(q[:, :, s:s + 1].contiguous(), k, v, table, near, 0.1, window=64 - first - s) if first + s < 64 else torch.zeros_like(got[:, :1]) for s in range(S)], 1)
+        assert torch.allclose(got.float(), want.float(), rtol=2.0 ** -7 if dt == "bf16" else 1e-5, atol=1e-5) and got[:, 0].any()
+    assert torch.equal(ops.paged_attention(q, k, v, table, last, 0.1, window=2 ** 31 - 1), ops.paged_attention(q, k, v, table, last, 0.1))
