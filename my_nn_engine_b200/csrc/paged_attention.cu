@@ -356,7 +356,8 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
         if constexpr (RW == 1) __syncwarp();
         else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(RW * 32) : "memory");
     };
-    const float unit = p.scale * kLog2e;
+    // scores in units of ln 2, or of the cap
+    const float unit = p.softcap > 0.f ? p.scale / p.softcap : p.scale * kLog2e;
     PagedRun run;
     run.begin(paged_find<W * 32>(p, cta, ctas));
     PagedSpan sp;
@@ -590,11 +591,11 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
                             if (KT == 1 && N == 1) x[n][k][i] += y[n][k][i];
                             x[n][k][i] *= unit;
                         }
-                    if (p.softcap > 0.f) {
+                    if (p.softcap > 0.f) {  // (tanhf is right relative to itself: a cap far above the scores leaves them as they are; no slower than a form in e^x)
 #pragma unroll
                         for (int k = 0; k < KT; k++)
 #pragma unroll
-                            for (int i = 0; i < 4; i++) x[n][k][i] = kLog2e * fast_soft_cap(x[n][k][i] * kLn2, p.softcap);
+                            for (int i = 0; i < 4; i++) x[n][k][i] = kLog2e * (p.softcap * tanhf(x[n][k][i]));
                     }
                     if (!full) {
 #pragma unroll

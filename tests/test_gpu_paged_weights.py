@@ -98,3 +98,29 @@ def test_scores_that_are_far_apart(dt, H, G, D, S):
     weight = 2.0 ** -24 * (12 * A * np.sqrt(D) + 64) + (2.0 ** -16 if dt != "f32" else 0)
     bound = HALF[dt] * np.abs(want) + 2 * weight * mass + (2.0 ** -25 if dt == "f16" else 1e-30)
     assert (np.abs(got - want) <= bound).all(), (np.abs(got - want) / bound).max()
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("cap,spread", [(0.5, 4.0), (30.0, 20.0), (1e3, 30.0), (1e4, 30.0), (1e4, 6000.0), (1e30, 8.0), (1e-3, 8.0)])
+@pytest.mark.parametrize("D,H", [(64, 1), (128, 20)])
+def test_capped_weights_one_by_one(dt, cap, spread, D, H):
+    """Caps far from the scores and close to them.  A capped score is right to 2^-21 of itself (argument, hyperbolic tangent and product), which moves each weight and the sum by
+    as much; else as ``test_weights_one_by_one``."""
+    rng = np.random.default_rng(int(spread) + D)
+    n = 60
+    k, v, table = cache(rng, [n], 1, D, 16, dt)
+    k.zero_()
+    v.zero_()
+    step = 4.0 if spread > 1000 else 1 / 16  # scores that all types hold
+    x = np.round(rng.uniform(-spread, spread, n) / step) * step if spread < 1000 else 5632.0 + 32 * rng.integers(0, 3, n)
+    for j in range(n):
+        pg = int(table[0, j // 16])
+        k[pg, 0, j % 16, 0], v[pg, 0, j % 16, j % D] = x[j], 1.0
+    x = np.array([float(k[int(table[0, j // 16]), 0, j % 16, 0]) for j in range(n)])
+    q = torch.zeros(1, H, 1, D, device="cuda", dtype=DT[dt])
+    q[..., 0] = 1.0
+    got = host(ops.paged_attention(q, k, v, table, torch.tensor([n], dtype=torch.int32, device="cuda"), 1.0, softcap=cap))
+    want, _ = want_attention(q, k, v, table, [n], [1], 1.0, cap=float(np.float32(cap)))
+    score = np.abs(cap * np.tanh(x / cap)).max() * 2.0 ** -21
+    bound = (HALF[dt] + 64 * 2.0 ** -24 + (2.0 ** -16 if dt != "f32" else 0) + 2 * score) * want + (2.0 ** -25 if dt == "f16" else 0) + (2.0 ** -38 if dt != "f32" else 0)
+    assert (np.abs(got - want) <= bound).all(), (np.abs(got - want) / bound).max()
