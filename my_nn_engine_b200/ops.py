@@ -624,6 +624,14 @@ def _pointers(*tensors):
     return device, out
 
 
+_INT_MAX = 2 ** 31 - 1
+
+
+def _nearest_int(x):
+    """Of the numbers that a C int holds the nearest one: ctypes would drop the upper bits."""
+    return max(-_INT_MAX, min(x, _INT_MAX))
+
+
 def _elsewhere(device):
     """The operators of this section run on their tensors' device and its current stream: is another device current?"""
     return _device is None or device != _device()
@@ -634,6 +642,8 @@ def _pages(k_pages, v_pages, dtype, block_table, lengths, counts, batch):
     shape, table = k_pages.shape, block_table.shape
     if len(shape) != 4 or shape != v_pages.shape:
         raise ValueError(f"k_pages and v_pages must have one shape [pages, kv heads, page, D], not {tuple(shape)} and {tuple(v_pages.shape)}")
+    if shape[0] > _INT_MAX:
+        raise ValueError(f"{shape[0]} pages (at most {_INT_MAX})")
     if k_pages.dtype != dtype or v_pages.dtype != dtype:
         raise TypeError("the pages must have the dtype of the queries")
     if len(table) != 2 or table[0] != batch or block_table.dtype != torch.int32:
@@ -664,11 +674,8 @@ def paged_rotary_append(proj, lengths, block_table, k_pages, v_pages, heads, cos
             return paged_rotary_append(proj, lengths, block_table, k_pages, v_pages, heads, cos, sin, counts, halves, qk_norm, eps)
     q = torch.empty_strided((B, heads, S, D), (heads * S * D, S * D, D, 1), dtype=proj.dtype, device=proj.device)  # (half the time of torch.empty)
     ffi.check(ffi.lib().mynn_b200_paged_rotary_append(_stream(), q.data_ptr(), k_p, v_p, proj_p, cos_p, sin_p, lengths_p, counts_p, table_p, B, S, heads, G, D, 2 * half,
-                                                      int(halves), int(qk_norm), eps, page, n, width, positions, _dt(proj)))
+                                                      int(halves), int(qk_norm), eps, page, n, width, _nearest_int(positions), _dt(proj)))
     return q
-
-
-_INT_MAX = 2 ** 31 - 1
 
 
 @functools.lru_cache(maxsize=4096)
@@ -697,7 +704,7 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale, counts=Non
     # not kept between calls: two captured graphs, or two streams, never share it
     size = _paged_ws_bytes(device, B, S, Hq, G, D, page, width)
     ws = torch.empty_strided((size,), (1,), dtype=torch.uint8, device=q.device) if size else None
-    ffi.check(ffi.lib().mynn_b200_paged_attention(_stream(), out_p, q_p, k_p, v_p, table_p, lengths_p, counts_p, scale, softcap, min(window, _INT_MAX), min(sinks, _INT_MAX),
+    ffi.check(ffi.lib().mynn_b200_paged_attention(_stream(), out_p, q_p, k_p, v_p, table_p, lengths_p, counts_p, scale, softcap, _nearest_int(window), _nearest_int(sinks),
                                                   B, S, Hq, G, D, page, n, width, _dt(q), ws.data_ptr() if size else None, size))
     return out
 

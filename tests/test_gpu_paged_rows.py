@@ -45,3 +45,15 @@ def test_windows_of_nearly_all_positions_there_can_be(dt, S):
         want = torch.cat([ops.paged_attention(q[:, :, s:s + 1].contiguous(), k, v, table, near, 0.1, window=64 - first - s) if first + s < 64 else torch.zeros_like(got[:, :1]) for s in range(S)], 1)
         assert torch.allclose(got.float(), want.float(), rtol=2.0 ** -7 if dt == "bf16" else 1e-5, atol=1e-5) and got[:, 0].any()
     assert torch.equal(ops.paged_attention(q, k, v, table, last, 0.1, window=2 ** 31 - 1), ops.paged_attention(q, k, v, table, last, 0.1))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_windows_below_32_bits_are_none_and_first_positions_below_zero_are_refused(dt):
+    k, table = torch.randn(4, 2, 16, 64, device="cuda").to(DT[dt]), torch.arange(4, dtype=torch.int32, device="cuda").view(1, 4)
+    q, n = torch.randn(1, 4, 1, 64, device="cuda").to(DT[dt]), torch.tensor([64], dtype=torch.int32, device="cuda")
+    whole = ops.paged_attention(q, k, k, table, n, 0.1)
+    for window in (-1, -2 ** 31, 5 - 2 ** 32, 5 - 2 ** 40):
+        assert torch.equal(ops.paged_attention(q, k, k, table, n, 0.1, window=window), whole)
+    for sinks in (-1, 4 - 2 ** 32, 4 - 2 ** 40):
+        with pytest.raises(RuntimeError, match="first positions"):
+            ops.paged_attention(q, k, k, table, n, 0.1, window=5, sinks=sinks)
