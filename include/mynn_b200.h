@@ -556,7 +556,8 @@ int mynn_b200_paged_rotary_append(void *stream, void *q_out, void *k_pages, void
                                   int positions, int dtype);
 /* out [B, S, Hq, D] = softmax(scale * q k^T) v over the cache, q [B, Hq, S, D].  A query at position i sees position j <= i when window <= 0, or
  * i - j < window, or j < sinks (pages that hold no such position may have been given back: their entries are not read).  softcap > 0: scores go through
- * softcap * tanh(. / softcap).  Rows that see nothing are zeros.  D <= 256.  workspace: scratch of mynn_b200_paged_attention_workspace_bytes
+ * softcap * tanh(. / softcap).  Rows that see nothing are zeros.  Keys are taken as they were stored (rotated at their position in the sequence): the streaming
+ * cache, whose keys are rotated at their rank among the cached ones, is mynn_b200_attention_streaming.  D <= 256.  workspace: scratch of mynn_b200_paged_attention_workspace_bytes
  * (of the current device; 0: none is needed; at most 80 MB on 148 SMs, whatever S is), 16-byte aligned; nothing in it outlives the call. */
 size_t mynn_b200_paged_attention_workspace_bytes(int B, int S, int Hq, int Hkv, int D, int page, int table_pages);
 int mynn_b200_paged_attention(void *stream, void *out, const void *q, const void *k_pages, const void *v_pages, const int32_t *block_table,
