@@ -313,8 +313,9 @@ __device__ __forceinline__ uint32_t special_mask(uint32_t x) {  // all ones over
 // of an f16 number end at 2^-24: with the largest weight near the other end of its range, 2^15, 16 bits are left of one 2^22 times as small as that of m (2^-9).  Where a lane has
 // none as large, the tile is multiplied with weights that are 2^up times as large, its own largest near 2^15, by sums that are brought there and back, powers of two that change no
 // bit.  So behind a key that leads by any number of nats, and whose value may be zero, the others keep 16 bits; those that share its tile are right to 2^-38 of
-// the largest.  Tiles that are all so small take longer: behind a first key that leads by 20 nats 131071 positions, 8 kv heads of 128, 123 us instead of 112 (32 sequences of 2048
-// 71 instead of 64; cold caches).  The check itself costs nothing with eight rows of a warp, 1 to 5 % with sixteen (20 rows of 64 numbers over 60000 positions 55 us without).
+// the largest.  Tiles that are all so small take longer: behind a first key that leads by 20 nats 131071 positions, 8 kv heads of 128, 123 us instead of 115 (32 sequences of 2048
+// 73 instead of 66; cold caches).  The check itself costs nothing with eight rows of a warp and heads of up to 128, up to 5 % else (20 rows of 64 numbers over 60000 positions 59.5 us,
+// 56 without).
 template <typename T>
 constexpr int kTop = std::is_same<T, __half>::value ? 13 : 0;
 template <typename T>
@@ -328,7 +329,8 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
     constexpr bool NARROW = kTop<T> != 0;
     constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
     extern __shared__ __align__(128) uint8_t raw[];
-    __shared__ float part_m[W][8 * NT], part_l[W][8 * NT], to_reference[W][8 * NT];
+    __shared__ float part_m[W][8 * NT], part_l[W][8 * NT];
+    __shared__ __align__(8) float to_reference[W][8 * NT];
     pdl_trigger();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, team = warp / RW;
@@ -380,13 +382,11 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
 #pragma unroll
         for (int n = 0; n < NT; n++) at[n][0] = last_seen(8 * n + 2 * t), at[n][1] = last_seen(8 * n + 2 * t + 1);
         auto sees = [&](int last, int j) { return j <= last && (p.window <= 0 || last - j < p.window || j < p.sinks); };
-        auto base_of = [&](int j) { return sp.at(t0 + team + TEAMS * j) * TILE; };
+        auto base_of = [&](int j) { return (int)((unsigned)sp.at(t0 + team + TEAMS * j) * TILE); };  // (behind the last tile it may wrap, and is not used)
         // The first row of eight positions whose rows lie one behind the other and are all seen, for 32 such strips at once, one per lane; -1 for others.
         auto strips_of = [&](int i) {
-            const int j = i / STRIPS;
-            if (j >= mine || !p.strips) return -1;
-            const int pos = base_of(j) + i % STRIPS * 8;
-            if (pos + 8 > sp.rows || (p.window > 0 && oldest - pos >= p.window && pos + 8 > p.sinks)) return -1;
+            const int j = i / STRIPS, pos = base_of(j) + i % STRIPS * 8;
+            if (j >= mine || !p.strips || pos + 8 > sp.rows || (p.window > 0 && oldest - pos >= p.window && pos + 8 > p.sinks)) return -1;
             return paged_row(p, sp, b, h, pos);
         };
         auto row_of = [&](int j) { return j < mine ? paged_row(p, sp, b, h, base_of(j) + (lane & (TILE - 1))) : -1; };
@@ -635,26 +635,27 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
                                 const float up = tops[e] > -INFINITY && ref[n][e] < INFINITY ? fminf(floorf(ref[n][e] + 15.f - tops[e]), 60.f) : 0.f;
 #pragma unroll
                                 for (int k = 0; k < KT; k++) x[n][k][e] += up, x[n][k][2 + e] += up;
+                                const float there = __int_as_float((127 + (int)up) << 23);  // 2^up
+                                l[n][e] *= there;
+#pragma unroll
+                                for (int i = 0; i < KS; i++) o[n][i][e] *= there, o[n][i][2 + e] *= there;
                                 if (g == 0) to_reference[warp][8 * n + 2 * t + e] = __int_as_float((127 - (int)up) << 23);  // 2^-up
                             }
                             __syncwarp();
                         }
                     }
-                    float mass[2] = {0.f, 0.f};  // of this lane's positions
 #pragma unroll
                     for (int k = 0; k < KT; k++) {
 #pragma unroll
                         for (int i = 0; i < 4; i++) x[n][k][i] = exp2_approx(x[n][k][i] - ref[n][i & 1]);
-                        mass[0] += x[n][k][0] + x[n][k][2];
-                        mass[1] += x[n][k][1] + x[n][k][3];
+                        l[n][0] += x[n][k][0] + x[n][k][2];  // of this lane's positions
+                        l[n][1] += x[n][k][1] + x[n][k][3];
 #pragma unroll
                         for (int c = 0; c < 2; c++) {
                             split_pack<T>(x[n][k][2 * c], x[n][k][2 * c + 1], hi[n][k][c], lo[n][k][c]);
                             hi[n][k][c] = transpose_8x8(hi[n][k][c]), lo[n][k][c] = transpose_8x8(lo[n][k][c]);  // positions 16 k + 8 c + 2 t, + 1 of row 8 n + g
                         }
                     }
-                    if (NARROW && (small >> n & 1)) mass[0] *= to_reference[warp][8 * n + 2 * t], mass[1] *= to_reference[warp][8 * n + 2 * t + 1];
-                    l[n][0] += mass[0], l[n][1] += mass[1];
                 }
             };
             if (more_rows) scores(std::integral_constant<int, NT>());
@@ -683,13 +684,6 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
                 const bool special = !NARROW || odd;
 #pragma unroll
                 for (int i = 0; i < KS; i++) {
-                    if constexpr (NARROW && decltype(rare)::value) {
-#pragma unroll
-                        for (int n = 0; n < N; n++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                if (small >> n & 1) o[n][i][e] *= __int_as_float((254 << 23) - __float_as_int(to_reference[warp][8 * n + 2 * t + (e & 1)]));  // 2^up
-                    }
 #pragma unroll
                     for (int k = 0; k < KT; k++) {
                         uint32_t a[4], c[4];
@@ -721,13 +715,16 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
                             }
                         }
                     }
-                    if constexpr (NARROW && decltype(rare)::value) {
+                }
+                if constexpr (NARROW && decltype(rare)::value) {
 #pragma unroll
-                        for (int n = 0; n < N; n++)
+                    for (int n = 0; n < N; n++)
+                        if (small >> n & 1) {
+                            const float2 back = *reinterpret_cast<const float2 *>(&to_reference[warp][8 * n + 2 * t]);
+                            l[n][0] *= back.x, l[n][1] *= back.y;
 #pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                if (small >> n & 1) o[n][i][e] *= to_reference[warp][8 * n + 2 * t + (e & 1)];
-                    }
+                            for (int i = 0; i < KS; i++) o[n][i][0] *= back.x, o[n][i][1] *= back.y, o[n][i][2] *= back.x, o[n][i][3] *= back.y;
+                        }
                 }
             };
             // Values that are no numbers are taken out of the product and added position by position where they are seen, so that the other rows keep their bits.
