@@ -238,6 +238,7 @@ extern "C" int mynn_b200_paged_rotary_append(void *stream, void *q_out, void *k_
         while (lanes < D / 16) lanes *= 2;
         // A step wants each head to begin at once, prompts want many CTAs side by side, since each begins with a chain of loads.  48 heads of 128, bf16, with 64 / 128 / 192 / 512
         // threads: 32 tokens 4.2 / 3.0 / 2.6 / 2.5 us, 512 tokens 6.2 / 5.3 / 4.4 / 4.9, 2048 tokens 9.2 / 8.9 / 10.0 / 15.0, 4662 places that are mostly padding 16 / 12.0 / 10.6 / 14.0.
+        // Places with counts are taken to be mostly padding, since the host does not know them: prompts of one length are better off without counts (8.9 instead of 10.0 us).
         const long long tokens = (long long)B * S;
         const int threads = (int)std::min<long long>(tokens < 300 ? 512 : tokens < 1024 || counts ? 192 : 128, ((long long)(Hq + 2 * Hkv) * lanes + 31) / 32 * 32);
         MYNN_DISPATCH_DTYPE(dtype, T, { MYNN_CUDA_OK(launch_dependent(paged_append_kernel<T>, dim3(S, B), dim3(threads), 0, st, p, lanes)); });

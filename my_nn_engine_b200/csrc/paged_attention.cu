@@ -17,8 +17,9 @@ constexpr int kPlainTile = 8;
 // ---- any sizes ----------------------------------------------------------------------------------------------------------
 // f32 caches, heads that are no multiple of 8 numbers, unaligned tensors.  Each warp takes tiles of 8 positions into shared memory as f32; in the first product
 // a lane has one key and a quarter of the dimensions, in the second the dimensions lane, lane + 32, ...  Small tiles leave room for many warps, which hide each other's
-// chains: with tiles of 16 and half the warps 64 sequences of 1000, 8 heads of 128, took 192 us, with every lane of a key going on with all rows 166, now 127 = 0.64 of the
-// copy bandwidth.  f32 has no tensor-core form that keeps 24 bits, so the instructions around the 2 RB D multiplications of a position bound it.
+// chains: with tiles of 16 and half the warps 64 sequences of 1000, 8 heads of 128, took 192 us, with every lane of a key going on with all rows 166, now 125 = 0.64 of the
+// copy bandwidth with four rows, 92 = 0.87 with one.  Bound by chains: a tile is copies, product, exchange, exponentials and product one behind the other, in eight warps per SM at D = 128 (140 KB
+// of shared memory: one CTA), sixteen up to D = 96, with a third of the issue slots used.  (Products of three bf16 parts per number on the tensor cores would keep 24 bits too; not built.)
 // RB: query rows of a CTA (one head per kv head: with eight rows where one is needed 7 sequences of 1 to 1501, 12 heads of 80, took 46 us).
 // VEC: elements of a copy to shared memory (cp.async, f32); 0: 16-bit elements, converted on the way.
 template <int DL>
@@ -267,11 +268,13 @@ __global__ void __launch_bounds__(kPlainWarps<DL> * 32, PlainShape<DL, RB>::CTAS
 // sums are f32.  The reference of the weights is moved only when a score exceeds it by 2^kLag, so most tiles need no maximum across lanes and no rescaling.  D is padded
 // to DP with zeros, on the chip only.
 // The chain of one tile is long (two products, a softmax) and each warp walks it alone, so warps are what hides it: sixteen per SM with eight query rows each (with eight
-// warps of sixteen rows 96 mixed sequences of heads of 64 took a fifth longer).  From 17 rows on the instructions bound it, and sixteen rows of a warp share the blocks
-// of keys and values and what goes on around the products (20 rows over 131072 positions: 110 us with eight rows per warp, 105 with sixteen).
-// Measured with the joining kernel behind it, 8 kv heads of 128, bf16: 32 sequences of 2048 47 us = 0.87 of the copy bandwidth, one of 131071 91 us = 0.90, 16 of 1500 to
-// 4500 with up to 5 queries of 4 heads 55 us = 0.54, 48 with windows of 1000 over pages of 24 41 us = 0.73, one of 300 7 us; 4 kv heads of 64, f16: 96 of 1 to 6000
-// 56 us = 0.81.  What is left is what a launch costs around its pass: to find its run, the first copies, the last sums and the join take some 8 us.
+// warps of sixteen rows 96 mixed sequences of heads of 64 took a fifth longer).  From 17 rows on sixteen rows of a warp share the blocks of keys and values and what goes on around the
+// products (20 rows over 131072 positions: 110 us with eight rows per warp, 105 with sixteen), and the chain bounds it: eight warps per SM (255 registers), a quarter of the issue slots and of the
+// tensor pipe, stalls that are fixed latencies and a loop that does not fit the instruction cache.  Rows are laid out for the batch's S, so places without a token are worked on as well.
+// Measured per call, with the joining kernel behind it, 8 kv heads of 128, bf16: 32 sequences of 2048 47 us = 0.87 of the copy bandwidth, 16 of 1500 to 4500 with 5 queries of 4
+// heads 56 us = 0.54, with 8 queries 61, with one query in 5 places 56, 48 with windows of 1000 over pages of 24 42 us = 0.72, one of 300 14 us (7 on the device); f16: one of 131071
+// 94 us = 0.87, 4 kv heads of 64, 96 of 1 to 6000 57 us = 0.79.  What is left of one query is what a launch costs around its pass: to find its run, the first copies, the last sums and
+// the join take some 8 us.
 template <int DP, int RW, int NT>
 struct MmaShape {
     static constexpr int W = 8, TEAMS = W / RW, ROWS = 8 * NT * RW;

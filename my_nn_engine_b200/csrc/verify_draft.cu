@@ -7,8 +7,9 @@
 // warp a part of it: sums per warp, then which CTA's and which warp's part the running sum ends in, then that part again, from L2.  A difference of two
 // f32 numbers and sums of 1e5 of them decide on whole numbers, so they are held in 64 bits: a sum in f32 is off by more than many a token's
 // probability.  The order of the sums is fixed.
-// Bound by the chain tokens - probabilities - row - sums - row again for few sequences (one over 32000 tokens: 6.5 us) and by instructions and bytes for many: 64 over
-// 128256 tokens in f32 20 us (66 MB: 0.50 of the copy bandwidth), 200 over 50257 in bf16 17 us.  Converting to 64 bits takes most of it.
+// Bound by the chain tokens - probabilities - row - sums - row again for few sequences (one over 32000 tokens: 6.5 us) and by too little on its way for many: 64 over
+// 128256 tokens in f32 21 us (66 MB: 0.48 of the copy bandwidth), 200 over 50257 in bf16 18 us = 0.17.  45 % of the issue slots are used; warps wait for loads, one step of which is ahead of the sums (in 16
+// bits one 16-byte load per lane), and for the cluster.
 #include <type_traits>
 
 #include "common.cuh"
