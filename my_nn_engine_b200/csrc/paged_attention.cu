@@ -355,8 +355,8 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
     const uint32_t copy_lane = copy_row * (DP * 2) + (copy_piece >> 3) * 128 + paged_swizzle(copy_row, copy_piece & 7) * 16;
     const uint32_t k_lane = ring_at + k_row * (DP * 2) + paged_swizzle(k_row, lane >> 4) * 16, v_lane = ring_at + v_row * (DP * 2) + paged_swizzle(v_row, lane >> 3 & 1) * 16;
     for (int b = cta; b < p.B; b += ctas)  // sequences that see nothing at all are in no CTA's run
-        if (blockIdx.y == 0 && paged_span(p, b).tiles == 0)
-            for (size_t n = (size_t)p.S * p.Hq * D / 8, i = threadIdx.x; i < n; i += W * 32) reinterpret_cast<uint4 *>(p.out)[b * n + i] = make_uint4(0, 0, 0, 0);
+        if (paged_span(p, b).tiles == 0)  // (a share for each block of rows)
+            for (size_t n = (size_t)p.S * p.Hq * D / 8, i = blockIdx.y * (W * 32) + threadIdx.x; i < n; i += (size_t)gridDim.y * (W * 32)) reinterpret_cast<uint4 *>(p.out)[b * n + i] = make_uint4(0, 0, 0, 0);
     auto team_sync = [&]() {
         if constexpr (RW == 1) __syncwarp();
         else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(RW * 32) : "memory");

@@ -688,8 +688,8 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale, counts=Non
     block_table): q [B, Hq, S, D], one query per sequence or a few drafted ones -> [B, S, Hq, D].  With ``window`` a query sees the last ``window`` positions
     up to its own, and the first ``sinks`` ones of the sequence; pages that hold none of these may have been given back.  Keys stay as they were stored, rotated at
     their position in the sequence; ``attention_streaming`` is another thing, its first tokens and ring are rotated at their rank in the cache.  softcap: cap on the
-    scores (0: none).  A query that sees nothing (an idle sequence, a place without a token) gives zeros; keys and values that are not finite matter to those queries only that see
-    them, whose outputs they make infinite or NaN."""
+    scores (0: none).  A query that sees nothing (an idle sequence, a place without a token) gives zeros.  Keys and values that are not finite matter to those queries only that
+    see them; an infinite value may come out as NaN."""
     B, Hq, S, D = q.shape
     n, G, page, head, width = _pages(k_pages, v_pages, q.dtype, block_table, lengths, counts, B)
     if head != D:

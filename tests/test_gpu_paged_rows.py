@@ -57,3 +57,19 @@ def test_windows_below_32_bits_are_none_and_first_positions_below_zero_are_refus
     for sinks in (-1, 4 - 2 ** 32, 4 - 2 ** 40):
         with pytest.raises(RuntimeError, match="first positions"):
             ops.paged_attention(q, k, k, table, n, 0.1, window=5, sinks=sinks)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("width", [100, 3])
+def test_idle_sequences_among_prompts_are_zeros(dt, width):
+    """Fewer CTAs than sequences, several blocks of rows: every element of an idle sequence is written by one of them."""
+    B, S, H, G, D = 40, 700, 4, 1, 64
+    counts = [S if b == 7 else 0 for b in range(B)]
+    k = torch.randn(50, G, 16, D, device="cuda").to(DT[dt])
+    table = torch.full((B, width), -1, dtype=torch.int32, device="cuda")
+    table[7, :min(width, 44)] = torch.arange(min(width, 44), dtype=torch.int32, device="cuda")
+    q = torch.randn(B, H, S, D, device="cuda").to(DT[dt])
+    n, c = torch.full((B,), 700, dtype=torch.int32, device="cuda"), torch.tensor(counts, dtype=torch.int32, device="cuda")
+    out = torch.full((B, S, H, D), float("nan"), device="cuda", dtype=DT[dt])
+    ops.paged_attention(q, k, k, table, n, 0.1, counts=c, out=out)
+    assert torch.isfinite(out).all() and out[7].any() and not out[:7].any() and not out[8:].any()
