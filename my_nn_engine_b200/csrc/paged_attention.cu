@@ -316,8 +316,8 @@ __device__ __forceinline__ uint32_t special_mask(uint32_t x) {  // all ones over
 // of an f16 number end at 2^-24: with the largest weight near the other end of its range, 2^15, 16 bits are left of one 2^22 times as small as that of m (2^-9).  Where a lane has
 // none as large, the tile is multiplied with weights that are 2^up times as large, its own largest near 2^15, by sums that are brought there and back, powers of two that change no
 // bit.  So behind a key that leads by any number of nats, and whose value may be zero, the others keep 16 bits; those that share its tile are right to 2^-38 of
-// the largest.  Tiles that are all so small take longer: behind a first key that leads by 20 nats 131071 positions, 8 kv heads of 128, 123 us instead of 115 (32 sequences of 2048
-// 73 instead of 66; cold caches).  The check itself costs nothing with eight rows of a warp and heads of up to 128, up to 5 % else (20 rows of 64 numbers over 60000 positions 59.5 us,
+// the largest.  Tiles that are all so small take longer: behind a first key that leads by 20 nats 131071 positions, 8 kv heads of 128, 119 us instead of 113 (32 sequences of 2048
+// 75 instead of 67; cold caches).  The check itself costs nothing with eight rows of a warp and heads of up to 128, up to 5 % else (20 rows of 64 numbers over 60000 positions 59.5 us,
 // 56 without).
 template <typename T>
 constexpr int kTop = std::is_same<T, __half>::value ? 13 : 0;
@@ -621,7 +621,8 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
                             float top = most[e];
 #pragma unroll
                             for (int s = 4; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-                            const float now = fmaxf(m[n][e], top), keep = exp2_approx(m[n][e] - merge_reference(now));
+                            // (only of rows that exceed it: what a row gives does not hang on the rows beside it)
+                            const float now = top > limit[n][e] ? top : m[n][e], keep = exp2_approx(m[n][e] - merge_reference(now));
                             m[n][e] = now;
                             ref[n][e] = merge_reference(now) - kTop<T>;
                             limit[n][e] = now + kLag<T>;
@@ -635,7 +636,8 @@ __global__ void __launch_bounds__(256, MmaShape<DP, RW, NT>::CTAS) paged_attenti
 #pragma unroll
                             for (int e = 0; e < 2; e++) {
                                 // brings the tile's largest weight to 2^14 .. 2^15 (or 2^60 times nearer: the sums have to stay numbers)
-                                const float up = tops[e] > -INFINITY && ref[n][e] < INFINITY ? fminf(floorf(ref[n][e] + 15.f - tops[e]), 60.f) : 0.f;
+                                const bool own = (__ballot_sync(0xffffffffu, below(e)) & 0x11111111u << t) != 0u;  // (the row's lanes)
+                                const float up = own ? fminf(floorf(ref[n][e] + 15.f - tops[e]), 60.f) : 0.f;
 #pragma unroll
                                 for (int k = 0; k < KT; k++) x[n][k][e] += up, x[n][k][2 + e] += up;
                                 const float there = __int_as_float((127 + (int)up) << 23);  // 2^up

@@ -73,3 +73,22 @@ def test_idle_sequences_among_prompts_are_zeros(dt, width):
     out = torch.full((B, S, H, D), float("nan"), device="cuda", dtype=DT[dt])
     ops.paged_attention(q, k, k, table, n, 0.1, counts=c, out=out)
     assert torch.isfinite(out).all() and out[7].any() and not out[:7].any() and not out[8:].any()
+
+
+@pytest.mark.parametrize("dt,D,group", [("f16", 128, 4), ("bf16", 64, 2), ("f16", 64, 8), ("f32", 64, 4)])
+@pytest.mark.parametrize("scale", [0.1, 0.6])
+def test_other_queries_leave_a_query_its_bits(dt, D, group, scale):
+    """Keys that only the last query sees, infinite or so large that its weights are all but one, over many batches: the first queries' outputs do not change by a bit."""
+    g = torch.Generator("cuda").manual_seed(D)
+    B, G, S, n = 48, 2, 4, 130
+    table = torch.randperm(B * 9, generator=g, device="cuda").int().view(B, 9)
+    lengths = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    for _ in range(4):
+        k, v = (torch.randn(B * 9, G, 16, D, generator=g, device="cuda").to(DT[dt]) for _ in range(2))
+        q = torch.randn(B, G * group, S, D, generator=g, device="cuda").to(DT[dt])
+        q[..., 0] = 1.0
+        clean = ops.paged_attention(q, k, v, table, lengths, scale)
+        for bad in (float("inf"), float("nan"), 300.0, -300.0):
+            k2 = k.clone()
+            k2[table[:, (n - 1) // 16].long(), :, (n - 1) % 16, 0] = bad
+            assert torch.equal(ops.paged_attention(q, k2, v, table, lengths, scale)[:, :S - 1], clean[:, :S - 1])
